@@ -40,7 +40,8 @@ enum {
 };
 
 /* Device element types (KernelBuffer::dtype subset). */
-enum { MLKHIP_F32 = 0, MLKHIP_F16 = 1, MLKHIP_F64 = 2 };
+/* MLKHIP_BF16 and MLKHIP_I32 are the operators' (see below). */
+enum { MLKHIP_F32 = 0, MLKHIP_F16 = 1, MLKHIP_F64 = 2, MLKHIP_BF16 = 3, MLKHIP_I32 = 4 };
 
 typedef struct mlkhip_artifact mlkhip_artifact;
 
@@ -48,7 +49,7 @@ typedef struct mlkhip_artifact mlkhip_artifact;
 typedef struct mlkhip_binding {
     void* ptr;          /* device address; NULL for a temp lets the artifact own it */
     int64_t elements;   /* capacity in elements */
-    int32_t dtype;      /* MLKHIP_F32 / MLKHIP_F16 / MLKHIP_F64, must equal the module's */
+    int32_t dtype;      /* one of the above, must equal the module's */
     int32_t pad;
 } mlkhip_binding;
 
@@ -203,6 +204,57 @@ int mlkhip_time_device(const mlkhip_artifact* a, const mlkhip_binding* binds, in
 int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* binds, int n_binds,
                             const double* scalars, int64_t n_scalars, int64_t elements, void* stream,
                             int warmup, int reps, float* avg_ms);
+
+/* ---- operators -------------------------------------------------------- */
+/* No counterpart in the reference: Call nodes that name one of the operators
+ * below in "math", their buffers in "operands" ({"q": 0, ...}, ids) and their
+ * options in "attrs" ({"heads": 32, ...}, numbers). Every entry of this
+ * header takes such a module as it takes the others. An operand is an input
+ * or output buffer with dims (not a temp). One that holds rows of heads has
+ * its rows along its first dim and `heads` (k, v and their outputs:
+ * `kv_heads`) heads of `dim` <= 256 elements in each row from column
+ * "<operand>_at" (0) on, so that q, k and v may be columns of one buffer.
+ * Rows are f16, bf16 or f32, all of one Call alike; offsets, lengths,
+ * positions and slots are i32 in device memory and may change from run to
+ * run. An output shares no elements with another operand, except where noted.
+ * What a Call may not hold is refused at build with a message that names it.
+ *
+ * qk_norm_rope (operands q, k, q_out, k_out; v with v_out; q_weight with
+ * k_weight; positions; slots; q_offsets. attrs heads, kv_heads, dim, eps
+ * (1e-6), theta (10000), rot (dim), interleaved (0), section_0..2): each head
+ * of q and k is x / sqrt(mean(x^2) + eps) * weight (unchanged without
+ * weights, which are f32 or of q's type), then its first `rot` elements turn
+ * in pairs (i, i + rot/2), or (2i, 2i+1) if interleaved, by the angle
+ * positions[axis, t] * theta^(-2i/rot); the first section_0 pairs take axis
+ * 0, the next section_1 axis 1, the last section_2 axis 2. Angles are reduced
+ * in f64. k_out and v_out hold token t in row slots[t], or in row t without
+ * slots; a slot outside the rows stores nothing, and slots that name a row
+ * twice leave one of its tokens there. With q_offsets (i32 [n + 1], n
+ * sequences) the tokens from its last element on are left alone. q_out may
+ * take q's place, and without slots k_out k's and v_out v's.
+ *
+ * attention (operands q, k, v, q_offsets, out; kv_start with kv_len; lse.
+ * attrs heads, kv_heads, dim, scale (1/sqrt(dim)), causal (1)): out =
+ * softmax(scale q k^T) v. Sequence b has the query rows q_offsets[b] ..
+ * q_offsets[b + 1] and the keys and values of rows kv_start[b] .. kv_start[b]
+ * + kv_len[b] (without the two arrays the rows of its queries); query head h
+ * reads head h / (heads / kv_heads) of them. Causal: query i of n sees the
+ * keys j <= i + kv_len - n. What a query does not see, or lies behind the
+ * keys, does not reach its result, whatever its bits. A query without keys,
+ * or with -inf scores alone, gets zeros and an lse of -inf. lse (f32 [rows,
+ * heads]) is the log of the sum of exp(scale q k^T). Rows behind the last
+ * sequence are left alone; offsets and lengths are clipped to the buffers.
+ *
+ * shared_prefix_attention (attention's operands, prefix_k, prefix_v;
+ * prefix_len): every sequence's keys follow prefix_k and prefix_v rows 0 ..
+ * prefix_len[0] (all rows without it), which every query sees. Where the
+ * sequences have few queries each, all of them read the prefix together.
+ *
+ * Attention's workspace (partial results of key ranges, where there are too
+ * few queries to fill the chip) is the artifact's, one per stream, as for the
+ * other steps; the allocation-free entry takes it from its array when it
+ * fits. Without it (an artifact first run under capture) the Call runs in one
+ * range. */
 
 /* ---- launch-form search (fastkernel on the gfx950 kernels) ------------ */
 /* The reference's fastkernel search (fastkernel/include/mlk/fastkernel/

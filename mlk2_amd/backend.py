@@ -24,9 +24,28 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("MLK_HIP_LIB") or os.path.join(HERE, "lib", "libmlk_hip.so")
 
 OK, NEG_STORE, RUNTIME, LAUNCH, NO_DEVICE, BAD_BINDING, REFUSED = 0, 1, 2, 3, 4, 6, 7
-F32, F16, F64 = 0, 1, 2
-DTYPE_CODE = {"f32": F32, "f16": F16, "f64": F64}
-NP_OF_CODE = {F32: np.float32, F16: np.float16, F64: np.float64}
+F32, F16, F64, BF16, I32 = 0, 1, 2, 3, 4
+DTYPE_CODE = {"f32": F32, "f16": F16, "f64": F64, "bf16": BF16, "i32": I32}
+# numpy has no bfloat16: its device elements are their 16 bits here.
+NP_OF_CODE = {F32: np.float32, F16: np.float16, F64: np.float64, BF16: np.uint16, I32: np.int32}
+
+
+def bf16_bits(a) -> np.ndarray:
+    """The bfloat16 bits of values, each rounded once, to the nearest even."""
+    d = np.asarray(a, dtype=np.float64)
+    with np.errstate(over="ignore"):
+        f = d.astype(np.float32)
+    u = f.view(np.uint32).astype(np.int64)
+    # Round to odd in f32, so that the second rounding sees what the first dropped.
+    inexact = np.isfinite(f) & (f.astype(np.float64) != d)
+    u = np.where(inexact, (u - (np.abs(f.astype(np.float64)) > np.abs(d))) | 1, u)
+    bits = (u + 0x7FFF + ((u >> 16) & 1)) >> 16
+    return np.where(np.isnan(d), 0x7FC0, bits).astype(np.uint16)
+
+
+def bf16_values(bits) -> np.ndarray:
+    """The f32 values of bfloat16 bits."""
+    return (np.asarray(bits, dtype=np.uint16).astype(np.uint32) << 16).view(np.float32)
 
 _PD = ctypes.POINTER(ctypes.c_double)
 
@@ -244,7 +263,8 @@ class DeviceBuffer:
 
     @classmethod
     def from_array(cls, a: np.ndarray, dtype: str) -> "DeviceBuffer":
-        host = np.ascontiguousarray(np.asarray(a).astype(NP_OF_CODE[DTYPE_CODE[dtype]]).reshape(-1))
+        host = bf16_bits(a) if dtype == "bf16" else np.asarray(a).astype(NP_OF_CODE[DTYPE_CODE[dtype]])
+        host = np.ascontiguousarray(host.reshape(-1))
         buf = cls(host.size, dtype)
         if host.size:
             _check(lib().mlkhip_memcpy_h2d(buf.ptr, host.ctypes.data, buf.nbytes))
@@ -257,7 +277,7 @@ class DeviceBuffer:
         out = np.empty(self.elements, dtype=NP_OF_CODE[self.code])
         if self.elements:
             _check(lib().mlkhip_memcpy_d2h(out.ctypes.data, self.ptr, self.nbytes))
-        return out
+        return bf16_values(out) if self.code == BF16 else out
 
     def binding(self) -> Binding:
         return Binding(self.ptr, self.elements, self.code, 0)

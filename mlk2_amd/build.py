@@ -29,9 +29,10 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 CLANG = os.path.join(ROCM, "llvm", "bin", "clang++")
 
-DEVICE_SOURCES = ["runtime.hip", "jit.hip", "softmax.hip", "gemm.hip", "gemm_general.hip", "score_softmax.hip", "probe.hip"]
-HOST_SOURCES = ["kernel_ir.cpp", "planner.cpp", "codegen.cpp", "nestgen.cpp", "canonical.cpp", "driver.cpp", "tune.cpp",
-                "artifact.cpp"]
+DEVICE_SOURCES = ["runtime.hip", "jit.hip", "softmax.hip", "gemm.hip", "gemm_general.hip", "score_softmax.hip", "attention.hip",
+                  "norm_rope.hip", "probe.hip"]
+HOST_SOURCES = ["kernel_ir.cpp", "planner.cpp", "codegen.cpp", "nestgen.cpp", "canonical.cpp", "operators.cpp", "driver.cpp",
+                "tune.cpp", "artifact.cpp"]
 
 HIP_FLAGS = [f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
              "-Wall", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

@@ -130,6 +130,16 @@ int mlkd_score_ranges(const mlkd_score_softmax* p);
 /// two-pass query-stationary).
 void mlkd_score_set_variant(int variant);
 
+int mlkd_launch_norm_rope(const mlkd_norm_rope* p, void* stream);
+const char* mlkd_norm_rope_kernel_name(const mlkd_norm_rope* p);
+int mlkd_launch_attention(const mlkd_attention* p, void* stream);
+/// Workspace bytes for the partial results of key ranges (0: the shape is run
+/// in one range); without it the operator runs in one range.
+int64_t mlkd_attention_work_bytes(const mlkd_attention* p);
+/// The kernels mlkd_launch_attention runs for `p`, joined by '+' (valid until
+/// this thread's next call).
+const char* mlkd_attention_kernel_names(const mlkd_attention* p);
+
 /// Measured HBM bandwidth (streaming copy of 256 MiB) and f16 MFMA
 /// throughput (register-only MFMAs, one wave per SIMD) of the current
 /// device, timed on `stream` (probe.hip).

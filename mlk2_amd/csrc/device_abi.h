@@ -11,7 +11,8 @@ extern "C" {
 
 /// Element types a device buffer may hold (KernelBuffer::dtype subset,
 /// compiler/include/mlk/type/domain.h:53-60).
-enum mlkd_dtype { MLKD_F32 = 0, MLKD_F16 = 1, MLKD_F64 = 2 };
+/// BF16 and I32 are the operators' (mlkd_norm_rope, mlkd_attention).
+enum mlkd_dtype { MLKD_F32 = 0, MLKD_F16 = 1, MLKD_F64 = 2, MLKD_BF16 = 3, MLKD_I32 = 4 };
 
 /// Runtime scalar parameters of a chain (ScalarParam operands,
 /// kernel_ir.h:58-70); indices past the bound table read 0.0 like the
@@ -79,6 +80,50 @@ typedef struct mlkd_score_softmax {
     void* work;
     int64_t work_bytes;
 } mlkd_score_softmax;
+
+/// Head norms and position rotation of q and k, and k's and v's rows of a
+/// cache. Row t of q, k, v: heads (kv_heads) heads of dim elements; strides
+/// are elements from row to row. y = x / sqrt(mean x^2 + eps) * weight (no
+/// weight: y = x), then the pairs of the first `rot` elements turned by
+/// positions[axis, t] * theta^(-2 i / rot). Tokens t < tokens and, with
+/// q_offsets, below q_offsets[sequences].
+typedef struct mlkd_norm_rope {
+    const void *q, *k, *v;               /* v may be NULL */
+    void *q_out, *k_out, *v_out;
+    const void *q_weight, *k_weight;     /* both or none */
+    const int32_t* positions;            /* [axes, tokens], or NULL: no rotation */
+    const int32_t* slots;                /* row of k_out and v_out, or NULL: row t */
+    const int32_t* q_offsets;            /* [sequences + 1], or NULL */
+    int32_t dtype, weight_dtype;
+    int32_t heads, kv_heads, dim, rot;
+    int32_t interleaved, axes, sequences, pad;
+    int32_t section_end[3], pad2;        /* frequency pairs below which axis 0, 1, 2 applies */
+    int64_t tokens, out_rows;            /* rows of q, k, v; rows of k_out and v_out */
+    int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride, v_out_stride;
+    double eps;
+    const double* quarters;              /* host memory: theta^(-2 i / rot) in quarter turns, rot / 2 of them */
+} mlkd_norm_rope;
+
+/// out = softmax(scale q k^T) v over packed sequences, and lse, the log of
+/// each row's sum. Sequence b has query rows q_offsets[b] .. q_offsets[b + 1]
+/// and keys kv_start[b] .. kv_start[b] + kv_len[b] (no arrays: its query rows);
+/// with `prefix_k` every sequence's keys follow prefix rows 0 .. prefix_len.
+/// Causal: query i of n sees own keys j <= i + kv_len - n. Lengths are clipped
+/// to the buffers.
+typedef struct mlkd_attention {
+    const void *q, *k, *v, *prefix_k, *prefix_v;
+    void* out;
+    float* lse;                          /* [q_rows, heads], or NULL */
+    const int32_t *q_offsets, *kv_start, *kv_len;
+    const int32_t* prefix_len;           /* [1], or NULL: prefix_rows */
+    int32_t dtype, causal;
+    int32_t heads, kv_heads, dim, sequences;
+    int64_t q_rows, kv_rows, prefix_rows;
+    int64_t q_stride, k_stride, v_stride, prefix_k_stride, prefix_v_stride, out_stride;
+    double scale;
+    void* work;                          /* mlkd_attention_work_bytes, or NULL: no key ranges */
+    int64_t work_bytes;
+} mlkd_attention;
 
 #ifdef __cplusplus
 }

@@ -47,6 +47,11 @@ std::vector<bool> storedBuffers(const KernelModule& km) {
         if ((n.op == KernelOp::Store || n.op == KernelOp::Call) && n.bufferOut < km.buffers.size()) {
             w[n.bufferOut] = true;
         }
+        if (!isOperatorCall(n)) continue;
+        for (const auto& [name, b] : n.operands) {   // outputs by their names
+            const bool out = name == "out" || name == "lse" || name == "q_out" || name == "k_out" || name == "v_out";
+            if (out && b < km.buffers.size()) w[b] = true;
+        }
     }
     return w;
 }

@@ -19,7 +19,15 @@ namespace mlk::hip {
 
 namespace {
 
-int dtypeCode(Dtype d) { return d == Dtype::F32 ? MLKD_F32 : (d == Dtype::F16 ? MLKD_F16 : MLKD_F64); }
+int dtypeCode(Dtype d) {
+    switch (d) {
+        case Dtype::F32: return MLKD_F32;
+        case Dtype::F16: return MLKD_F16;
+        case Dtype::BF16: return MLKD_BF16;
+        case Dtype::I32: return MLKD_I32;
+        default: return MLKD_F64;
+    }
+}
 
 unsigned gridFor(int64_t threads, int64_t perGroup = 256) {
     int64_t blocks = (threads + perGroup - 1) / perGroup;
@@ -36,6 +44,29 @@ uint16_t toHalfBits(double d) {
     uint16_t bits = 0;
     std::memcpy(&bits, &h, sizeof(bits));
     return bits;
+}
+
+/// f64 -> bf16 bits with one rounding (round to nearest even): through f32
+/// rounded to odd, whose 16 extra bits keep what decides the tie.
+uint16_t toBf16Bits(double d) {
+    float f = static_cast<float>(d);
+    uint32_t u = 0;
+    std::memcpy(&u, &f, sizeof(u));
+    if (d != d) return static_cast<uint16_t>((u >> 16) | 0x40u);
+    // A double past f32's range, and past bf16's, is an infinity either way.
+    if (!std::isinf(f) && static_cast<double>(f) != d) {
+        if (std::fabs(static_cast<double>(f)) > std::fabs(d)) --u;   // toward zero
+        u |= 1u;
+    }
+    return static_cast<uint16_t>((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+
+/// f64 -> i32, rounded toward zero and clipped; NaN is 0.
+int32_t toInt32(double d) {
+    if (d != d) return 0;
+    if (d <= -2147483648.0) return INT32_MIN;
+    if (d >= 2147483647.0) return INT32_MAX;
+    return static_cast<int32_t>(d);
 }
 
 double fromHalfBits(uint16_t bits) {
@@ -88,7 +119,7 @@ void parallelRange(int64_t n, const F& fn) {
 }
 
 /// The caller's f64 values [0, cnt) as `dt` elements at `out` (one rounding
-/// to nearest even for f32 and f16).
+/// to nearest even for f32, f16 and bf16).
 void narrowTo(void* out, const double* src, int64_t cnt, Dtype dt) {
     if (dt == Dtype::F64) {
         double* o = static_cast<double*>(out);
@@ -99,6 +130,16 @@ void narrowTo(void* out, const double* src, int64_t cnt, Dtype dt) {
         float* o = static_cast<float*>(out);
         parallelRange(cnt, [&](int64_t b, int64_t e) {
             for (int64_t x = b; x < e; ++x) o[x] = static_cast<float>(src[x]);
+        });
+    } else if (dt == Dtype::BF16) {
+        uint16_t* o = static_cast<uint16_t*>(out);
+        parallelRange(cnt, [&](int64_t b, int64_t e) {
+            for (int64_t x = b; x < e; ++x) o[x] = toBf16Bits(src[x]);
+        });
+    } else if (dt == Dtype::I32) {
+        int32_t* o = static_cast<int32_t*>(out);
+        parallelRange(cnt, [&](int64_t b, int64_t e) {
+            for (int64_t x = b; x < e; ++x) o[x] = toInt32(src[x]);
         });
     } else {
         uint16_t* o = static_cast<uint16_t*>(out);
@@ -119,6 +160,21 @@ void widenFrom(double* dst, const void* in, int64_t cnt, Dtype dt) {
         const float* s = static_cast<const float*>(in);
         parallelRange(cnt, [&](int64_t b, int64_t e) {
             for (int64_t x = b; x < e; ++x) dst[x] = static_cast<double>(s[x]);
+        });
+    } else if (dt == Dtype::BF16) {
+        const uint16_t* s = static_cast<const uint16_t*>(in);
+        parallelRange(cnt, [&](int64_t b, int64_t e) {
+            for (int64_t x = b; x < e; ++x) {
+                const uint32_t u = static_cast<uint32_t>(s[x]) << 16;
+                float f;
+                std::memcpy(&f, &u, sizeof(f));
+                dst[x] = f;
+            }
+        });
+    } else if (dt == Dtype::I32) {
+        const int32_t* s = static_cast<const int32_t*>(in);
+        parallelRange(cnt, [&](int64_t b, int64_t e) {
+            for (int64_t x = b; x < e; ++x) dst[x] = s[x];
         });
     } else {
         const uint16_t* s = static_cast<const uint16_t*>(in);
@@ -177,6 +233,11 @@ Result<std::unique_ptr<HipLoadedKernel>> buildHipKernelArtifact(const KernelModu
         for (const uint32_t b : st.nestBufs) {
             if (b >= km.buffers.size() || k->bindIndex_[b] < 0) {
                 return err(ErrorCode::InvalidGraph, "loop-nest buffer is not bindable");
+            }
+        }
+        for (const Operand& o : st.oper.op) {
+            if (o.buffer != kInvalidId && k->bindIndex_[o.buffer] < 0) {
+                return err(ErrorCode::InvalidGraph, "operator operand is not bindable");
             }
         }
     }
@@ -389,6 +450,18 @@ const char* HipLoadedKernel::stepKernelName(size_t si) const {
                 p.work_bytes = need;
             }
             name = mlkd_score_kernel_names(&p);
+        } else if (st.kind == StepKind::NormRope) {
+            mlkd_norm_rope p;
+            fillNormRope(km_, st, ptr, p);
+            name = mlkd_norm_rope_kernel_name(&p);
+        } else if (st.kind == StepKind::Attention) {
+            mlkd_attention p;
+            fillAttention(km_, st, ptr, p);
+            if (const int64_t need = mlkd_attention_work_bytes(&p); need > 0) {
+                p.work = ptr[0];   // runDevice gives such a step its workspace
+                p.work_bytes = need;
+            }
+            name = mlkd_attention_kernel_names(&p);
         }
     }
     std::lock_guard<std::mutex> g(scratchLock_);
@@ -466,7 +539,8 @@ int HipLoadedKernel::arenaLayout(const DeviceBinding* binds, int64_t elements, c
         return MLKHIP_REFUSED;
     }
     // Workspaces a step can do without (aligned copies of a GEMM's operands
-    // or the sums of its K ranges, score-softmax statistics) take the room that
+    // or the sums of its K ranges, score-softmax statistics, the results of
+    // attention's key ranges) take the room that
     // is left, in step order; a step whose workspace does
     // not fit runs on the kernels that need none.
     padOff.assign(plan_.steps.size(), SIZE_MAX);
@@ -481,6 +555,10 @@ int HipLoadedKernel::arenaLayout(const DeviceBinding* binds, int64_t elements, c
             mlkd_score_softmax p;
             fillScoreParams(st, ptr, p);
             pad = mlkd_score_pad_bytes(&p);
+        } else if (st.kind == StepKind::Attention) {
+            mlkd_attention p;
+            fillAttention(km_, st, ptr, p);
+            pad = mlkd_attention_work_bytes(&p);
         }
         if (pad > 0 && align256(static_cast<size_t>(pad)) <= arena.bytes - used) {
             padOff[si] = used;
@@ -718,6 +796,26 @@ int HipLoadedKernel::runDevice(const DeviceBinding* binds, int n, const double* 
                 rc = mlkd_launch_score_softmax(&p, stream);
                 break;
             }
+            case StepKind::NormRope: {
+                mlkd_norm_rope p;
+                fillNormRope(km_, st, ptr, p);
+                rc = mlkd_launch_norm_rope(&p, stream);
+                break;
+            }
+            case StepKind::Attention: {
+                mlkd_attention p;
+                fillAttention(km_, st, ptr, p);
+                // Without the workspace the step runs in one key range.
+                const int64_t need = mlkd_attention_work_bytes(&p);
+                if (need > 0 && arena != nullptr && padOff[si] != SIZE_MAX) {
+                    p.work = arena->base + padOff[si];
+                    p.work_bytes = need;
+                } else if (need > 0 && arena == nullptr) {
+                    p.work_bytes = stepScratch(*rs, si, 0, need, stream, &p.work);
+                }
+                rc = mlkd_launch_attention(&p, stream);
+                break;
+            }
         }
         if (rc != 0) {
             why = std::string("launch failed: ") + mlkd_rt_last_error();
@@ -830,6 +928,9 @@ int HipLoadedKernel::runHost(double* const* ptrs, int n, const double* scalars, 
         }
         for (const uint32_t b : st.nestWrites) {
             if (b < written.size()) written[b] = true;
+        }
+        for (int i = kFirstOpOutput; i < kOperandSlots; ++i) {
+            if (st.oper.op[i].buffer != kInvalidId) written[st.oper.op[i].buffer] = true;
         }
     }
     std::vector<DeviceBinding> binds(bindables_.size());
@@ -1014,7 +1115,7 @@ int mlkhip_bindable_info(const mlkhip_artifact* a, int i, int32_t* dtype, int64_
                          int* is_output, int* is_temp) {
     if (a == nullptr || i < 0 || static_cast<size_t>(i) >= a->k->bindables().size()) return MLKHIP_BAD_BINDING;
     const mlk::hip::KernelBuffer& b = a->k->module().buffers[a->k->bindables()[static_cast<size_t>(i)]];
-    if (dtype) *dtype = b.dtype == mlk::hip::Dtype::F32 ? MLKHIP_F32 : (b.dtype == mlk::hip::Dtype::F16 ? MLKHIP_F16 : MLKHIP_F64);
+    if (dtype) *dtype = mlk::hip::dtypeCode(b.dtype);
     if (elements) *elements = mlk::hip::bufferElements(b, -1);
     if (is_input) *is_input = b.isInput ? 1 : 0;
     if (is_output) *is_output = b.isOutput ? 1 : 0;

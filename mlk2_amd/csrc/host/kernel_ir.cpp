@@ -204,7 +204,9 @@ MathOp mathFromName(const std::string& s) {
                   {"cos", MathOp::Cos},   {"tan", MathOp::Tan},     {"tanh", MathOp::Tanh},
                   {"sqrt", MathOp::Sqrt}, {"rsqrt", MathOp::Rsqrt}, {"erf", MathOp::Erf},
                   {"gelu", MathOp::Gelu}, {"matmul", MathOp::MatMul},
-                  {"reduce_sum", MathOp::ReduceSum}, {"softmax", MathOp::Softmax}};
+                  {"reduce_sum", MathOp::ReduceSum}, {"softmax", MathOp::Softmax},
+                  {"qk_norm_rope", MathOp::QkNormRope}, {"attention", MathOp::Attention},
+                  {"shared_prefix_attention", MathOp::SharedPrefixAttention}};
     for (const auto& e : kNames) {
         if (s == e.name) return e.op;
     }
@@ -233,6 +235,8 @@ Dtype dtypeFromName(const std::string& s) {
     if (s == "f32") return Dtype::F32;
     if (s == "f16") return Dtype::F16;
     if (s == "f64") return Dtype::F64;
+    if (s == "bf16") return Dtype::BF16;
+    if (s == "i32") return Dtype::I32;
     return Dtype::Other;
 }
 
@@ -375,6 +379,18 @@ Result<KernelModule> parseKernelModule(const char* text, size_t len) {
         for (const int64_t c : d.ints(rd.member(n, "children"))) {
             kn.children.push_back(static_cast<uint32_t>(c));
         }
+        const uint32_t ops = rd.member(n, "operands");
+        if (ops != kInvalidId && rd.at(ops).type == JNode::Object) {
+            for (const uint32_t m : rd.at(ops).items) {
+                kn.operands.emplace_back(rd.at(m).text, static_cast<uint32_t>(d.integer(rd.at(m).items[0], -1)));
+            }
+        }
+        const uint32_t attrs = rd.member(n, "attrs");
+        if (attrs != kInvalidId && rd.at(attrs).type == JNode::Object) {
+            for (const uint32_t m : rd.at(attrs).items) {
+                kn.attrs.emplace_back(rd.at(m).text, d.number(rd.at(m).items[0], NAN));
+            }
+        }
         if (kn.op == KernelOp::Call && mathAbsent) callMath.push_back(static_cast<uint32_t>(km.nodes.size()));
         km.nodes.push_back(std::move(kn));
     }
@@ -437,6 +453,8 @@ int dtypeBytes(Dtype d) {
         case Dtype::F32: return 4;
         case Dtype::F16: return 2;
         case Dtype::F64: return 8;
+        case Dtype::BF16: return 2;
+        case Dtype::I32: return 4;
         case Dtype::Other: return 0;
     }
     return 0;
@@ -445,8 +463,14 @@ int dtypeBytes(Dtype d) {
 const char* mathOpName(MathOp op) {
     static const char* kNames[] = {"add", "sub", "mul", "div", "neg", "pow", "exp", "log",
                                    "sin", "cos", "tan", "tanh", "sqrt", "rsqrt", "erf", "gelu",
-                                   "matmul", "reduce_sum", "softmax", "?"};
+                                   "matmul", "reduce_sum", "softmax", "?",
+                                   "qk_norm_rope", "attention", "shared_prefix_attention"};
     return kNames[static_cast<int>(op)];
+}
+
+bool isOperatorCall(const KernelNode& n) {
+    return n.op == KernelOp::Call && (n.math == MathOp::QkNormRope || n.math == MathOp::Attention ||
+                                      n.math == MathOp::SharedPrefixAttention);
 }
 
 bool isUnaryMath(MathOp op) {
@@ -520,6 +544,12 @@ uint64_t moduleHash(const KernelModule& km) {
         }
         for (const uint32_t c : n.children) h = mix(h, c);
         h = mix(h, n.children.size());
+        for (const auto& [name, id] : n.operands) h = mix(mixStr(h, name), id);
+        for (const auto& [name, value] : n.attrs) {
+            uint64_t bits = 0;
+            std::memcpy(&bits, &value, sizeof(bits));
+            h = mix(mixStr(h, name), bits);
+        }
     }
     for (const auto& kv : km.schedule) {
         h = mixStr(h, kv.first);

@@ -23,11 +23,14 @@ enum class KernelOp : uint8_t { Loop, Compute, Load, Store, AllocBuffer, CopyBuf
 /// MathOp subset the Kernel IR carries (compiler/include/mlk/ir/math_op.h:18-79).
 enum class MathOp : uint8_t {
     Add, Sub, Mul, Div, Neg, Pow, Exp, Log, Sin, Cos, Tan, Tanh, Sqrt, Rsqrt, Erf, Gelu,
-    MatMul, ReduceSum, Softmax, Other
+    MatMul, ReduceSum, Softmax, Other,
+    // Operators of this backend (Call nodes with named operands and attributes).
+    QkNormRope, Attention, SharedPrefixAttention
 };
 
 enum class AccumMode : uint8_t { None, Add, Max };
-enum class Dtype : uint8_t { F32, F16, F64, Other };
+/// BF16 and I32 buffers are read and written by operator Calls only.
+enum class Dtype : uint8_t { F32, F16, F64, Other, BF16, I32 };
 
 struct KernelOperand {
     enum class Kind : uint8_t { Const, ElemA, ElemB, ScalarParam, Temp, ElemIdx };
@@ -67,6 +70,9 @@ struct KernelNode {
     std::string family;
     std::vector<KernelExpr> exprs;
     std::vector<uint32_t> children;
+    /// Operator Calls: buffer ids and numbers by name.
+    std::vector<std::pair<std::string, uint32_t>> operands;
+    std::vector<std::pair<std::string, double>> attrs;
 
     bool hasAffineStore() const { return !outIndexCoeffs.empty(); }
     bool hasAffineGuard() const { return !guardCoeffs.empty(); }
@@ -95,8 +101,9 @@ struct KernelModule {
 };
 
 /// Parses an "mlk-kernel" document. Accepts the reference writer's output
-/// and two extensions: "math" on Call nodes, and Infinity/-Infinity/NaN
-/// tokens for exact non-finite constants.
+/// and three extensions: "math" on Call nodes, Infinity/-Infinity/NaN
+/// tokens for exact non-finite constants, and the "operands" and "attrs"
+/// objects of operator Calls.
 Result<KernelModule> parseKernelModule(const char* text, size_t len);
 
 /// Same multi-dim test as the reference executor (kernel_buffers.cpp:883-901)
@@ -109,6 +116,7 @@ std::vector<uint32_t> forestRoots(const KernelModule& km);
 
 int dtypeBytes(Dtype d);
 const char* mathOpName(MathOp op);
+bool isOperatorCall(const KernelNode& n);
 bool isUnaryMath(MathOp op);
 
 /// 64-bit structural hash of the module (the role of KernelModule::hash,

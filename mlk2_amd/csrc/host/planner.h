@@ -8,11 +8,36 @@
 #include <string>
 #include <vector>
 
+#include "../device_abi.h"
 #include "kernel_ir.h"
 
 namespace mlk::hip {
 
-enum class StepKind : uint8_t { Elementwise, Softmax, Gemm, RowSum, ScoreSoftmax, Nest, Fail };
+enum class StepKind : uint8_t { Elementwise, Softmax, Gemm, RowSum, ScoreSoftmax, Nest, Fail, NormRope, Attention };
+
+/// Operands of the operator Calls; each names a buffer of the module.
+enum OperandSlot : int {
+    kOpQ, kOpK, kOpV, kOpPrefixK, kOpPrefixV, kOpQWeight, kOpKWeight, kOpPositions, kOpSlots, kOpQOffsets, kOpKvStart,
+    kOpKvLen, kOpPrefixLen, kOpQOut, kOpKOut, kOpVOut, kOpOut, kOpLse, kOperandSlots
+};
+constexpr int kFirstOpOutput = kOpQOut;
+
+/// An operand's buffer as rows: `width` elements from row to row, the
+/// operand's own from column `at` on.
+struct Operand {
+    uint32_t buffer{kInvalidId};
+    int64_t rows{0}, width{0}, at{0};
+};
+
+/// A Call of an operator (operators.cpp).
+struct OperatorStep {
+    Operand op[kOperandSlots];
+    int32_t heads{0}, kvHeads{0}, dim{0}, sequences{0};
+    int32_t rot{0}, axes{1}, sections[3]{0, 0, 0};
+    bool interleaved{false}, causal{true};
+    double scale{0.0}, eps{0.0};
+    std::vector<double> quarters;   // frequency of each pair, in quarter turns per position
+};
 
 /// One read or write of a buffer over an R-dim box: element (v0..vR-1),
 /// v_d in [0, extent_d), touches buffer[offset + sum coeff[d] * v_d].
@@ -95,6 +120,9 @@ struct Step {
     bool narrowRoundTrip{false};
     bool touchesF16{false};
 
+    // NormRope / Attention.
+    OperatorStep oper;
+
     // Launch form of a hand-written kernel (-1: the kernel's default); set
     // by mlkhip_set_step_variant, the variant search or its cache.
     int variant{-1};
@@ -140,6 +168,14 @@ KernelModule canonicalModule(const KernelModule& km, int* rewrites);
 /// subtree as straight-line f64 device code, the outermost parallel loops
 /// collapsed onto threads. The step's `source` holds the hipRTC text.
 Result<Step> planNest(const KernelModule& km, uint32_t root);
+
+/// The step of an operator Call (operators.cpp): names, shapes, dtypes and
+/// overlaps checked.
+Result<Step> operatorStep(const KernelModule& km, const KernelNode& call);
+bool isOperator(const Step& st);
+/// Launch descriptors of an operator step; `ptr` holds an address per buffer id.
+void fillNormRope(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_norm_rope& p);
+void fillAttention(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_attention& p);
 
 /// Launch forms of a loop-nest step (nestgen.cpp): 0 the step's own kernel
 /// (its LDS slabs, 256 threads per workgroup); 1 the same kernel without

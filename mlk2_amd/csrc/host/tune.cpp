@@ -80,6 +80,8 @@ const char* kindName(StepKind k) {
         case StepKind::RowSum: return "rowsum";
         case StepKind::ScoreSoftmax: return "score-softmax";
         case StepKind::Nest: return "loop-nest";
+        case StepKind::NormRope: return "qk-norm-rope";
+        case StepKind::Attention: return "attention";
         case StepKind::Fail: return "empty";
     }
     return "?";
@@ -252,6 +254,8 @@ EssentialWork essentialWork(const KernelModule& km) {
         w.minBytes += elems * dtypeBytes(b.dtype);
     }
     for (const KernelNode& n : km.nodes) {
+        // An operator's work depends on the lengths and rows in its buffers.
+        if (isOperatorCall(n)) w.bytesKnown = w.opsKnown = false;
         walkOps(km, n, w, 0);
         if (!w.opsKnown) break;
     }
@@ -268,7 +272,8 @@ double peakOpsPerSec(const KernelModule& km, const Plan& plan) {
     }
     for (const Step& st : plan.steps) {
         if ((st.kind == StepKind::Gemm && st.a != kInvalidId && km.buffers[st.a].dtype == Dtype::F16) ||
-            st.kind == StepKind::ScoreSoftmax) {
+            st.kind == StepKind::ScoreSoftmax ||
+            (st.kind == StepKind::Attention && km.buffers[st.oper.op[kOpQ].buffer].dtype != Dtype::F32)) {
             return 2.5e15;
         }
     }
@@ -424,6 +429,15 @@ std::string launchCoverage(const KernelModule& km, const Step& st, int64_t eleme
                                    : "128-row blocks x key ranges, per pass";
             break;
         }
+        case StepKind::NormRope:
+        case StepKind::Attention:
+            // Query heads of the buffer's rows; workgroups that find no work
+            // (rows behind the last sequence) leave at once.
+            instances = st.oper.op[kOpQ].rows * st.oper.heads;
+            workgroups = instances;
+            perGroup = 1;
+            form = "query heads, by the lengths in the buffers";
+            break;
         case StepKind::Fail:
             covered = false;
             break;
@@ -562,6 +576,9 @@ int HipLoadedKernel::autotune(const DeviceBinding* binds, int n, const double* s
             if (b != kInvalidId && b < written.size()) written[b] = true;
         }
         for (const uint32_t b : st.nestWrites) written[b] = true;
+        for (int i = kFirstOpOutput; i < kOperandSlots; ++i) {
+            if (st.oper.op[i].buffer != kInvalidId) written[st.oper.op[i].buffer] = true;
+        }
     }
     struct Saved {
         int bind;
@@ -610,6 +627,16 @@ int HipLoadedKernel::autotune(const DeviceBinding* binds, int n, const double* s
                     float f;
                     std::memcpy(&f, raw.data() + e * 4, 4);
                     v[static_cast<size_t>(e)] = f;
+                } else if (kb.dtype == Dtype::BF16) {
+                    uint32_t bits = 0;
+                    std::memcpy(reinterpret_cast<char*>(&bits) + 2, raw.data() + e * 2, 2);
+                    float f;
+                    std::memcpy(&f, &bits, 4);
+                    v[static_cast<size_t>(e)] = f;
+                } else if (kb.dtype == Dtype::I32) {
+                    int32_t i;
+                    std::memcpy(&i, raw.data() + e * 4, 4);
+                    v[static_cast<size_t>(e)] = i;
                 } else {
                     _Float16 h;
                     std::memcpy(&h, raw.data() + e * 2, 2);

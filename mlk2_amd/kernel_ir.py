@@ -6,7 +6,8 @@ as plain Python objects, and serializes them to the "mlk-kernel" JSON document
 that ``KernelModule::toJson`` writes (``compiler/src/support/kernel_ir.cpp:97-254``).
 That document is the module interchange of the HIP backend's C ABI.
 
-``to_json`` writes two extensions of the reference writer that carry a module
+``to_json`` writes extensions of the reference writer. Operator Calls (see
+``operators``) carry ``"operands"`` and ``"attrs"``; two others carry a module
 losslessly: Call nodes carry ``"math"`` (the reference writer emits it for
 Compute nodes only), and non-finite constants are written as the tokens
 ``Infinity`` / ``-Infinity`` / ``NaN`` (the reference writer clamps +/-inf to
@@ -118,6 +119,8 @@ class KernelNode:
     family: Optional[str] = None
     exprs: List[KernelExpr] = field(default_factory=list)
     children: List[int] = field(default_factory=list)
+    operands: dict = field(default_factory=dict)   # operator Calls: buffer ids by name
+    attrs: dict = field(default_factory=dict)      # and numbers by name
 
     def to_json(self) -> dict:
         o = {"op": self.op}
@@ -160,6 +163,10 @@ class KernelNode:
             o["out"] = int(self.out)
         if self.exprs:
             o["exprs"] = [e.to_json() for e in self.exprs]
+        if self.operands:
+            o["operands"] = {k: int(v) for k, v in self.operands.items()}
+        if self.attrs:
+            o["attrs"] = dict(self.attrs)
         o["children"] = [int(c) for c in self.children]
         return o
 
