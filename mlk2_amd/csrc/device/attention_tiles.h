@@ -1,0 +1,388 @@
+// Attention on matrix cores: NW waves, 32 query rows each, over tiles of keys
+// in LDS, for f16 and bf16 rows of head dims that are multiples of 8.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "attention_span.h"
+
+namespace mlk {
+
+using f32x16 = float __attribute__((ext_vector_type(16)));
+using f32x4 = float __attribute__((ext_vector_type(4)));
+template <typename T>
+using Vec8 = T __attribute__((ext_vector_type(8)));
+template <typename T>
+using Vec4 = T __attribute__((ext_vector_type(4)));
+
+constexpr float kLowest = -3.402823466e38f;   // a running maximum before any score
+
+__device__ __forceinline__ f32x16 mfma(Vec8<_Float16> a, Vec8<_Float16> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(Vec8<__bf16> a, Vec8<__bf16> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+/// The other half wave's value of the same query (lanes l and l ^ 32).
+__device__ __forceinline__ float otherHalf(float v) {
+    const int i = __builtin_bit_cast(int, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(i, i, false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 32) != 0 ? r[0] : r[1]);
+}
+
+/// What a launch of tiles works on: which keys, which rows, and where the
+/// results go.
+struct TileArgs {
+    mlkd_attention p;
+    int keys;         // 1: the prefix, 2: the sequences' own, 3: both
+    int all_rows;     // 1: rows of all sequences together (prefix keys only)
+    int splits;       // key ranges of each row block
+    int part0;        // partial results: the first range's index ...
+    int parts;        // ... of so many (0: results go straight to out)
+    float* acc;       // [parts][rows * heads][dim]
+    float2* ml;       // [parts][rows * heads]: maximum (times log2 e), sum
+};
+
+/// The row block `tile` counted from the end of the batch: its sequence and
+/// first row. Rows are (token, head of the group); each sequence has
+/// ceil(nq * group / rows) blocks. All lanes return the same; false past the
+/// first block.
+__device__ __forceinline__ bool rowBlock(const mlkd_attention& p, int group, int rows, int tile, int& b, int& r0) {
+    const int ln = threadIdx.x & 63;
+    for (int s0 = 0; s0 < p.sequences; s0 += 64) {
+        const int s = p.sequences - 1 - s0 - ln;
+        const int mine = s >= 0 ? (spanOf(p, s).nq * group + rows - 1) / rows : 0;
+        int sum = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int v = __shfl_up(sum, d, 64);
+            sum += ln >= d ? v : 0;
+        }
+        const uint64_t past = __ballot(sum > tile);
+        if (past != 0) {
+            const int at = __builtin_ctzll(past);
+            b = __builtin_amdgcn_readfirstlane(p.sequences - 1 - s0 - at);
+            r0 = __builtin_amdgcn_readfirstlane((__builtin_amdgcn_readlane(sum, at) - 1 - tile) * rows);
+            return true;
+        }
+        tile -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
+/// Keys (or values) in LDS: rows of RB bytes in 16-byte pieces, piece c of row
+/// j at c ^ swizzle(j), so that the reads below meet every bank once: keys are
+/// read 16 rows x 16 bytes at a time, values 4 rows x 64 bytes.
+template <int RB>
+__device__ __forceinline__ int swizzleK(int j) {
+    return RB == 128 ? (j >> 1) & 7 : j & 15;
+}
+template <int RB>
+__device__ __forceinline__ int swizzleV(int j) {
+    return RB == 128 ? ((j >> 1) & 1) << 2 : (j & 3) << 2;
+}
+
+template <typename T, int DT, int NW, int KEYS, int STAGES>
+struct Tiles {
+    static constexpr int KS = DT / 16, DB = (DT + 31) / 32;        // steps of q k^T, 32-column blocks of out
+    static constexpr int RB = DT <= 64 ? 128 : DT <= 128 ? 256 : 512;
+    static constexpr int kTile = KEYS * RB;                          // bytes of a tile of keys
+    static constexpr int kStage = 2 * kTile;
+    static constexpr int kLds = STAGES * kStage;
+    static constexpr int kRows = 32 * NW;
+    static constexpr int IPW = kTile / 1024 / NW;                    // 1024-byte loads of a wave, for keys and again for values
+    static constexpr int KB = KEYS / 32;
+    static_assert(IPW >= 1 && IPW * NW * 1024 == kTile, "a tile is whole loads of the waves");
+    static_assert((STAGES - 1) * 2 * IPW <= 63, "loads in flight fit the counter");
+
+    /// This wave's loads of a tile, straight to LDS: rows past the last valid
+    /// one repeat it; pieces past the head dim stay zero.
+    static __device__ __forceinline__ void load(const void* k, const void* v, uint32_t ks, uint32_t vs, int last, int pieces, uint32_t lds, int wave) {
+        const int ln = threadIdx.x & 63;
+        constexpr int P = RB / 16;   // pieces of a row
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int i = 0; i < IPW; ++i) {
+                const int n = wave * IPW + i, row = n * (64 / P) + ln / P;
+                const int piece = (ln % P) ^ (half == 0 ? swizzleK<RB>(row) : swizzleV<RB>(row));
+                const uint32_t off = static_cast<uint32_t>(min(row, last)) * (half == 0 ? ks : vs) + piece * 16;
+                const uint32_t m0 = lds + half * kTile + n * 1024;
+                if (piece < pieces) {
+                    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(half == 0 ? k : v), "s"(m0) : "memory");
+                }
+            }
+        }
+    }
+
+    /// Waits until at most `ahead` tiles of this wave's loads are in flight.
+    static __device__ __forceinline__ void wait(int ahead) {
+        static_assert(STAGES <= 4, "");
+        if (ahead >= 2 && STAGES >= 4) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * 2 * IPW) : "memory");
+        else if (ahead >= 1 && STAGES >= 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * IPW) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+};
+
+/// One row block of one key/value head. With S^T = K Q^T in 32 x 32 blocks a
+/// lane holds 16 keys' scores of one query (the other 16 in lane ^ 32), so the
+/// softmax is register work but for one exchange of maxima, and its weights are
+/// as they stand the operand of out^T = V^T W^T: the keys of a 16-key step are
+/// taken in the order the scores have. V^T comes out of V's rows in LDS by
+/// transposing reads. The maximum that the weights are taken relative to
+/// follows the running one only when that has grown by 2^8: sums of weights
+/// up to 2^8 lose nothing in f32, and out is rescaled in few tiles.
+template <typename T, int DT, int NW, int KEYS, int STAGES>
+__global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(TileArgs a) {
+    using S = Tiles<T, DT, NW, KEYS, STAGES>;
+    using V8 = Vec8<T>;
+    using V4 = Vec4<T>;
+    using Short4 = short __attribute__((ext_vector_type(4)));
+    constexpr int KS = S::KS, DB = S::DB, RB = S::RB, KB = S::KB;
+    extern __shared__ __align__(16) char ldsTiles[];
+    const mlkd_attention& p = a.p;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int ln = threadIdx.x & 63, l32 = ln & 31, hl = ln >> 5;
+    const int group = p.heads / p.kv_heads, g = static_cast<int>(blockIdx.x) % p.kv_heads;
+    int rest = static_cast<int>(blockIdx.x) / p.kv_heads;
+    const int split = rest % a.splits;
+    rest /= a.splits;
+    SeqSpan s;
+    int r0 = 0;
+    if (a.all_rows != 0) {
+        s = SeqSpan{0, 0, static_cast<int32_t>(p.q_rows), 0};
+        r0 = rest * S::kRows;
+        if (r0 >= s.nq * group) return;
+    } else {
+        int b = 0;
+        if (!rowBlock(p, group, S::kRows, rest, b, r0)) return;
+        s = spanOf(p, b);
+    }
+    const int rows = s.nq * group;
+    // Keys that a row sees: the prefix, and own keys below lim = token + slope.
+    const int np = (a.keys & 1) != 0 ? prefixOf(p) : 0, nk = (a.keys & 2) != 0 ? s.nk : 0;
+    auto limit = [&](int r) {
+        return p.causal != 0 ? min(max(min(r, rows - 1) / group + s.nk - s.nq + 1, 0), nk) : nk;
+    };
+    const int tilesP = (np + KEYS - 1) / KEYS, tiles = tilesP + (limit(r0 + S::kRows - 1) + KEYS - 1) / KEYS;
+    const int first = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
+    const int end = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+    const int rw = r0 + wave * 32;                       // this wave's first row
+    const int limLo = limit(rw), limHi = limit(rw + 31);
+    const int r = min(rw + l32, rows - 1), lim = limit(r), head = g * group + r % group;
+    const bool valid = rw + l32 < rows;
+    const int64_t token = s.q0 + r / group;
+
+    // Queries, 8 columns a step; a negative scale turns their signs.
+    const float c = static_cast<float>(fabs(p.scale) * 1.4426950408889634);
+    V8 q[KS];
+    {
+        const T* qr = static_cast<const T*>(p.q) + token * p.q_stride + static_cast<int64_t>(head) * p.dim;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) {
+            const int d = i * 16 + hl * 8;
+            V8 x = {};
+            if (d < p.dim) x = *reinterpret_cast<const V8*>(qr + d);
+            if (p.scale < 0.0) x = -x;
+            q[i] = x;
+        }
+    }
+
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ldsTiles));
+    const int pieces = p.dim / 8;
+    if (p.dim < DT) {   // what the loads leave out
+        for (int i = threadIdx.x * 16; i < S::kLds; i += NW * 64 * 16) *reinterpret_cast<f32x4*>(ldsTiles + i) = f32x4{};
+        __syncthreads();
+    }
+    const uint32_t ksOwn = static_cast<uint32_t>(p.k_stride * sizeof(T)), vsOwn = static_cast<uint32_t>(p.v_stride * sizeof(T));
+    const T* kOwn = static_cast<const T*>(p.k) + s.k0 * p.k_stride + g * p.dim;
+    const T* vOwn = static_cast<const T*>(p.v) + s.k0 * p.v_stride + g * p.dim;
+    const T* kPre = static_cast<const T*>(p.prefix_k) + g * p.dim;
+    const T* vPre = static_cast<const T*>(p.prefix_v) + g * p.dim;
+    auto load = [&](int it) {
+        const uint32_t lds = lds0 + (it - first) % STAGES * S::kStage;
+        if (it < tilesP) {
+            S::load(kPre + static_cast<int64_t>(it) * KEYS * p.prefix_k_stride, vPre + static_cast<int64_t>(it) * KEYS * p.prefix_v_stride,
+                    static_cast<uint32_t>(p.prefix_k_stride * sizeof(T)), static_cast<uint32_t>(p.prefix_v_stride * sizeof(T)),
+                    np - it * KEYS - 1, pieces, lds, wave);
+        } else {
+            const int t = it - tilesP;
+            S::load(kOwn + static_cast<int64_t>(t) * KEYS * p.k_stride, vOwn + static_cast<int64_t>(t) * KEYS * p.v_stride, ksOwn, vsOwn,
+                    nk - t * KEYS - 1, pieces, lds, wave);
+        }
+    };
+
+    // Offsets of this lane's reads within a tile.
+    uint32_t atK[KS], atV[DB];
+#pragma unroll
+    for (int i = 0; i < KS; ++i) atK[i] = l32 * RB + (((2 * i + hl) ^ swizzleK<RB>(l32)) << 4);
+    const int vr = 4 * hl + (ln & 15) / 4;   // the row of four that this lane's read starts
+#pragma unroll
+    for (int i = 0; i < DB; ++i) {
+        const int byte = i * 64 + ((ln >> 4) & 1) * 32 + (ln & 3) * 8;
+        atV[i] = S::kTile + vr * RB + (((byte >> 4) ^ swizzleV<RB>(vr)) << 4) + (byte & 15);
+    }
+
+    f32x16 o[DB];
+    float m = kLowest, l = 0.0f;   // of this lane's query; l of this lane's keys
+    // Only a second pass is careful: a weight of 0 takes an infinite or NaN
+    // value to NaN, so where a row of the first came out non-finite, the tiles
+    // that hide keys from some rows are summed key by key, hidden ones left out.
+    for (int careful = 0; careful < 2; ++careful) {
+#pragma unroll
+        for (int i = 0; i < DB; ++i) o[i] = f32x16{};
+        m = kLowest;
+        l = 0.0f;
+        for (int it = first; it < min(first + STAGES - 1, end); ++it) load(it);
+        for (int it = first; it < end; ++it) {
+            S::wait(min(end - 1 - it, STAGES - 2));
+            if (NW > 1) __builtin_amdgcn_s_barrier();
+            if (it + STAGES - 1 < end) load(it + STAGES - 1);
+            const bool pre = it < tilesP;
+            const int j0 = (pre ? it : it - tilesP) * KEYS;         // first key
+            if ((pre ? np : limHi) <= j0) continue;
+            const bool hides = (pre ? np : limLo) < j0 + KEYS;
+            const int seen = (pre ? np : lim) - j0;                  // keys of the tile that this row sees
+            const char* tile = ldsTiles + (it - first) % STAGES * S::kStage;
+            if (careful != 0 && hides) {
+                const int n = min((pre ? np : nk) - j0, KEYS);
+                for (int j = 0; j < n; ++j) {
+                    float x = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < KS; ++i) {
+                        const V8 kk = *reinterpret_cast<const V8*>(tile + j * RB + (((2 * i + hl) ^ swizzleK<RB>(j)) << 4));
+                        // This path is rare: no registers for its sake, so that
+                        // its conversions of q stay where they are.
+                        f32x4 bits = __builtin_bit_cast(f32x4, q[i]);
+                        asm volatile("" : "+v"(bits));
+                        const V8 qq = __builtin_bit_cast(V8, bits);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) x += static_cast<float>(qq[e]) * static_cast<float>(kk[e]);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    x += otherHalf(x);
+                    if (j >= seen) x = -INFINITY;
+                    const float top = fmaxf(m, x * c), keep = __builtin_amdgcn_exp2f(m - top);
+                    const float w = __builtin_amdgcn_exp2f(x * c - top);
+                    m = top;
+                    l = l * keep + (hl == 0 ? w : 0.0f);
+                    const float wt = static_cast<float>(static_cast<T>(w));
+#pragma unroll
+                    for (int i = 0; i < DB; ++i) {
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) {
+                            const int byte = i * 64 + e * 4 + hl * 8;   // columns 32 i + 2 e + 4 hl on
+                            const V4 vv = *reinterpret_cast<const V4*>(tile + S::kTile + j * RB + (((byte >> 4) ^ swizzleV<RB>(j)) << 4) + (byte & 15));
+#pragma unroll
+                            for (int f = 0; f < 4; ++f) {
+                                const float old = o[i][e + f] * keep;
+                                o[i][e + f] = j < seen ? old + wt * static_cast<float>(vv[f]) : old;
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                }
+                continue;
+            }
+            f32x16 x[KB];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                x[kb] = f32x16{};
+#pragma unroll
+                for (int i = 0; i < KS; ++i) x[kb] = mfma(*reinterpret_cast<const V8*>(tile + kb * 32 * RB + atK[i]), q[i], x[kb]);
+            }
+            if (hides) {
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        if (kb * 32 + 8 * (e / 4) + e % 4 + 4 * hl >= seen) x[kb][e] = -INFINITY;
+                    }
+                }
+            }
+            float top = x[0][0];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[kb][e]);
+            }
+            top = fmaxf(top, otherHalf(top)) * c;
+            if (__any(top > m + 8.0f)) {
+                const float base = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - base);
+                m = base;
+                l *= keep;
+#pragma unroll
+                for (int i = 0; i < DB; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[i][e] *= keep;
+                }
+            }
+            V8 w[KEYS / 16];
+#pragma unroll
+            for (int kg = 0; kg < KEYS / 16; ++kg) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kg / 2][kg % 2 * 8 + e], c, -m));
+                    l += v;
+                    w[kg][e] = static_cast<T>(v);
+                }
+            }
+#pragma unroll
+            for (int kg = 0; kg < KEYS / 16; ++kg) {
+#pragma unroll
+                for (int i = 0; i < DB; ++i) {
+                    using Lds = __attribute__((address_space(3))) Short4;
+                    const char* at = tile + atV[i] + kg * 16 * RB;
+                    const Short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at));
+                    const Short4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at + 8 * RB));
+                    const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[i] = mfma(__builtin_bit_cast(V8, both), w[kg], o[i]);
+                }
+            }
+        }
+        bool bad = !(fabsf(l) < INFINITY);
+#pragma unroll
+        for (int i = 0; i < DB; ++i) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) bad |= !(fabsf(o[i][e]) < INFINITY);
+        }
+        if (careful != 0 || !__syncthreads_or(bad)) break;
+    }
+
+    l += otherHalf(l);
+    if (!valid) return;
+    const int64_t row = token * p.heads + head;
+    if (a.parts > 0) {
+        const int64_t at = static_cast<int64_t>(a.part0 + split) * p.q_rows * p.heads + row;
+        if (hl == 0) a.ml[at] = make_float2(m, l);
+        float* out = a.acc + at * p.dim;
+#pragma unroll
+        for (int i = 0; i < DB; ++i) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int d = i * 32 + 2 * e + 4 * hl;
+                if (d < p.dim) *reinterpret_cast<f32x4*>(out + d) = f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+            }
+        }
+        return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = static_cast<T*>(p.out) + token * p.out_stride + static_cast<int64_t>(head) * p.dim;
+#pragma unroll
+    for (int i = 0; i < DB; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int d = i * 32 + 2 * e + 4 * hl;
+            V4 v;
+#pragma unroll
+            for (int f = 0; f < 4; ++f) v[f] = static_cast<T>(o[i][e + f] * inv);
+            if (d < p.dim) *reinterpret_cast<V4*>(out + d) = v;
+        }
+    }
+    if (p.lse != nullptr && hl == 0) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+}  // namespace mlk
