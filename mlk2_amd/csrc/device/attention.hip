@@ -156,18 +156,28 @@ struct Plan {
     int parts() const { return splitsOwn + splitsPrefix > 1 ? splitsOwn + splitsPrefix : 0; }
 };
 
-bool aligned(const void* ptr, int64_t stride, int elements) {
-    return reinterpret_cast<uintptr_t>(ptr) % (2 * elements) == 0 && stride % elements == 0 && stride < (int64_t{1} << 23);
+bool aligned(const void* ptr, int64_t stride, int bytes, int size) {
+    return reinterpret_cast<uintptr_t>(ptr) % bytes == 0 && stride * size % bytes == 0 && stride < (int64_t{1} << 22);
 }
 
-/// The matrix-core kernels take 16-bit rows whose 16-byte pieces are aligned.
+/// The matrix-core kernels take rows whose 16-byte pieces are aligned.
 bool tilesApply(const mlkd_attention* p) {
-    if (p->dtype == MLKD_F32 || p->dim % 8 != 0) return false;
+    const int size = p->dtype == MLKD_F32 ? 4 : 2;
+    if (p->dim % 8 != 0) return false;
     if (p->q_rows * (p->heads / p->kv_heads) >= (int64_t{1} << 30)) return false;   // rows are counted in 32 bits
-    return aligned(p->q, p->q_stride, 8) && aligned(p->k, p->k_stride, 8) && aligned(p->v, p->v_stride, 8) &&
-           aligned(p->out, p->out_stride, 4) && aligned(p->prefix_k, p->prefix_k_stride, 8) &&
-           aligned(p->prefix_v, p->prefix_v_stride, 8);
+    return aligned(p->q, p->q_stride, 16, size) && aligned(p->k, p->k_stride, 16, size) && aligned(p->v, p->v_stride, 16, size) &&
+           aligned(p->out, p->out_stride, 4 * size, size) && aligned(p->prefix_k, p->prefix_k_stride, 16, size) &&
+           aligned(p->prefix_v, p->prefix_v_stride, 16, size);
 }
+
+/// Tiles of the matrix-core kernels: keys a tile and tiles in LDS.
+constexpr int keysOf(int size, int dt, int waves) { return waves > 1 && size == 2 && dt <= 128 ? 64 : 32; }
+constexpr int stagesOf(int size, int dt, int waves) {
+    const int bytes = 2 * keysOf(size, dt, waves) * (dt <= 64 ? 64 : dt <= 128 ? 128 : 256) * size;   // of a tile
+    return waves > 1 ? (bytes <= 32768 ? 3 : 2) : bytes <= 16384 ? 4 : 2;
+}
+constexpr int wideOf(int size, int dt) { return size == 2 && dt <= 128 ? 8 : 4; }
+int dimOf(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
 
 Plan planOf(const mlkd_attention* p) {
     Plan n;
@@ -176,7 +186,7 @@ Plan planOf(const mlkd_attention* p) {
     const int64_t group = p->heads / p->kv_heads;
     const int64_t each = (p->q_rows + p->sequences - 1) / p->sequences * group;   // rows of a sequence, on average
     const int64_t keys = std::max<int64_t>(1, p->kv_rows / p->sequences);
-    const int wide = p->dim <= 128 ? 8 : 4;
+    const int wide = wideOf(p->dtype == MLKD_F32 ? 4 : 2, dimOf(p->dim));
     n.wavesOwn = each > 64 ? wide : 1;
     n.shared = p->prefix_k != nullptr && n.wavesOwn == 1;
     auto ranges = [&](int64_t blocks, int64_t count, int64_t fill) {
@@ -203,8 +213,7 @@ Plan planFor(const mlkd_attention* p) {
 
 template <typename T, int DT, int NW>
 int launchTiles(const mlk::TileArgs& a, int64_t blocks, hipStream_t st) {
-    constexpr int KEYS = NW > 1 && DT <= 128 ? 64 : 32;
-    constexpr int STAGES = NW > 1 ? 3 : DT <= 128 ? 4 : 2;
+    constexpr int KEYS = keysOf(sizeof(T), DT, NW), STAGES = stagesOf(sizeof(T), DT, NW);
     constexpr int bytes = mlk::Tiles<T, DT, NW, KEYS, STAGES>::kLds;
     auto* kernel = mlk::attentionTiles<T, DT, NW, KEYS, STAGES>;
     // Once per process; a function-local static initializes thread-safely.
@@ -225,16 +234,18 @@ int64_t rowBlocks(const mlk::TileArgs& a, int waves) {
 
 template <typename T, int DT>
 int launchWaves(const mlk::TileArgs& a, int waves, hipStream_t st) {
-    constexpr int WIDE = DT <= 128 ? 8 : 4;
+    constexpr int WIDE = wideOf(sizeof(T), DT);
     return waves == 1 ? launchTiles<T, DT, 1>(a, rowBlocks(a, 1), st) : launchTiles<T, DT, WIDE>(a, rowBlocks(a, WIDE), st);
 }
 
 template <typename T>
 int launchDim(const mlk::TileArgs& a, int waves, hipStream_t st) {
-    return a.p.dim <= 64    ? launchWaves<T, 64>(a, waves, st)
-           : a.p.dim <= 96  ? launchWaves<T, 96>(a, waves, st)
-           : a.p.dim <= 128 ? launchWaves<T, 128>(a, waves, st)
-                            : launchWaves<T, 256>(a, waves, st);
+    switch (dimOf(a.p.dim)) {
+        case 64: return launchWaves<T, 64>(a, waves, st);
+        case 96: return launchWaves<T, 96>(a, waves, st);
+        case 128: return launchWaves<T, 128>(a, waves, st);
+        default: return launchWaves<T, 256>(a, waves, st);
+    }
 }
 
 template <typename T>
@@ -283,10 +294,10 @@ const char* mlkd_attention_kernel_names(const mlkd_attention* p) {
         name = "attentionRows<" + type + ">";
         return name.c_str();
     }
-    const int dt = p->dim <= 64 ? 64 : p->dim <= 96 ? 96 : p->dim <= 128 ? 128 : 256;
+    const int dt = dimOf(p->dim), size = p->dtype == MLKD_F32 ? 4 : 2;
     auto tiles = [&](int waves) {
         return "attentionTiles<" + type + ", " + std::to_string(dt) + ", " + std::to_string(waves) + ", " +
-               std::to_string(waves > 1 && dt <= 128 ? 64 : 32) + ", " + std::to_string(waves > 1 ? 3 : dt <= 128 ? 4 : 2) + ">";
+               std::to_string(keysOf(size, dt, waves)) + ", " + std::to_string(stagesOf(size, dt, waves)) + ">";
     };
     name = n.shared ? tiles(n.wavesPrefix) + "+" + tiles(n.wavesOwn) : tiles(n.wavesOwn);
     if (n.parts() > 0) name += "+attentionJoin<" + type + ", " + std::to_string(dt <= 64 ? 16 : dt <= 128 ? 32 : 64) + ">";
@@ -298,7 +309,9 @@ int mlkd_launch_attention(const mlkd_attention* p, void* stream) {
     if (rows == 0) return 0;
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (const Plan n = planFor(p); n.tiles) {
-        const int rc = p->dtype == MLKD_F16 ? launchPlan<_Float16>(p, n, st) : launchPlan<__bf16>(p, n, st);
+        const int rc = p->dtype == MLKD_F32   ? launchPlan<float>(p, n, st)
+                       : p->dtype == MLKD_F16 ? launchPlan<_Float16>(p, n, st)
+                                              : launchPlan<__bf16>(p, n, st);
         if (rc >= 0) return rc;   // else a grid past the limit
     }
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((rows + 3) / 4, int64_t{1} << 20)));

@@ -1,5 +1,5 @@
 // Attention on matrix cores: NW waves, 32 query rows each, over tiles of keys
-// in LDS, for f16 and bf16 rows of head dims that are multiples of 8.
+// in LDS, for rows whose heads are whole 16-byte pieces.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -13,17 +13,25 @@ namespace mlk {
 using f32x16 = float __attribute__((ext_vector_type(16)));
 using f32x4 = float __attribute__((ext_vector_type(4)));
 template <typename T>
-using Vec8 = T __attribute__((ext_vector_type(8)));
-template <typename T>
 using Vec4 = T __attribute__((ext_vector_type(4)));
+/// 16 bytes of a row.
+template <typename T>
+using Piece = T __attribute__((ext_vector_type(16 / sizeof(T))));
 
 constexpr float kLowest = -3.402823466e38f;   // a running maximum before any score
 
-__device__ __forceinline__ f32x16 mfma(Vec8<_Float16> a, Vec8<_Float16> b, f32x16 c) {
+/// c += a b over the columns of a piece in either half wave: 16 of f16 and
+/// bf16, 8 of f32.
+__device__ __forceinline__ f32x16 mfma(Piece<_Float16> a, Piece<_Float16> b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mfma(Vec8<__bf16> a, Vec8<__bf16> b, f32x16 c) {
+__device__ __forceinline__ f32x16 mfma(Piece<__bf16> a, Piece<__bf16> b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma(Piece<float> a, Piece<float> b, f32x16 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+    return c;
 }
 
 /// The other half wave's value of the same query (lanes l and l ^ 32).
@@ -75,20 +83,21 @@ __device__ __forceinline__ bool rowBlock(const mlkd_attention& p, int group, int
 
 /// Keys (or values) in LDS: rows of RB bytes in 16-byte pieces, piece c of row
 /// j at c ^ swizzle(j), so that the reads below meet every bank once: keys are
-/// read 16 rows x 16 bytes at a time, values 4 rows x 64 bytes.
+/// read 16 rows x 16 bytes at a time, 16-bit values 4 rows x 64 bytes, f32 values
+/// two rows four apart x 128 bytes.
 template <int RB>
 __device__ __forceinline__ int swizzleK(int j) {
     return RB == 128 ? (j >> 1) & 7 : j & 15;
 }
-template <int RB>
+template <typename T, int RB>
 __device__ __forceinline__ int swizzleV(int j) {
-    return RB == 128 ? ((j >> 1) & 1) << 2 : (j & 3) << 2;
+    return sizeof(T) == 4 ? (j >> 2 & 1) << 3 : RB == 128 ? (j >> 1 & 1) << 2 : (j & 3) << 2;
 }
 
 template <typename T, int DT, int NW, int KEYS, int STAGES>
 struct Tiles {
-    static constexpr int KS = DT / 16, DB = (DT + 31) / 32;        // steps of q k^T, 32-column blocks of out
-    static constexpr int RB = DT <= 64 ? 128 : DT <= 128 ? 256 : 512;
+    static constexpr int KS = DT * sizeof(T) / 32, DB = DT / 32;      // steps of q k^T, two pieces each; 32-column blocks of out
+    static constexpr int RB = (DT <= 64 ? 64 : DT <= 128 ? 128 : 256) * sizeof(T);
     static constexpr int kTile = KEYS * RB;                          // bytes of a tile of keys
     static constexpr int kStage = 2 * kTile;
     static constexpr int kLds = STAGES * kStage;
@@ -96,24 +105,44 @@ struct Tiles {
     static constexpr int IPW = kTile / 1024 / NW;                    // 1024-byte loads of a wave, for keys and again for values
     static constexpr int KB = KEYS / 32;
     static_assert(IPW >= 1 && IPW * NW * 1024 == kTile, "a tile is whole loads of the waves");
-    static_assert((STAGES - 1) * 2 * IPW <= 63, "loads in flight fit the counter");
+    static_assert(STAGES == 2 || (STAGES - 2) * 2 * IPW <= 63, "the loads waited on by number fit the counter");
+
+    static __device__ __forceinline__ void dma(const void* base, uint32_t off, uint32_t m0) {
+        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory");
+    }
+
+    static __device__ __forceinline__ int swizzle(int half, int row) {
+        return half == 0 ? swizzleK<RB>(row) : swizzleV<T, RB>(row);
+    }
 
     /// This wave's loads of a tile, straight to LDS: rows past the last valid
     /// one repeat it; pieces past the head dim stay zero.
     static __device__ __forceinline__ void load(const void* k, const void* v, uint32_t ks, uint32_t vs, int last, int pieces, uint32_t lds, int wave) {
-        const int ln = threadIdx.x & 63;
-        constexpr int P = RB / 16;   // pieces of a row
+        constexpr int P = RB / 16, R = 64 / P;   // pieces of a row, rows of a load
+        int ln = threadIdx.x & 63;
+        asm volatile("" : "+v"(ln));   // the offsets are taken anew for each tile: kept, they are up to 64 registers
+        if (last >= KEYS - 1 && pieces == P) {
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
+            for (int half = 0; half < 2; ++half) {
+                const uint32_t stride = half == 0 ? ks : vs;
+                const char* base = static_cast<const char*>(half == 0 ? k : v) + static_cast<uint64_t>(wave * IPW * R) * stride;
+                const uint32_t row = ln / P * stride, piece = ((ln % P) ^ swizzle(half, wave * IPW * R + ln / P)) << 4;
 #pragma unroll
-            for (int i = 0; i < IPW; ++i) {
-                const int n = wave * IPW + i, row = n * (64 / P) + ln / P;
-                const int piece = (ln % P) ^ (half == 0 ? swizzleK<RB>(row) : swizzleV<RB>(row));
-                const uint32_t off = static_cast<uint32_t>(min(row, last)) * (half == 0 ? ks : vs) + piece * 16;
-                const uint32_t m0 = lds + half * kTile + n * 1024;
-                if (piece < pieces) {
-                    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(half == 0 ? k : v), "s"(m0) : "memory");
+                for (int i = 0; i < IPW; ++i) {
+                    // Rows i R + r with r < R: their swizzle is i R's and r's.
+                    const int w0 = wave * IPW * R, turned = swizzle(half, w0 + i * R) ^ swizzle(half, w0);
+                    dma(base + static_cast<uint64_t>(i * R) * stride, (piece ^ (turned << 4)) + row, lds + half * kTile + (wave * IPW + i) * 1024);
                 }
+            }
+            return;
+        }
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll 1
+            for (int i = 0; i < IPW; ++i) {
+                const int n = wave * IPW + i, row = n * R + ln / P, piece = (ln % P) ^ swizzle(half, row);
+                const uint32_t off = static_cast<uint32_t>(min(row, last)) * (half == 0 ? ks : vs) + piece * 16;
+                if (piece < pieces) dma(half == 0 ? k : v, off, lds + half * kTile + n * 1024);
             }
         }
     }
@@ -138,7 +167,7 @@ struct Tiles {
 template <typename T, int DT, int NW, int KEYS, int STAGES>
 __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(TileArgs a) {
     using S = Tiles<T, DT, NW, KEYS, STAGES>;
-    using V8 = Vec8<T>;
+    using P = Piece<T>;
     using V4 = Vec4<T>;
     using Short4 = short __attribute__((ext_vector_type(4)));
     constexpr int KS = S::KS, DB = S::DB, RB = S::RB, KB = S::KB;
@@ -176,23 +205,23 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
     const bool valid = rw + l32 < rows;
     const int64_t token = s.q0 + r / group;
 
-    // Queries, 8 columns a step; a negative scale turns their signs.
+    // Queries, a piece a step; a negative scale turns their signs.
     const float c = static_cast<float>(fabs(p.scale) * 1.4426950408889634);
-    V8 q[KS];
+    P q[KS];
     {
         const T* qr = static_cast<const T*>(p.q) + token * p.q_stride + static_cast<int64_t>(head) * p.dim;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-            const int d = i * 16 + hl * 8;
-            V8 x = {};
-            if (d < p.dim) x = *reinterpret_cast<const V8*>(qr + d);
+            const int d = (2 * i + hl) * (16 / static_cast<int>(sizeof(T)));
+            P x = {};
+            if (d < p.dim) x = *reinterpret_cast<const P*>(qr + d);
             if (p.scale < 0.0) x = -x;
             q[i] = x;
         }
     }
 
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ldsTiles));
-    const int pieces = p.dim / 8;
+    const int pieces = p.dim * static_cast<int>(sizeof(T)) / 16;
     if (p.dim < DT) {   // what the loads leave out
         for (int i = threadIdx.x * 16; i < S::kLds; i += NW * 64 * 16) *reinterpret_cast<f32x4*>(ldsTiles + i) = f32x4{};
         __syncthreads();
@@ -216,14 +245,15 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
     };
 
     // Offsets of this lane's reads within a tile.
-    uint32_t atK[KS], atV[DB];
-#pragma unroll
-    for (int i = 0; i < KS; ++i) atK[i] = l32 * RB + (((2 * i + hl) ^ swizzleK<RB>(l32)) << 4);
-    const int vr = 4 * hl + (ln & 15) / 4;   // the row of four that this lane's read starts
+    const uint32_t atK = l32 * RB + ((hl ^ swizzleK<RB>(l32)) << 4);   // step i: its piece bits turned by 2 i
+    uint32_t atV[DB];
+    // 16-bit values: the row of four, and their eight bytes, that this lane
+    // hands the transposing read; f32: the first row and its column.
+    const int vr = 4 * hl + (sizeof(T) == 4 ? 0 : (ln & 15) / 4);
 #pragma unroll
     for (int i = 0; i < DB; ++i) {
-        const int byte = i * 64 + ((ln >> 4) & 1) * 32 + (ln & 3) * 8;
-        atV[i] = S::kTile + vr * RB + (((byte >> 4) ^ swizzleV<RB>(vr)) << 4) + (byte & 15);
+        const int byte = sizeof(T) == 4 ? i * 128 + l32 * 4 : i * 64 + ((ln >> 4) & 1) * 32 + (ln & 3) * 8;
+        atV[i] = S::kTile + vr * RB + (((byte >> 4) ^ swizzleV<T, RB>(vr)) << 4) + (byte & 15);
     }
 
     f32x16 o[DB];
@@ -253,14 +283,14 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
                     float x = 0.0f;
 #pragma unroll
                     for (int i = 0; i < KS; ++i) {
-                        const V8 kk = *reinterpret_cast<const V8*>(tile + j * RB + (((2 * i + hl) ^ swizzleK<RB>(j)) << 4));
+                        const P kk = *reinterpret_cast<const P*>(tile + j * RB + (((2 * i + hl) ^ swizzleK<RB>(j)) << 4));
                         // This path is rare: no registers for its sake, so that
                         // its conversions of q stay where they are.
                         f32x4 bits = __builtin_bit_cast(f32x4, q[i]);
                         asm volatile("" : "+v"(bits));
-                        const V8 qq = __builtin_bit_cast(V8, bits);
+                        const P qq = __builtin_bit_cast(P, bits);
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x += static_cast<float>(qq[e]) * static_cast<float>(kk[e]);
+                        for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) x += static_cast<float>(qq[e]) * static_cast<float>(kk[e]);
                         __builtin_amdgcn_sched_barrier(0);
                     }
                     x += otherHalf(x);
@@ -274,8 +304,8 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
                     for (int i = 0; i < DB; ++i) {
 #pragma unroll
                         for (int e = 0; e < 16; e += 4) {
-                            const int byte = i * 64 + e * 4 + hl * 8;   // columns 32 i + 2 e + 4 hl on
-                            const V4 vv = *reinterpret_cast<const V4*>(tile + S::kTile + j * RB + (((byte >> 4) ^ swizzleV<RB>(j)) << 4) + (byte & 15));
+                            const int byte = (32 * i + 2 * e + 4 * hl) * static_cast<int>(sizeof(T));
+                            const V4 vv = *reinterpret_cast<const V4*>(tile + S::kTile + j * RB + (((byte >> 4) ^ swizzleV<T, RB>(j)) << 4) + (byte & 15));
 #pragma unroll
                             for (int f = 0; f < 4; ++f) {
                                 const float old = o[i][e + f] * keep;
@@ -288,11 +318,13 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
                 continue;
             }
             f32x16 x[KB];
+            uint32_t lane = atK;
+            if (KS > 8) asm volatile("" : "+v"(lane));   // taken anew for each tile, where 16 of them take registers
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 x[kb] = f32x16{};
 #pragma unroll
-                for (int i = 0; i < KS; ++i) x[kb] = mfma(*reinterpret_cast<const V8*>(tile + kb * 32 * RB + atK[i]), q[i], x[kb]);
+                for (int i = 0; i < KS; ++i) x[kb] = mfma(*reinterpret_cast<const P*>(tile + kb * 32 * RB + (lane ^ (i << 5))), q[i], x[kb]);
             }
             if (hides) {
 #pragma unroll
@@ -320,26 +352,45 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
                     for (int e = 0; e < 16; ++e) o[i][e] *= keep;
                 }
             }
-            V8 w[KEYS / 16];
+            if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int kg = 0; kg < KEYS / 16; ++kg) {
+                for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kg / 2][kg % 2 * 8 + e], c, -m));
-                    l += v;
-                    w[kg][e] = static_cast<T>(v);
+                    for (int e = 0; e < 16; ++e) {
+                        x[kb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][e], c, -m));
+                        l += x[kb][e];
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+#pragma unroll
+                        for (int i = 0; i < DB; ++i) {
+                            const float v = *reinterpret_cast<const float*>(tile + atV[i] + (kb * 32 + 8 * (e / 4) + e % 4) * RB);
+                            o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, x[kb][e], o[i], 0, 0, 0);
+                        }
+                    }
                 }
-            }
+            } else {
+                P w[KEYS / 16];
 #pragma unroll
-            for (int kg = 0; kg < KEYS / 16; ++kg) {
+                for (int kg = 0; kg < KEYS / 16; ++kg) {
 #pragma unroll
-                for (int i = 0; i < DB; ++i) {
-                    using Lds = __attribute__((address_space(3))) Short4;
-                    const char* at = tile + atV[i] + kg * 16 * RB;
-                    const Short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at));
-                    const Short4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at + 8 * RB));
-                    const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[i] = mfma(__builtin_bit_cast(V8, both), w[kg], o[i]);
+                    for (int e = 0; e < 8; ++e) {
+                        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kg / 2][kg % 2 * 8 + e], c, -m));
+                        l += v;
+                        w[kg][e] = static_cast<T>(v);
+                    }
+                }
+#pragma unroll
+                for (int kg = 0; kg < KEYS / 16; ++kg) {
+#pragma unroll
+                    for (int i = 0; i < DB; ++i) {
+                        using Lds = __attribute__((address_space(3))) Short4;
+                        const char* at = tile + atV[i] + kg * 16 * RB;
+                        const Short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at));
+                        const Short4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at + 8 * RB));
+                        const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                        o[i] = mfma(__builtin_bit_cast(P, both), w[kg], o[i]);
+                    }
                 }
             }
         }

@@ -101,7 +101,7 @@ typedef struct mlkd_norm_rope {
     int64_t tokens, out_rows;            /* rows of q, k, v; rows of k_out and v_out */
     int64_t q_stride, k_stride, v_stride, q_out_stride, k_out_stride, v_out_stride;
     double eps;
-    const double* quarters;              /* host memory: theta^(-2 i / rot) in quarter turns, rot / 2 of them */
+    double power[7];                     /* theta^(-2 2^k / rot): pair i turns by the product of its bits' powers */
 } mlkd_norm_rope;
 
 /// out = softmax(scale q k^T) v over packed sequences, and lse, the log of

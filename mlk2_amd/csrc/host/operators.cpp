@@ -236,9 +236,7 @@ bool normRope(Reader& r, OperatorStep& o) {
     if (rot % 2 != 0) return r.fail("rot must be even");
     o.rot = static_cast<int32_t>(rot);
     o.interleaved = inter != 0;
-    for (int64_t i = 0; i < rot / 2; ++i) {
-        o.quarters.push_back(std::pow(theta, -2.0 * static_cast<double>(i) / static_cast<double>(rot)) * (2.0 / M_PI));
-    }
+    for (int k = 0; k < 7 && rot > 0; ++k) o.power[k] = std::pow(theta, -2.0 * (1 << k) / static_cast<double>(rot));
     int64_t section[3] = {0, 0, 0};
     if (!r.whole("section_0", rot / 2, 0, kMaxDim, section[0]) || !r.whole("section_1", 0, 0, kMaxDim, section[1]) ||
         !r.whole("section_2", 0, 0, kMaxDim, section[2])) {
@@ -365,7 +363,7 @@ void fillNormRope(const KernelModule& km, const Step& st, const std::vector<void
     p.k_out_stride = o.op[kOpKOut].width;
     p.v_out_stride = o.op[kOpVOut].width;
     p.eps = o.eps;
-    p.quarters = o.quarters.data();
+    for (int k = 0; k < 7; ++k) p.power[k] = o.power[k];
 }
 
 void fillAttention(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_attention& p) {

@@ -36,7 +36,7 @@ struct OperatorStep {
     int32_t rot{0}, axes{1}, sections[3]{0, 0, 0};
     bool interleaved{false}, causal{true};
     double scale{0.0}, eps{0.0};
-    std::vector<double> quarters;   // frequency of each pair, in quarter turns per position
+    double power[7]{};   // theta^(-2 2^k / rot)
 };
 
 /// One read or write of a buffer over an R-dim box: element (v0..vR-1),
