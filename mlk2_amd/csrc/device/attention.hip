@@ -174,7 +174,7 @@ bool tilesApply(const mlkd_attention* p) {
 constexpr int keysOf(int size, int dt, int waves) { return waves > 1 && size == 2 && dt <= 128 ? 64 : 32; }
 constexpr int stagesOf(int size, int dt, int waves) {
     const int bytes = 2 * keysOf(size, dt, waves) * (dt <= 64 ? 64 : dt <= 128 ? 128 : 256) * size;   // of a tile
-    return waves > 1 ? (bytes <= 32768 ? 3 : 2) : bytes <= 16384 ? 4 : 2;
+    return waves > 1 ? (bytes <= 32768 ? 4 : 2) : bytes <= 16384 ? 4 : 2;
 }
 constexpr int wideOf(int size, int dt) { return size == 2 && dt <= 128 ? 8 : 4; }
 int dimOf(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }

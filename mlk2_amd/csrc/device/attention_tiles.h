@@ -6,6 +6,8 @@
 
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "attention_span.h"
 
 namespace mlk {
@@ -108,7 +110,7 @@ struct Tiles {
     static_assert(STAGES == 2 || (STAGES - 2) * 2 * IPW <= 63, "the loads waited on by number fit the counter");
 
     static __device__ __forceinline__ void dma(const void* base, uint32_t off, uint32_t m0) {
-        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(m0) : "memory");
+        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory");
     }
 
     static __device__ __forceinline__ int swizzle(int half, int row) {
@@ -171,6 +173,7 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
     using V4 = Vec4<T>;
     using Short4 = short __attribute__((ext_vector_type(4)));
     constexpr int KS = S::KS, DB = S::DB, RB = S::RB, KB = S::KB;
+    constexpr bool PING = NW == 8;
     extern __shared__ __align__(16) char ldsTiles[];
     const mlkd_attention& p = a.p;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
@@ -197,8 +200,8 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         return p.causal != 0 ? min(max(min(r, rows - 1) / group + s.nk - s.nq + 1, 0), nk) : nk;
     };
     const int tilesP = (np + KEYS - 1) / KEYS, tiles = tilesP + (limit(r0 + S::kRows - 1) + KEYS - 1) / KEYS;
-    const int first = static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits);
-    const int end = static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits);
+    const int first = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits));
+    const int end = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits));
     const int rw = r0 + wave * 32;                       // this wave's first row
     const int limLo = limit(rw), limHi = limit(rw + 31);
     const int r = min(rw + l32, rows - 1), lim = limit(r), head = g * group + r % group;
@@ -256,151 +259,201 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         atV[i] = S::kTile + vr * RB + (((byte >> 4) ^ swizzleV<T, RB>(vr)) << 4) + (byte & 15);
     }
 
-    f32x16 o[DB];
+    f32x16 o[DB] = {};
     float m = kLowest, l = 0.0f;   // of this lane's query; l of this lane's keys
-    // Only a second pass is careful: a weight of 0 takes an infinite or NaN
-    // value to NaN, so where a row of the first came out non-finite, the tiles
-    // that hide keys from some rows are summed key by key, hidden ones left out.
-    for (int careful = 0; careful < 2; ++careful) {
+    auto place = [&](int it) { return ldsTiles + (it - first) % STAGES * S::kStage; };
+    auto firstKey = [&](int it) { return (it < tilesP ? it : it - tilesP) * KEYS; };
+    // Scores of a tile.
+    f32x16 x[KB];
+    auto scores = [&](int it) {
+        const char* tile = place(it);
+        uint32_t lane = atK;
+        if (KS > 8) asm volatile("" : "+v"(lane));   // taken anew for each tile, where 16 of them take registers
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            x[kb] = f32x16{};
+#pragma unroll
+            for (int i = 0; i < KS; ++i) x[kb] = mfma(*reinterpret_cast<const P*>(tile + kb * 32 * RB + (lane ^ (i << 5))), q[i], x[kb]);
+        }
+    };
+    // Their weights, in place for f32, else rounded to the type.
+    P w[sizeof(T) == 4 ? 1 : KEYS / 16];
+    auto weights = [&](int it) {
+        const int j0 = firstKey(it);
+        if ((it < tilesP ? np : limLo) < j0 + KEYS) {
+            const int seen = (it < tilesP ? np : lim) - j0 - 4 * hl;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[kb][e] = kb * 32 + 8 * (e / 4) + e % 4 < seen ? x[kb][e] : -INFINITY;
+            }
+        }
+        float top = x[0][0];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, x[kb][e]);
+        }
+        top = fmaxf(top, otherHalf(top)) * c;
+        while (__any(top > m + 8.0f)) {   // once at most; as an if it has out copied in every tile
+            const float base = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - base);
+            m = base;
+            l *= keep;
+#pragma unroll
+            for (int i = 0; i < DB; ++i) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] *= keep;
+            }
+        }
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][e], c, -m));
+                l += v;
+                if constexpr (sizeof(T) == 4) x[kb][e] = v;
+                else w[kb * 2 + e / 8][e % 8] = static_cast<T>(v);
+            }
+        }
+    };
+    // The weights' sums of values.
+    auto values = [&](int it) {
+        const char* tile = place(it);
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+#pragma unroll
+                    for (int i = 0; i < DB; ++i) {
+                        const float v = *reinterpret_cast<const float*>(tile + atV[i] + (kb * 32 + 8 * (e / 4) + e % 4) * RB);
+                        o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, x[kb][e], o[i], 0, 0, 0);
+                    }
+                }
+            }
+        } else {
+#pragma unroll
+            for (int kg = 0; kg < KEYS / 16; ++kg) {
+#pragma unroll
+                for (int i = 0; i < DB; ++i) {
+                    using Lds = __attribute__((address_space(3))) Short4;
+                    const char* at = tile + atV[i] + kg * 16 * RB;
+                    const Short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at));
+                    const Short4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at + 8 * RB));
+                    const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[i] = mfma(__builtin_bit_cast(P, both), w[kg], o[i]);
+                }
+            }
+        }
+    };
+    // Waits for this wave's part of tile `it`, where those up to `it` + STAGES -
+    // 3 have been asked for.
+    auto arrived = [&](int it) { S::wait(max(0, min(STAGES - 3, end - 1 - it))); };
+    auto barrier = [] {
+        __builtin_amdgcn_sched_barrier(0);
+        if (NW > 1) __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const int mine = min(end, tilesP + (limHi + KEYS - 1) / KEYS);   // this wave's last tile, and one
+    // A tile takes two phases: its weights on the vector units, then its values
+    // and the next tile's scores on the matrix cores. Of eight waves, two on
+    // each SIMD, the second four run half a tile late: while one wave of a SIMD
+    // is in one phase, the other is in the other.
+    const bool late = PING && wave >= NW / 2;
+    if constexpr (STAGES == 2) {   // no room to have the next tile's keys early
+        if (first < end) load(first);
+        for (int it = first; it < end; ++it) {
+            S::wait(0);
+            barrier();
+            if (it + 1 < end) load(it + 1);
+            if (it >= mine) continue;
+            scores(it);
+            weights(it);
+            values(it);
+        }
+    } else if (first < end) {
+        for (int it = first; it < min(first + STAGES - 1, end); ++it) load(it);
+        S::wait(min(STAGES - 2, end - 1 - first));
+        barrier();
+        if (first < mine) scores(first);
+        if (late) {
+            arrived(first + 1);
+            barrier();
+        }
+        for (int it = first; it < end; ++it) {
+            if (it < mine) weights(it);
+            if (!late) arrived(it + 1);
+            barrier();
+            if (it + STAGES - 1 < end) load(it + STAGES - 1);
+            __builtin_amdgcn_s_setprio(1);
+            if (it < mine) values(it);
+            if (it + 1 < mine) scores(it + 1);
+            __builtin_amdgcn_s_setprio(0);
+            if (PING) {
+                if (late) arrived(it + 2);
+                barrier();
+            }
+        }
+        if (PING && !late) barrier();
+    }
+    // A weight of 0 takes an infinite or NaN value to NaN: where a row came out
+    // non-finite, the block is summed again key by key, hidden keys left out.
+    bool bad = !(fabsf(l) < INFINITY);
+#pragma unroll
+    for (int i = 0; i < DB; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) bad |= !(fabsf(o[i][e]) < INFINITY);
+    }
+    if (__syncthreads_or(bad)) {
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[i] = f32x16{};
         m = kLowest;
         l = 0.0f;
-        for (int it = first; it < min(first + STAGES - 1, end); ++it) load(it);
         for (int it = first; it < end; ++it) {
-            S::wait(min(end - 1 - it, STAGES - 2));
-            if (NW > 1) __builtin_amdgcn_s_barrier();
-            if (it + STAGES - 1 < end) load(it + STAGES - 1);
-            const bool pre = it < tilesP;
-            const int j0 = (pre ? it : it - tilesP) * KEYS;         // first key
-            if ((pre ? np : limHi) <= j0) continue;
-            const bool hides = (pre ? np : limLo) < j0 + KEYS;
-            const int seen = (pre ? np : lim) - j0;                  // keys of the tile that this row sees
-            const char* tile = ldsTiles + (it - first) % STAGES * S::kStage;
-            if (careful != 0 && hides) {
-                const int n = min((pre ? np : nk) - j0, KEYS);
-                for (int j = 0; j < n; ++j) {
-                    float x = 0.0f;
+            load(it);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const char* tile = place(it);
+            const int j0 = firstKey(it), seen = (it < tilesP ? np : lim) - j0;
+            const int n = it < mine ? min((it < tilesP ? np : nk) - j0, KEYS) : 0;
+            for (int j = 0; j < n; ++j) {
+                float s = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < KS; ++i) {
-                        const P kk = *reinterpret_cast<const P*>(tile + j * RB + (((2 * i + hl) ^ swizzleK<RB>(j)) << 4));
-                        // This path is rare: no registers for its sake, so that
-                        // its conversions of q stay where they are.
-                        f32x4 bits = __builtin_bit_cast(f32x4, q[i]);
-                        asm volatile("" : "+v"(bits));
-                        const P qq = __builtin_bit_cast(P, bits);
+                for (int i = 0; i < KS; ++i) {
+                    const P kk = *reinterpret_cast<const P*>(tile + j * RB + (((2 * i + hl) ^ swizzleK<RB>(j)) << 4));
+                    // This path is rare: no registers for its sake, so that
+                    // its conversions of q stay where they are.
+                    f32x4 bits = __builtin_bit_cast(f32x4, q[i]);
+                    asm volatile("" : "+v"(bits));
+                    const P qq = __builtin_bit_cast(P, bits);
 #pragma unroll
-                        for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) x += static_cast<float>(qq[e]) * static_cast<float>(kk[e]);
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                    x += otherHalf(x);
-                    if (j >= seen) x = -INFINITY;
-                    const float top = fmaxf(m, x * c), keep = __builtin_amdgcn_exp2f(m - top);
-                    const float w = __builtin_amdgcn_exp2f(x * c - top);
-                    m = top;
-                    l = l * keep + (hl == 0 ? w : 0.0f);
-                    const float wt = static_cast<float>(static_cast<T>(w));
-#pragma unroll
-                    for (int i = 0; i < DB; ++i) {
-#pragma unroll
-                        for (int e = 0; e < 16; e += 4) {
-                            const int byte = (32 * i + 2 * e + 4 * hl) * static_cast<int>(sizeof(T));
-                            const V4 vv = *reinterpret_cast<const V4*>(tile + S::kTile + j * RB + (((byte >> 4) ^ swizzleV<T, RB>(j)) << 4) + (byte & 15));
-#pragma unroll
-                            for (int f = 0; f < 4; ++f) {
-                                const float old = o[i][e + f] * keep;
-                                o[i][e + f] = j < seen ? old + wt * static_cast<float>(vv[f]) : old;
-                            }
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    }
+                    for (int e = 0; e < 16 / static_cast<int>(sizeof(T)); ++e) s += static_cast<float>(qq[e]) * static_cast<float>(kk[e]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-                continue;
-            }
-            f32x16 x[KB];
-            uint32_t lane = atK;
-            if (KS > 8) asm volatile("" : "+v"(lane));   // taken anew for each tile, where 16 of them take registers
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                x[kb] = f32x16{};
-#pragma unroll
-                for (int i = 0; i < KS; ++i) x[kb] = mfma(*reinterpret_cast<const P*>(tile + kb * 32 * RB + (lane ^ (i << 5))), q[i], x[kb]);
-            }
-            if (hides) {
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        if (kb * 32 + 8 * (e / 4) + e % 4 + 4 * hl >= seen) x[kb][e] = -INFINITY;
-                    }
-                }
-            }
-            float top = x[0][0];
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-                for (int e = 0; e < 16; ++e) top = fmaxf(top, x[kb][e]);
-            }
-            top = fmaxf(top, otherHalf(top)) * c;
-            if (__any(top > m + 8.0f)) {
-                const float base = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - base);
-                m = base;
-                l *= keep;
+                s += otherHalf(s);
+                if (j >= seen) s = -INFINITY;
+                const float top = fmaxf(m, s * c), keep = __builtin_amdgcn_exp2f(m - top);
+                const float u = __builtin_amdgcn_exp2f(s * c - top);
+                m = top;
+                l = l * keep + (hl == 0 ? u : 0.0f);
+                const float ut = static_cast<float>(static_cast<T>(u));
 #pragma unroll
                 for (int i = 0; i < DB; ++i) {
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) o[i][e] *= keep;
-                }
-            }
-            if constexpr (sizeof(T) == 4) {
+                    for (int e = 0; e < 16; e += 4) {
+                        const int byte = (32 * i + 2 * e + 4 * hl) * static_cast<int>(sizeof(T));
+                        const V4 vv = *reinterpret_cast<const V4*>(tile + S::kTile + j * RB + (((byte >> 4) ^ swizzleV<T, RB>(j)) << 4) + (byte & 15));
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        x[kb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kb][e], c, -m));
-                        l += x[kb][e];
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-#pragma unroll
-                        for (int i = 0; i < DB; ++i) {
-                            const float v = *reinterpret_cast<const float*>(tile + atV[i] + (kb * 32 + 8 * (e / 4) + e % 4) * RB);
-                            o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, x[kb][e], o[i], 0, 0, 0);
+                        for (int f = 0; f < 4; ++f) {
+                            const float old = o[i][e + f] * keep;
+                            o[i][e + f] = j < seen ? old + ut * static_cast<float>(vv[f]) : old;
                         }
-                    }
-                }
-            } else {
-                P w[KEYS / 16];
-#pragma unroll
-                for (int kg = 0; kg < KEYS / 16; ++kg) {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float v = __builtin_amdgcn_exp2f(__builtin_fmaf(x[kg / 2][kg % 2 * 8 + e], c, -m));
-                        l += v;
-                        w[kg][e] = static_cast<T>(v);
-                    }
-                }
-#pragma unroll
-                for (int kg = 0; kg < KEYS / 16; ++kg) {
-#pragma unroll
-                    for (int i = 0; i < DB; ++i) {
-                        using Lds = __attribute__((address_space(3))) Short4;
-                        const char* at = tile + atV[i] + kg * 16 * RB;
-                        const Short4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at));
-                        const Short4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds*)(at + 8 * RB));
-                        const auto both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                        o[i] = mfma(__builtin_bit_cast(P, both), w[kg], o[i]);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
                 }
             }
+            __syncthreads();
         }
-        bool bad = !(fabsf(l) < INFINITY);
-#pragma unroll
-        for (int i = 0; i < DB; ++i) {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) bad |= !(fabsf(o[i][e]) < INFINITY);
-        }
-        if (careful != 0 || !__syncthreads_or(bad)) break;
     }
 
     l += otherHalf(l);
