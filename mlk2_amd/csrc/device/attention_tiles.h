@@ -43,6 +43,17 @@ __device__ __forceinline__ float otherHalf(float v) {
     return __builtin_bit_cast(float, (threadIdx.x & 32) != 0 ? r[0] : r[1]);
 }
 
+/// Orders a block of NV products of two LDS reads each and NK of one each:
+/// every product's reads AHEAD products before it.
+template <int NV, int NK, int AHEAD, int J = -1>
+__device__ __forceinline__ void readAhead() {
+    constexpr int reads = J >= 0 ? (J + AHEAD < NV ? 2 : J + AHEAD < NV + NK ? 1 : 0)
+                          : AHEAD <= NV ? 2 * AHEAD : NV + (AHEAD < NV + NK ? AHEAD : NV + NK);
+    if constexpr (J >= 0) __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    if constexpr (reads > 0) __builtin_amdgcn_sched_group_barrier(0x100, reads, 0);
+    if constexpr (J + 1 < NV + NK) readAhead<NV, NK, AHEAD, J + 1>();
+}
+
 /// What a launch of tiles works on: which keys, which rows, and where the
 /// results go.
 struct TileArgs {
@@ -315,6 +326,19 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
                 else w[kb * 2 + e / 8][e % 8] = static_cast<T>(v);
             }
         }
+        // They are taken here: the compiler would move them behind the barrier, to their use.
+        asm volatile("" : "+v"(l));
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) asm volatile("" : "+v"(x[kb]));
+        } else {
+#pragma unroll
+            for (int kg = 0; kg < KEYS / 16; ++kg) {
+                f32x4 bits = __builtin_bit_cast(f32x4, w[kg]);
+                asm volatile("" : "+v"(bits));
+                w[kg] = __builtin_bit_cast(P, bits);
+            }
+        }
     };
     // The weights' sums of values.
     auto values = [&](int it) {
@@ -380,19 +404,38 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
             arrived(first + 1);
             barrier();
         }
-        for (int it = first; it < end; ++it) {
-            if (it < mine) weights(it);
+        auto before = [&](int it) {
             if (!late) arrived(it + 1);
             barrier();
             if (it + STAGES - 1 < end) load(it + STAGES - 1);
             __builtin_amdgcn_s_setprio(1);
-            if (it < mine) values(it);
-            if (it + 1 < mine) scores(it + 1);
+        };
+        auto after = [&](int it) {
             __builtin_amdgcn_s_setprio(0);
             if (PING) {
                 if (late) arrived(it + 2);
                 barrier();
             }
+        };
+        int it = first;
+        for (; it + 1 < mine; ++it) {
+            weights(it);
+            before(it);
+            values(it);
+            scores(it + 1);
+            if constexpr (sizeof(T) == 2) readAhead<KEYS / 16 * DB, KB * KS, 6>();
+            after(it);
+        }
+        if (it < mine) {
+            weights(it);
+            before(it);
+            values(it);
+            if constexpr (sizeof(T) == 2) readAhead<KEYS / 16 * DB, 0, 6>();
+            after(it++);
+        }
+        for (; it < end; ++it) {
+            before(it);
+            after(it);
         }
         if (PING && !late) barrier();
     }
