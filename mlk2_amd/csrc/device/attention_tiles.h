@@ -240,22 +240,35 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         for (int i = threadIdx.x * 16; i < S::kLds; i += NW * 64 * 16) *reinterpret_cast<f32x4*>(ldsTiles + i) = f32x4{};
         __syncthreads();
     }
-    const uint32_t ksOwn = static_cast<uint32_t>(p.k_stride * sizeof(T)), vsOwn = static_cast<uint32_t>(p.v_stride * sizeof(T));
-    const T* kOwn = static_cast<const T*>(p.k) + s.k0 * p.k_stride + g * p.dim;
-    const T* vOwn = static_cast<const T*>(p.v) + s.k0 * p.v_stride + g * p.dim;
-    const T* kPre = static_cast<const T*>(p.prefix_k) + g * p.dim;
-    const T* vPre = static_cast<const T*>(p.prefix_v) + g * p.dim;
+    // The next tile to load: its rows, how many of its keys are left, its place.
+    struct Next {
+        const char *k, *v;
+        uint32_t ks, vs;   // bytes from row to row
+        int left, at;
+    };
+    auto rowsFrom = [&](const void* k, const void* v, int64_t ks, int64_t vs, int64_t row, int left) {
+        constexpr int64_t size = sizeof(T);
+        return Next{static_cast<const char*>(k) + (row * ks + static_cast<int64_t>(g) * p.dim) * size,
+                    static_cast<const char*>(v) + (row * vs + static_cast<int64_t>(g) * p.dim) * size,
+                    static_cast<uint32_t>(ks * size), static_cast<uint32_t>(vs * size), left, 0};
+    };
+    auto start = [&](int it) {
+        const int64_t j = static_cast<int64_t>(it < tilesP ? it : it - tilesP) * KEYS;
+        return it < tilesP ? rowsFrom(p.prefix_k, p.prefix_v, p.prefix_k_stride, p.prefix_v_stride, j, np - static_cast<int>(j))
+                           : rowsFrom(p.k, p.v, p.k_stride, p.v_stride, s.k0 + j, nk - static_cast<int>(j));
+    };
+    Next next = start(first);
     auto load = [&](int it) {
-        const uint32_t lds = lds0 + (it - first) % STAGES * S::kStage;
-        if (it < tilesP) {
-            S::load(kPre + static_cast<int64_t>(it) * KEYS * p.prefix_k_stride, vPre + static_cast<int64_t>(it) * KEYS * p.prefix_v_stride,
-                    static_cast<uint32_t>(p.prefix_k_stride * sizeof(T)), static_cast<uint32_t>(p.prefix_v_stride * sizeof(T)),
-                    np - it * KEYS - 1, pieces, lds, wave);
-        } else {
-            const int t = it - tilesP;
-            S::load(kOwn + static_cast<int64_t>(t) * KEYS * p.k_stride, vOwn + static_cast<int64_t>(t) * KEYS * p.v_stride, ksOwn, vsOwn,
-                    nk - t * KEYS - 1, pieces, lds, wave);
+        if (it == tilesP && it > first) {   // from the prefix to the sequence's own keys
+            const int at = next.at;
+            next = start(it);
+            next.at = at;
         }
+        S::load(next.k, next.v, next.ks, next.vs, next.left - 1, pieces, lds0 + next.at, wave);
+        next.k += static_cast<uint64_t>(KEYS) * next.ks;
+        next.v += static_cast<uint64_t>(KEYS) * next.vs;
+        next.left -= KEYS;
+        next.at = next.at == (STAGES - 1) * S::kStage ? 0 : next.at + S::kStage;
     };
 
     // Offsets of this lane's reads within a tile.
@@ -297,6 +310,7 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
             for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) x[kb][e] = kb * 32 + 8 * (e / 4) + e % 4 < seen ? x[kb][e] : -INFINITY;
+                asm volatile("" : "+v"(x[kb]));   // a branch: selects would cost every tile a hundred instructions
             }
         }
         float top = x[0][0];
@@ -452,6 +466,7 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         for (int i = 0; i < DB; ++i) o[i] = f32x16{};
         m = kLowest;
         l = 0.0f;
+        next = start(first);
         for (int it = first; it < end; ++it) {
             load(it);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
