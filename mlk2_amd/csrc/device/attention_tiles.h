@@ -294,10 +294,11 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         uint32_t lane = atK;
         if (KS > 8) asm volatile("" : "+v"(lane));   // taken anew for each tile, where 16 of them take registers
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            x[kb] = f32x16{};
+        for (int kb = 0; kb < KB; ++kb) x[kb] = f32x16{};
 #pragma unroll
-            for (int i = 0; i < KS; ++i) x[kb] = mfma(*reinterpret_cast<const P*>(tile + kb * 32 * RB + (lane ^ (i << 5))), q[i], x[kb]);
+        for (int i = 0; i < KS; ++i) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) x[kb] = mfma(*reinterpret_cast<const P*>(tile + kb * 32 * RB + (lane ^ (i << 5))), q[i], x[kb]);
         }
     };
     // Their weights, in place for f32, else rounded to the type.
@@ -384,9 +385,6 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
             }
         }
     };
-    // Waits for this wave's part of tile `it`, where those up to `it` + STAGES -
-    // 3 have been asked for.
-    auto arrived = [&](int it) { S::wait(max(0, min(STAGES - 3, end - 1 - it))); };
     auto barrier = [] {
         __builtin_amdgcn_sched_barrier(0);
         if (NW > 1) __builtin_amdgcn_s_barrier();
@@ -410,8 +408,16 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
             values(it);
         }
     } else if (first < end) {
-        for (int it = first; it < min(first + STAGES - 1, end); ++it) load(it);
-        S::wait(min(STAGES - 2, end - 1 - first));
+        // A wave asks for a tile so far ahead that all waves are done with the
+        // one in its place: in their weights of tile `it`, the late waves know
+        // the others to be past the values of it - 1, those know no more than
+        // that the late ones are at them.
+        const int ahead = NW == 1 || late ? STAGES - 1 : STAGES - 2;
+        // Waits for this wave's part of tile `it`, where the next STAGES - 3
+        // were asked for too.
+        auto arrived = [&](int it) { S::wait(max(0, min(NW == 1 ? STAGES - 2 : STAGES - 3, end - 1 - it))); };
+        for (int it = first; it < min(first + ahead, end); ++it) load(it);
+        S::wait(max(0, min(ahead, end - first) - 1));
         barrier();
         if (first < mine) scores(first);
         if (late) {
@@ -421,7 +427,6 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         auto before = [&](int it) {
             if (!late) arrived(it + 1);
             barrier();
-            if (it + STAGES - 1 < end) load(it + STAGES - 1);
             __builtin_amdgcn_s_setprio(1);
         };
         auto after = [&](int it) {
@@ -433,21 +438,24 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         };
         int it = first;
         for (; it + 1 < mine; ++it) {
+            if (it + ahead < end) load(it + ahead);
             weights(it);
             before(it);
             values(it);
             scores(it + 1);
-            if constexpr (sizeof(T) == 2) readAhead<KEYS / 16 * DB, KB * KS, 6>();
+            if constexpr (sizeof(T) == 2) readAhead<KEYS / 16 * DB, KB * KS, 4>();
             after(it);
         }
         if (it < mine) {
+            if (it + ahead < end) load(it + ahead);
             weights(it);
             before(it);
             values(it);
-            if constexpr (sizeof(T) == 2) readAhead<KEYS / 16 * DB, 0, 6>();
+            if constexpr (sizeof(T) == 2) readAhead<KEYS / 16 * DB, 0, 4>();
             after(it++);
         }
         for (; it < end; ++it) {
+            if (it + ahead < end) load(it + ahead);
             before(it);
             after(it);
         }
