@@ -114,44 +114,71 @@ __global__ __launch_bounds__(256) void attentionRows(mlkd_attention p) {
 }
 
 /// The results of key ranges joined: out = sum acc_i 2^(m_i - m) / sum l_i
-/// 2^(m_i - m), m the largest maximum. LPR lanes a row, 4 columns each.
+/// 2^(m_i - m), m the largest maximum. A wave a row, LPR lanes to a range with 4
+/// columns each, so that ranges are read side by side; four in flight.
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void attentionJoin(mlk::TileArgs a) {
     const mlkd_attention& p = a.p;
     using mlk::f32x4;
-    const int ln = threadIdx.x % LPR;
+    constexpr int SIDE = 64 / LPR;
+    const int ln = threadIdx.x & 63, column = ln % LPR * 4;
     const int64_t rows = p.q_rows * p.heads;
-    for (int64_t r = blockIdx.x * int64_t{256 / LPR} + threadIdx.x / LPR; r < rows; r += static_cast<int64_t>(gridDim.x) * (256 / LPR)) {
+    for (int64_t r = blockIdx.x * int64_t{4} + threadIdx.x / 64; r < rows; r += static_cast<int64_t>(gridDim.x) * 4) {
         const int64_t t = r / p.heads;
         if (sequenceOf(p, t) < 0) continue;
-        float m = mlk::kLowest;
-        for (int i = 0; i < a.parts; ++i) m = fmaxf(m, a.ml[i * rows + r].x);
-        float l = 0.0f;
+        // The weights of the ranges, lane i those of i and 64 + i; below 0: a
+        // range without keys, its sums may not have been written.
+        float2 ml[2];
+        float w[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) ml[h] = ln + 64 * h < a.parts ? a.ml[(ln + 64 * h) * rows + r] : make_float2(mlk::kLowest, 0.0f);
+        const float m = waveMax(fmaxf(ml[0].x, ml[1].x));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[h] = __builtin_amdgcn_exp2f(ml[h].x - m);
+        const float l = waveSum(ml[0].y * w[0] + ml[1].y * w[1]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) w[h] = ml[h].y == 0.0f ? -1.0f : w[h];
         f32x4 sum = {};
-        for (int i = 0; i < a.parts; ++i) {
-            const float2 ml = a.ml[i * rows + r];
-            if (ml.y == 0.0f) continue;   // no weights: its sums may not have been written
-            const float w = __builtin_amdgcn_exp2f(ml.x - m);
-            l += ml.y * w;
-            if (4 * ln < p.dim) sum += w * *reinterpret_cast<const f32x4*>(a.acc + (i * rows + r) * p.dim + 4 * ln);
+        const float* from = a.acc + r * p.dim + column;
+        for (int i0 = 0; i0 < a.parts; i0 += 4 * SIDE) {
+            f32x4 v[4];
+            float u[4];
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const int i = i0 + n * SIDE + ln / LPR;
+                u[n] = __shfl(i0 + n * SIDE < 64 ? w[0] : w[1], i & 63);
+                v[n] = f32x4{};
+                if (i < a.parts && u[n] >= 0.0f && column < p.dim) v[n] = *reinterpret_cast<const f32x4*>(from + i * rows * p.dim);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) sum += fmaxf(u[n], 0.0f) * v[n];
+        }
+#pragma unroll
+        for (int d = LPR; d < 64; d *= 2) {
+#pragma unroll
+            for (int f = 0; f < 4; ++f) sum[f] += __shfl_xor(sum[f], d);
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        if (4 * ln < p.dim) {
+        if (column < p.dim && ln < LPR) {
             mlk::Vec4<T> v;
 #pragma unroll
             for (int f = 0; f < 4; ++f) v[f] = static_cast<T>(sum[f] * inv);
-            *reinterpret_cast<mlk::Vec4<T>*>(static_cast<T*>(p.out) + t * p.out_stride + (r % p.heads) * p.dim + 4 * ln) = v;
+            *reinterpret_cast<mlk::Vec4<T>*>(static_cast<T*>(p.out) + t * p.out_stride + (r % p.heads) * p.dim + column) = v;
         }
         if (p.lse != nullptr && ln == 0) p.lse[r] = l == 0.0f ? -INFINITY : (m + log2f(l)) * kLn2;
     }
 }
+
+/// Row blocks of the matrix-core kernels: one wave of 32 rows; eight waves in
+/// two groups, 128 rows; the widest, see wavesOf.
+enum Block { kNarrow, kHalves, kWide };
 
 /// How a launch runs: on the matrix cores or row by row, with which row
 /// blocks, in how many key ranges.
 struct Plan {
     bool tiles{false};
     bool shared{false};     // the prefix for all sequences' rows together
-    int wavesOwn{0}, wavesPrefix{0};   // of a row block, 32 rows each
+    Block own{kNarrow}, prefix{kNarrow};
     int splitsOwn{1}, splitsPrefix{0};
     int parts() const { return splitsOwn + splitsPrefix > 1 ? splitsOwn + splitsPrefix : 0; }
 };
@@ -166,17 +193,21 @@ bool tilesApply(const mlkd_attention* p) {
     if (p->dim % 8 != 0) return false;
     if (p->q_rows * (p->heads / p->kv_heads) >= (int64_t{1} << 30)) return false;   // rows are counted in 32 bits
     return aligned(p->q, p->q_stride, 16, size) && aligned(p->k, p->k_stride, 16, size) && aligned(p->v, p->v_stride, 16, size) &&
-           aligned(p->out, p->out_stride, 4 * size, size) && aligned(p->prefix_k, p->prefix_k_stride, 16, size) &&
+           aligned(p->out, p->out_stride, 16, size) && aligned(p->prefix_k, p->prefix_k_stride, 16, size) &&
            aligned(p->prefix_v, p->prefix_v_stride, 16, size);
 }
 
-/// Tiles of the matrix-core kernels: keys a tile and tiles in LDS.
-constexpr int keysOf(int size, int dt, int waves) { return waves > 1 && size == 2 && dt <= 128 ? 64 : 32; }
-constexpr int stagesOf(int size, int dt, int waves) {
-    const int bytes = 2 * keysOf(size, dt, waves) * (dt <= 64 ? 64 : dt <= 128 ? 128 : 256) * size;   // of a tile
-    return waves > 1 ? (bytes <= 32768 ? 4 : 2) : bytes <= 16384 ? 4 : 2;
+/// The matrix-core kernels: waves of a row block and their groups, keys of a
+/// tile, tiles in LDS.
+constexpr bool eight(int size, int dt) { return size == 2 && dt <= 128; }
+constexpr int wavesOf(Block block, int size, int dt) { return block == kNarrow ? 1 : eight(size, dt) ? 8 : 4; }
+constexpr int groupsOf(Block block) { return block == kHalves ? 2 : 1; }
+constexpr int keysOf(Block block, int size, int dt) { return wavesOf(block, size, dt) == 8 ? 64 : 32; }
+constexpr int stagesOf(Block block, int size, int dt) {
+    const int bytes = 2 * keysOf(block, size, dt) * (dt <= 64 ? 64 : dt <= 128 ? 128 : 256) * size;   // of a tile
+    return block != kNarrow ? (bytes <= 32768 ? 4 : 2) : size == 2 && bytes <= 16384 ? 4 : 2;
 }
-constexpr int wideOf(int size, int dt) { return size == 2 && dt <= 128 ? 8 : 4; }
+constexpr int rowsOf(Block block, int size, int dt) { return 32 * wavesOf(block, size, dt) / groupsOf(block); }
 int dimOf(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
 
 Plan planOf(const mlkd_attention* p) {
@@ -184,18 +215,43 @@ Plan planOf(const mlkd_attention* p) {
     n.tiles = tilesApply(p);
     if (!n.tiles) return n;
     const int64_t group = p->heads / p->kv_heads;
-    const int64_t each = (p->q_rows + p->sequences - 1) / p->sequences * group;   // rows of a sequence, on average
-    const int64_t keys = std::max<int64_t>(1, p->kv_rows / p->sequences);
-    const int wide = wideOf(p->dtype == MLKD_F32 ? 4 : 2, dimOf(p->dim));
-    n.wavesOwn = each > 64 ? wide : 1;
-    n.shared = p->prefix_k != nullptr && n.wavesOwn == 1;
-    auto ranges = [&](int64_t blocks, int64_t count, int64_t fill) {
-        return static_cast<int>(std::max<int64_t>(1, std::min({fill / std::max<int64_t>(1, blocks * p->kv_heads), count / 128, int64_t{64}})));
+    const int64_t tokens = (p->q_rows + p->sequences - 1) / p->sequences, each = tokens * group;   // rows of a sequence, on average
+    const int64_t keys = std::max<int64_t>(1, p->kv_rows / p->sequences), all = keys + (p->prefix_k != nullptr ? p->prefix_rows : 0);
+    const int size = p->dtype == MLKD_F32 ? 4 : 2, dt = dimOf(p->dim);
+    // Row blocks of all sequences' and all key/value heads', of rows of average sequences.
+    auto blocks = [&](int64_t count, int64_t rows, Block block) {
+        const int64_t of = rowsOf(block, size, dt);
+        return count * ((rows + of - 1) / of) * p->kv_heads;
     };
-    if (n.wavesOwn == 1) n.splitsOwn = ranges((p->q_rows * group + 31) / 32 + p->sequences - 1, keys, 1024);
+    auto ranges = [&](int64_t count, int64_t keys, int64_t fill) {
+        return static_cast<int>(std::max<int64_t>(1, std::min({fill / std::max<int64_t>(1, count), keys / 128, int64_t{64}})));
+    };
+    const int64_t narrow = blocks(p->sequences, each, kNarrow), wide = blocks(p->sequences, each, kWide);
+    // One wave to a block where a sequence has two blocks' rows at most, and, of
+    // 16-bit types, where there is little to do: 19 tokens over 1000 keys, 32 and
+    // 8 heads of 128, in 15 us against 26, 256 over 256 in 17 against 13.5.
+    const bool few = each <= 64 || (size == 2 && narrow * all <= 32768);
+    // Half the rows to a workgroup where whole blocks leave compute units idle:
+    // 1024 tokens, every key seen, in 29 us against 39, 1536 in 68 against 55.
+    // Where the rows see unlike numbers of keys, the shorter blocks also even
+    // out what the units do: 2048 tokens in 55 us against 57, 2304 in 75
+    // against 80, 4096 in 183 against 161.
+    const bool level = p->causal == 0 || all >= 2 * tokens;
+    if (few) n.own = kNarrow;
+    else if (eight(size, dt)) n.own = wide <= (level ? 128 : 320) ? kHalves : kWide;
+    // f32 takes its time in the products alone, 16 times those of 16 bits: one
+    // wave to a block and key ranges where blocks of four leave units idle (two
+    // sequences of 1001, 8 heads of 64: 51 us against 79; four, 16 heads: 182
+    // against 143).
+    else n.own = size == 4 && wide < 256 ? kNarrow : kWide;
+    n.shared = p->prefix_k != nullptr && each <= 64;
+    // Ranges of 128 keys and more, so many that each SIMD has a wave (f32, with
+    // two tiles in LDS: two).
+    if (n.own == kNarrow) n.splitsOwn = ranges(narrow, n.shared ? keys : all, size == 4 ? 2048 : 1024);
     if (n.shared) {
-        n.wavesPrefix = wide;
-        n.splitsPrefix = ranges((p->q_rows * group + 32 * wide - 1) / (32 * wide), p->prefix_rows, 256);
+        const int64_t rows = p->q_rows * group;
+        n.prefix = eight(size, dt) && blocks(1, rows, kWide) <= 128 ? kHalves : kWide;
+        n.splitsPrefix = ranges(blocks(1, rows, n.prefix), p->prefix_rows, 256);
     }
     return n;
 }
@@ -211,40 +267,52 @@ Plan planFor(const mlkd_attention* p) {
     return n;
 }
 
-template <typename T, int DT, int NW>
-int launchTiles(const mlk::TileArgs& a, int64_t blocks, hipStream_t st) {
-    constexpr int KEYS = keysOf(sizeof(T), DT, NW), STAGES = stagesOf(sizeof(T), DT, NW);
-    constexpr int bytes = mlk::Tiles<T, DT, NW, KEYS, STAGES>::kLds;
-    auto* kernel = mlk::attentionTiles<T, DT, NW, KEYS, STAGES>;
+mlk::Divider dividerOf(int d) {
+    if (d == 1) return {0, 0};
+    int up = 0;
+    while ((int64_t{1} << up) < d) ++up;
+    return {static_cast<uint32_t>(((uint64_t{1} << (31 + up)) + d - 1) / d), up - 1};
+}
+
+/// The row blocks of a launch: at most so many for any lengths.
+int64_t rowBlocks(const mlk::TileArgs& a, int each) {
+    const int64_t rows = a.p.q_rows * (a.p.heads / a.p.kv_heads);
+    return a.all_rows != 0 ? (rows + each - 1) / each : rows / each + std::min<int64_t>(a.p.sequences, rows);
+}
+
+template <typename T, int DT, Block BLOCK>
+int launchTiles(mlk::TileArgs a, hipStream_t st) {
+    a.by_group = dividerOf(a.p.heads / a.p.kv_heads);
+    a.by_kv_heads = dividerOf(a.p.kv_heads);
+    a.by_splits = dividerOf(a.splits);
+    constexpr int NW = wavesOf(BLOCK, sizeof(T), DT), KG = groupsOf(BLOCK), KEYS = keysOf(BLOCK, sizeof(T), DT);
+    constexpr int STAGES = stagesOf(BLOCK, sizeof(T), DT), bytes = mlk::Tiles<T, DT, NW, KG, KEYS, STAGES>::kLds;
+    auto* kernel = mlk::attentionTiles<T, DT, NW, KG, KEYS, STAGES>;
     // Once per process; a function-local static initializes thread-safely.
     static const bool allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                     bytes) == hipSuccess;
     if (!allowed) return MLKD_RT_LAUNCH;
-    const int64_t grid = blocks * a.splits * a.p.kv_heads;
+    const int64_t grid = rowBlocks(a, rowsOf(BLOCK, sizeof(T), DT)) * a.splits * a.p.kv_heads;
     if (grid * NW * 64 >= (int64_t{1} << 32)) return -1;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(NW * 64), bytes, st, a);
     return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
 }
 
-/// The row blocks of a launch: at most so many for any lengths.
-int64_t rowBlocks(const mlk::TileArgs& a, int waves) {
-    const int64_t rows = a.p.q_rows * (a.p.heads / a.p.kv_heads), each = 32 * waves;
-    return a.all_rows != 0 ? (rows + each - 1) / each : rows / each + std::min<int64_t>(a.p.sequences, rows);
-}
-
 template <typename T, int DT>
-int launchWaves(const mlk::TileArgs& a, int waves, hipStream_t st) {
-    constexpr int WIDE = wideOf(sizeof(T), DT);
-    return waves == 1 ? launchTiles<T, DT, 1>(a, rowBlocks(a, 1), st) : launchTiles<T, DT, WIDE>(a, rowBlocks(a, WIDE), st);
+int launchBlock(const mlk::TileArgs& a, Block block, hipStream_t st) {
+    if constexpr (eight(sizeof(T), DT)) {
+        if (block == kHalves) return launchTiles<T, DT, kHalves>(a, st);
+    }
+    return block == kNarrow ? launchTiles<T, DT, kNarrow>(a, st) : launchTiles<T, DT, kWide>(a, st);
 }
 
 template <typename T>
-int launchDim(const mlk::TileArgs& a, int waves, hipStream_t st) {
+int launchDim(const mlk::TileArgs& a, Block block, hipStream_t st) {
     switch (dimOf(a.p.dim)) {
-        case 64: return launchWaves<T, 64>(a, waves, st);
-        case 96: return launchWaves<T, 96>(a, waves, st);
-        case 128: return launchWaves<T, 128>(a, waves, st);
-        default: return launchWaves<T, 256>(a, waves, st);
+        case 64: return launchBlock<T, 64>(a, block, st);
+        case 96: return launchBlock<T, 96>(a, block, st);
+        case 128: return launchBlock<T, 128>(a, block, st);
+        default: return launchBlock<T, 256>(a, block, st);
     }
 }
 
@@ -261,18 +329,17 @@ int launchPlan(const mlkd_attention* p, const Plan& n, hipStream_t st) {
         a.keys = 1;
         a.all_rows = 1;
         a.splits = n.splitsPrefix;
-        if (const int rc = launchDim<T>(a, n.wavesPrefix, st); rc != 0) return rc;
+        if (const int rc = launchDim<T>(a, n.prefix, st); rc != 0) return rc;
         a.part0 = n.splitsPrefix;
         a.all_rows = 0;
     }
     a.keys = n.shared ? 2 : 3;
     a.splits = n.splitsOwn;
-    if (const int rc = launchDim<T>(a, n.wavesOwn, st); rc != 0) return rc;
+    if (const int rc = launchDim<T>(a, n.own, st); rc != 0) return rc;
     if (a.parts == 0) return 0;
     const int64_t rows = p->q_rows * p->heads;
     auto* join = p->dim <= 64 ? attentionJoin<T, 16> : p->dim <= 128 ? attentionJoin<T, 32> : attentionJoin<T, 64>;
-    const int per = p->dim <= 64 ? 16 : p->dim <= 128 ? 8 : 4;
-    hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(std::min<int64_t>((rows + per - 1) / per, int64_t{1} << 20))), dim3(256), 0, st, a);
+    hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(std::min<int64_t>((rows + 3) / 4, int64_t{1} << 20))), dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
 }
 
@@ -295,11 +362,12 @@ const char* mlkd_attention_kernel_names(const mlkd_attention* p) {
         return name.c_str();
     }
     const int dt = dimOf(p->dim), size = p->dtype == MLKD_F32 ? 4 : 2;
-    auto tiles = [&](int waves) {
-        return "attentionTiles<" + type + ", " + std::to_string(dt) + ", " + std::to_string(waves) + ", " +
-               std::to_string(keysOf(size, dt, waves)) + ", " + std::to_string(stagesOf(size, dt, waves)) + ">";
+    auto tiles = [&](Block block) {
+        std::string s = "attentionTiles<" + type;
+        for (const int v : {dt, wavesOf(block, size, dt), groupsOf(block), keysOf(block, size, dt), stagesOf(block, size, dt)}) s += ", " + std::to_string(v);
+        return s + ">";
     };
-    name = n.shared ? tiles(n.wavesPrefix) + "+" + tiles(n.wavesOwn) : tiles(n.wavesOwn);
+    name = n.shared ? tiles(n.prefix) + "+" + tiles(n.own) : tiles(n.own);
     if (n.parts() > 0) name += "+attentionJoin<" + type + ", " + std::to_string(dt <= 64 ? 16 : dt <= 128 ? 32 : 64) + ">";
     return name.c_str();
 }

@@ -54,6 +54,16 @@ __device__ __forceinline__ void readAhead() {
     if constexpr (J + 1 < NV + NK) readAhead<NV, NK, AHEAD, J + 1>();
 }
 
+/// n / d for n < 2^30 by a product: mul = ceil(2^(31 + L) / d), 2^L the power
+/// of two at or above d, is off d's reciprocal by less than 2^L / 2^(31 + L).
+struct Divider {
+    uint32_t mul;   // 0: d is 1
+    int shift;      // L - 1
+};
+__device__ __forceinline__ int operator/(int n, const Divider& d) {
+    return d.mul == 0 ? n : static_cast<int>(__umulhi(static_cast<uint32_t>(n), d.mul) >> d.shift);
+}
+
 /// What a launch of tiles works on: which keys, which rows, and where the
 /// results go.
 struct TileArgs {
@@ -65,28 +75,51 @@ struct TileArgs {
     int parts;        // ... of so many (0: results go straight to out)
     float* acc;       // [parts][rows * heads][dim]
     float2* ml;       // [parts][rows * heads]: maximum (times log2 e), sum
+    Divider by_group, by_kv_heads, by_splits;
 };
+
+/// A value that all lanes have alike, in scalar registers.
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(static_cast<int>(v)), hi = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
+    return static_cast<int64_t>(hi) << 32 | lo;
+}
+
+__device__ __forceinline__ int64_t laneOf(int64_t v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), lane);
+    return static_cast<int64_t>(hi) << 32 | lo;
+}
+
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int addFrom(int v) {
+    return v + __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+
+/// The sum of the lanes up to and with this one.
+__device__ __forceinline__ int sumUpTo(int v) {
+    v = addFrom<0x111, 0xf>(v);   // rows of 16 lanes, from 1, 2, 4, 8 before
+    v = addFrom<0x112, 0xf>(v);
+    v = addFrom<0x114, 0xf>(v);
+    v = addFrom<0x118, 0xf>(v);
+    v = addFrom<0x142, 0xa>(v);   // the last lane of rows 0 and 2 to rows 1 and 3
+    return addFrom<0x143, 0xc>(v);   // lane 31 to rows 2 and 3
+}
 
 /// The row block `tile` counted from the end of the batch: its sequence and
 /// first row. Rows are (token, head of the group); each sequence has
-/// ceil(nq * group / rows) blocks. All lanes return the same; false past the
-/// first block.
-__device__ __forceinline__ bool rowBlock(const mlkd_attention& p, int group, int rows, int tile, int& b, int& r0) {
+/// ceil(nq * group / ROWS) blocks. A lane reads a sequence's lengths. All lanes
+/// return the same; false past the first block.
+template <int ROWS>
+__device__ __forceinline__ bool rowBlock(const mlkd_attention& p, int group, int tile, SeqSpan& s, int& r0) {
     const int ln = threadIdx.x & 63;
-    for (int s0 = 0; s0 < p.sequences; s0 += 64) {
-        const int s = p.sequences - 1 - s0 - ln;
-        const int mine = s >= 0 ? (spanOf(p, s).nq * group + rows - 1) / rows : 0;
-        int sum = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int v = __shfl_up(sum, d, 64);
-            sum += ln >= d ? v : 0;
-        }
+    for (int s0 = p.sequences - 1; s0 >= 0; s0 -= 64) {
+        SeqSpan of{};
+        if (s0 >= ln) of = spanOf(p, s0 - ln);
+        const int sum = sumUpTo((of.nq * group + ROWS - 1) / ROWS);
         const uint64_t past = __ballot(sum > tile);
         if (past != 0) {
             const int at = __builtin_ctzll(past);
-            b = __builtin_amdgcn_readfirstlane(p.sequences - 1 - s0 - at);
-            r0 = __builtin_amdgcn_readfirstlane((__builtin_amdgcn_readlane(sum, at) - 1 - tile) * rows);
+            s = SeqSpan{laneOf(of.q0, at), laneOf(of.k0, at), __builtin_amdgcn_readlane(of.nq, at), __builtin_amdgcn_readlane(of.nk, at)};
+            r0 = (__builtin_amdgcn_readlane(sum, at) - 1 - tile) * ROWS;
             return true;
         }
         tile -= __builtin_amdgcn_readlane(sum, 63);
@@ -107,16 +140,18 @@ __device__ __forceinline__ int swizzleV(int j) {
     return sizeof(T) == 4 ? (j >> 2 & 1) << 3 : RB == 128 ? (j >> 1 & 1) << 2 : (j & 3) << 2;
 }
 
-template <typename T, int DT, int NW, int KEYS, int STAGES>
+/// NW waves of 32 rows each, in KG groups: those of a group have different
+/// rows, the groups the same rows and different keys of a tile.
+template <typename T, int DT, int NW, int KG, int KEYS, int STAGES>
 struct Tiles {
     static constexpr int KS = DT * sizeof(T) / 32, DB = DT / 32;      // steps of q k^T, two pieces each; 32-column blocks of out
     static constexpr int RB = (DT <= 64 ? 64 : DT <= 128 ? 128 : 256) * sizeof(T);
     static constexpr int kTile = KEYS * RB;                          // bytes of a tile of keys
     static constexpr int kStage = 2 * kTile;
     static constexpr int kLds = STAGES * kStage;
-    static constexpr int kRows = 32 * NW;
+    static constexpr int kRows = 32 * NW / KG;
     static constexpr int IPW = kTile / 1024 / NW;                    // 1024-byte loads of a wave, for keys and again for values
-    static constexpr int KB = KEYS / 32;
+    static constexpr int kKeys = KEYS / KG, KB = kKeys / 32;         // keys of a tile that a wave takes
     static_assert(IPW >= 1 && IPW * NW * 1024 == kTile, "a tile is whole loads of the waves");
     static_assert(STAGES == 2 || (STAGES - 2) * 2 * IPW <= 63, "the loads waited on by number fit the counter");
 
@@ -128,35 +163,30 @@ struct Tiles {
         return half == 0 ? swizzleK<RB>(row) : swizzleV<T, RB>(row);
     }
 
-    /// This wave's loads of a tile, straight to LDS: rows past the last valid
-    /// one repeat it; pieces past the head dim stay zero.
-    static __device__ __forceinline__ void load(const void* k, const void* v, uint32_t ks, uint32_t vs, int last, int pieces, uint32_t lds, int wave) {
+    /// This wave's loads of a tile's keys (half 0) or values (1), straight to
+    /// LDS: rows past the last valid one repeat it; pieces past the head dim
+    /// stay zero.
+    static __device__ __forceinline__ void load(int half, const char* from, uint32_t stride, int last, int pieces, uint32_t lds, int wave) {
         constexpr int P = RB / 16, R = 64 / P;   // pieces of a row, rows of a load
+        from = reinterpret_cast<const char*>(uniform(reinterpret_cast<int64_t>(from)));
         int ln = threadIdx.x & 63;
         asm volatile("" : "+v"(ln));   // the offsets are taken anew for each tile: kept, they are up to 64 registers
         if (last >= KEYS - 1 && pieces == P) {
+            const int w0 = wave * IPW * R;
+            const uint32_t row = ln / P * stride, piece = ((ln % P) ^ swizzle(half, w0 + ln / P)) << 4;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const uint32_t stride = half == 0 ? ks : vs;
-                const char* base = static_cast<const char*>(half == 0 ? k : v) + static_cast<uint64_t>(wave * IPW * R) * stride;
-                const uint32_t row = ln / P * stride, piece = ((ln % P) ^ swizzle(half, wave * IPW * R + ln / P)) << 4;
-#pragma unroll
-                for (int i = 0; i < IPW; ++i) {
-                    // Rows i R + r with r < R: their swizzle is i R's and r's.
-                    const int w0 = wave * IPW * R, turned = swizzle(half, w0 + i * R) ^ swizzle(half, w0);
-                    dma(base + static_cast<uint64_t>(i * R) * stride, (piece ^ (turned << 4)) + row, lds + half * kTile + (wave * IPW + i) * 1024);
-                }
+            for (int i = 0; i < IPW; ++i) {
+                // Rows i R + r with r < R: their swizzle is i R's and r's.
+                const int turned = swizzle(half, w0 + i * R) ^ swizzle(half, w0);
+                dma(from + static_cast<uint64_t>(w0 + i * R) * stride, (piece ^ (turned << 4)) + row, lds + half * kTile + (wave * IPW + i) * 1024);
             }
             return;
         }
 #pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-#pragma unroll 1
-            for (int i = 0; i < IPW; ++i) {
-                const int n = wave * IPW + i, row = n * R + ln / P, piece = (ln % P) ^ swizzle(half, row);
-                const uint32_t off = static_cast<uint32_t>(min(row, last)) * (half == 0 ? ks : vs) + piece * 16;
-                if (piece < pieces) dma(half == 0 ? k : v, off, lds + half * kTile + n * 1024);
-            }
+        for (int i = 0; i < IPW; ++i) {
+            const int n = wave * IPW + i, row = n * R + ln / P, piece = (ln % P) ^ swizzle(half, row);
+            const uint32_t off = static_cast<uint32_t>(min(row, last)) * stride + piece * 16;
+            if (piece < pieces) dma(from, off, lds + half * kTile + n * 1024);
         }
     }
 
@@ -177,9 +207,9 @@ struct Tiles {
 /// transposing reads. The maximum that the weights are taken relative to
 /// follows the running one only when that has grown by 2^8: sums of weights
 /// up to 2^8 lose nothing in f32, and out is rescaled in few tiles.
-template <typename T, int DT, int NW, int KEYS, int STAGES>
-__global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(TileArgs a) {
-    using S = Tiles<T, DT, NW, KEYS, STAGES>;
+template <typename T, int DT, int NW, int KG, int KEYS, int STAGES>
+__global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : DT == 64 && sizeof(T) == 2 ? 4 : 2) void attentionTiles(TileArgs a) {
+    using S = Tiles<T, DT, NW, KG, KEYS, STAGES>;
     using P = Piece<T>;
     using V4 = Vec4<T>;
     using Short4 = short __attribute__((ext_vector_type(4)));
@@ -187,52 +217,39 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
     constexpr bool PING = NW == 8;
     extern __shared__ __align__(16) char ldsTiles[];
     const mlkd_attention& p = a.p;
-    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     const int ln = threadIdx.x & 63, l32 = ln & 31, hl = ln >> 5;
-    const int group = p.heads / p.kv_heads, g = static_cast<int>(blockIdx.x) % p.kv_heads;
-    int rest = static_cast<int>(blockIdx.x) / p.kv_heads;
-    const int split = rest % a.splits;
-    rest /= a.splits;
-    SeqSpan s;
-    int r0 = 0;
-    if (a.all_rows != 0) {
-        s = SeqSpan{0, 0, static_cast<int32_t>(p.q_rows), 0};
-        r0 = rest * S::kRows;
-        if (r0 >= s.nq * group) return;
-    } else {
-        int b = 0;
-        if (!rowBlock(p, group, S::kRows, rest, b, r0)) return;
-        s = spanOf(p, b);
-    }
+    const int id = static_cast<int>(blockIdx.x), of = id / a.by_kv_heads, g = id - of * p.kv_heads;
+    const int rest = of / a.by_splits, split = of - rest * a.splits, group = p.heads / p.kv_heads;
+    int np = (a.keys & 1) != 0 ? prefixOf(p) : 0;
+    SeqSpan s{0, 0, static_cast<int32_t>(p.q_rows), 0};
+    int r0 = rest * S::kRows;
+    if (a.all_rows != 0 ? r0 >= s.nq * group : !rowBlock<S::kRows>(p, group, rest, s, r0)) return;
+    s = SeqSpan{uniform(s.q0), uniform(s.k0), static_cast<int32_t>(uniform(s.nq)), static_cast<int32_t>(uniform(s.nk))};
+    r0 = __builtin_amdgcn_readfirstlane(r0);
+    np = __builtin_amdgcn_readfirstlane(np);
     const int rows = s.nq * group;
     // Keys that a row sees: the prefix, and own keys below lim = token + slope.
-    const int np = (a.keys & 1) != 0 ? prefixOf(p) : 0, nk = (a.keys & 2) != 0 ? s.nk : 0;
+    const int nk = (a.keys & 2) != 0 ? s.nk : 0;
     auto limit = [&](int r) {
-        return p.causal != 0 ? min(max(min(r, rows - 1) / group + s.nk - s.nq + 1, 0), nk) : nk;
+        return p.causal != 0 ? min(max(min(r, rows - 1) / a.by_group + s.nk - s.nq + 1, 0), nk) : nk;
     };
     const int tilesP = (np + KEYS - 1) / KEYS, tiles = tilesP + (limit(r0 + S::kRows - 1) + KEYS - 1) / KEYS;
-    const int first = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(tiles) * split / a.splits));
-    const int end = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(tiles) * (split + 1) / a.splits));
-    const int rw = r0 + wave * 32;                       // this wave's first row
+    // Tiles of this range: so many each, the first `more` one more.
+    const int each = tiles / a.by_splits, more = tiles - each * a.splits;
+    const int first = __builtin_amdgcn_readfirstlane(each * split + min(split, more));
+    const int end = __builtin_amdgcn_readfirstlane(first + each + (split < more ? 1 : 0));
+    const int rw = r0 + wave % (NW / KG) * 32, key0 = wave / (NW / KG) * S::kKeys;   // this wave's first row, first key of a tile
     const int limLo = limit(rw), limHi = limit(rw + 31);
-    const int r = min(rw + l32, rows - 1), lim = limit(r), head = g * group + r % group;
-    const bool valid = rw + l32 < rows;
-    const int64_t token = s.q0 + r / group;
-
-    // Queries, a piece a step; a negative scale turns their signs.
-    const float c = static_cast<float>(fabs(p.scale) * 1.4426950408889634);
-    P q[KS];
-    {
-        const T* qr = static_cast<const T*>(p.q) + token * p.q_stride + static_cast<int64_t>(head) * p.dim;
-#pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            const int d = (2 * i + hl) * (16 / static_cast<int>(sizeof(T)));
-            P x = {};
-            if (d < p.dim) x = *reinterpret_cast<const P*>(qr + d);
-            if (p.scale < 0.0) x = -x;
-            q[i] = x;
-        }
-    }
+    const int lim = limit(rw + l32);
+    // Row r of the block's sequence: its token, counted from the block's first,
+    // and its elements' place, counted from that token's.
+    const int token0 = __builtin_amdgcn_readfirstlane(r0 / a.by_group);
+    auto tokenOf = [&](int r) { return r / a.by_group - token0; };
+    auto placeOf = [&](int r, int64_t stride) {
+        const int t = tokenOf(r);
+        return static_cast<uint32_t>(t) * static_cast<uint32_t>(stride) + static_cast<uint32_t>((r - (t + token0) * group + g * group) * p.dim);
+    };
 
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ldsTiles));
     const int pieces = p.dim * static_cast<int>(sizeof(T)) / 16;
@@ -240,6 +257,46 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         for (int i = threadIdx.x * 16; i < S::kLds; i += NW * 64 * 16) *reinterpret_cast<f32x4*>(ldsTiles + i) = f32x4{};
         __syncthreads();
     }
+    // Queries, a piece a step; a negative scale turns their signs. Eight waves
+    // ask for them by whole rows, to the LDS of the last two stages: the 16
+    // bytes of 64 rows that a step takes are 64 cycles of a load otherwise, 16
+    // loads a wave.
+    const float c = static_cast<float>(fabs(p.scale) * 1.4426950408889634);
+    constexpr int kPieces = RB / 16, kRowsOfLoad = 64 / kPieces;
+    const T* q0 = static_cast<const T*>(p.q) + (s.q0 + token0) * p.q_stride;
+    static_assert(!PING || NW * 32 * RB == 2 * S::kStage, "the queries take the last two stages");
+    constexpr int kQueries = 2 * S::kStage / NW;   // of a wave
+    const uint32_t atQ = S::kLds - 2 * S::kStage + wave * kQueries;
+    P q[KS];
+    auto askQueries = [&] {
+        if constexpr (PING) {
+#pragma unroll
+            for (int i = 0; i < 32 / kRowsOfLoad; ++i) {
+                const int row = i * kRowsOfLoad + ln / kPieces, piece = (ln % kPieces) ^ swizzleK<RB>(row);
+                const uint32_t off = placeOf(min(rw + row, rows - 1), p.q_stride) * static_cast<uint32_t>(sizeof(T)) + piece * 16;
+                if (piece < pieces) S::dma(q0, off, lds0 + atQ + i * 1024);
+            }
+        } else {
+            const T* row = q0 + placeOf(min(rw + l32, rows - 1), p.q_stride);
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                const int d = (2 * i + hl) * (16 / static_cast<int>(sizeof(T)));
+                q[i] = P{};
+                if (d < p.dim) q[i] = *reinterpret_cast<const P*>(row + d);
+            }
+        }
+    };
+    auto takeQueries = [&] {
+        if constexpr (PING) {
+            const char* at = ldsTiles + atQ;
+#pragma unroll
+            for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const P*>(at + l32 * RB + (((2 * i + hl) ^ swizzleK<RB>(l32)) << 4));
+        }
+        if (p.scale < 0.0) {
+#pragma unroll
+            for (int i = 0; i < KS; ++i) q[i] = -q[i];
+        }
+    };
     // The next tile to load: its rows, how many of its keys are left, its place.
     struct Next {
         const char *k, *v;
@@ -264,7 +321,8 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
             next = start(it);
             next.at = at;
         }
-        S::load(next.k, next.v, next.ks, next.vs, next.left - 1, pieces, lds0 + next.at, wave);
+        S::load(0, next.k, next.ks, next.left - 1, pieces, lds0 + next.at, wave);
+        S::load(1, next.v, next.vs, next.left - 1, pieces, lds0 + next.at, wave);
         next.k += static_cast<uint64_t>(KEYS) * next.ks;
         next.v += static_cast<uint64_t>(KEYS) * next.vs;
         next.left -= KEYS;
@@ -285,8 +343,8 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
 
     f32x16 o[DB] = {};
     float m = kLowest, l = 0.0f;   // of this lane's query; l of this lane's keys
-    auto place = [&](int it) { return ldsTiles + (it - first) % STAGES * S::kStage; };
-    auto firstKey = [&](int it) { return (it < tilesP ? it : it - tilesP) * KEYS; };
+    auto place = [&](int it) { return ldsTiles + (it - first) % STAGES * S::kStage + key0 * RB; };
+    auto firstKey = [&](int it) { return (it < tilesP ? it : it - tilesP) * KEYS + key0; };
     // Scores of a tile.
     f32x16 x[KB];
     auto scores = [&](int it) {
@@ -302,10 +360,10 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         }
     };
     // Their weights, in place for f32, else rounded to the type.
-    P w[sizeof(T) == 4 ? 1 : KEYS / 16];
+    P w[sizeof(T) == 4 ? 1 : S::kKeys / 16];
     auto weights = [&](int it) {
         const int j0 = firstKey(it);
-        if ((it < tilesP ? np : limLo) < j0 + KEYS) {
+        if ((it < tilesP ? np : limLo) < j0 + S::kKeys) {
             const int seen = (it < tilesP ? np : lim) - j0 - 4 * hl;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -348,7 +406,7 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
             for (int kb = 0; kb < KB; ++kb) asm volatile("" : "+v"(x[kb]));
         } else {
 #pragma unroll
-            for (int kg = 0; kg < KEYS / 16; ++kg) {
+            for (int kg = 0; kg < S::kKeys / 16; ++kg) {
                 f32x4 bits = __builtin_bit_cast(f32x4, w[kg]);
                 asm volatile("" : "+v"(bits));
                 w[kg] = __builtin_bit_cast(P, bits);
@@ -372,7 +430,7 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
             }
         } else {
 #pragma unroll
-            for (int kg = 0; kg < KEYS / 16; ++kg) {
+            for (int kg = 0; kg < S::kKeys / 16; ++kg) {
 #pragma unroll
                 for (int i = 0; i < DB; ++i) {
                     using Lds = __attribute__((address_space(3))) Short4;
@@ -397,7 +455,11 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
     // is in one phase, the other is in the other.
     const bool late = PING && wave >= NW / 2;
     if constexpr (STAGES == 2) {   // no room to have the next tile's keys early
-        if (first < end) load(first);
+        if (first < end) {
+            askQueries();
+            takeQueries();
+            load(first);
+        }
         for (int it = first; it < end; ++it) {
             S::wait(0);
             barrier();
@@ -416,14 +478,23 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         // Waits for this wave's part of tile `it`, where the next STAGES - 3
         // were asked for too.
         auto arrived = [&](int it) { S::wait(max(0, min(NW == 1 ? STAGES - 2 : STAGES - 3, end - 1 - it))); };
-        for (int it = first; it < min(first + ahead, end); ++it) load(it);
-        S::wait(max(0, min(ahead, end - first) - 1));
+        constexpr int kBefore = NW == 1 ? STAGES - 1 : STAGES - 2;
+        askQueries();
+        for (int it = first; it < min(first + kBefore, end); ++it) load(it);
+        if (PING) S::wait(min(kBefore, end - first));
+        takeQueries();
+        S::wait(max(0, min(kBefore, end - first) - 1));
+        if (PING) asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         barrier();
+        if (late && first + kBefore < end) load(first + kBefore);
         if (first < mine) scores(first);
         if (late) {
             arrived(first + 1);
             barrier();
         }
+        auto keep = [&](int it) {
+            if (it + ahead < end) load(it + ahead);
+        };
         auto before = [&](int it) {
             if (!late) arrived(it + 1);
             barrier();
@@ -438,24 +509,24 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         };
         int it = first;
         for (; it + 1 < mine; ++it) {
-            if (it + ahead < end) load(it + ahead);
+            keep(it);
             weights(it);
             before(it);
             values(it);
             scores(it + 1);
-            if constexpr (sizeof(T) == 2) readAhead<KEYS / 16 * DB, KB * KS, 4>();
+            if constexpr (sizeof(T) == 2) readAhead<S::kKeys / 16 * DB, KB * KS, 4>();
             after(it);
         }
         if (it < mine) {
-            if (it + ahead < end) load(it + ahead);
+            keep(it);
             weights(it);
             before(it);
             values(it);
-            if constexpr (sizeof(T) == 2) readAhead<KEYS / 16 * DB, 0, 4>();
+            if constexpr (sizeof(T) == 2) readAhead<S::kKeys / 16 * DB, 0, 4>();
             after(it++);
         }
         for (; it < end; ++it) {
-            if (it + ahead < end) load(it + ahead);
+            keep(it);
             before(it);
             after(it);
         }
@@ -463,13 +534,13 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
     }
     // A weight of 0 takes an infinite or NaN value to NaN: where a row came out
     // non-finite, the block is summed again key by key, hidden keys left out.
-    bool bad = !(fabsf(l) < INFINITY);
+    float zero = 0.0f * l;
 #pragma unroll
     for (int i = 0; i < DB; ++i) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) bad |= !(fabsf(o[i][e]) < INFINITY);
+        for (int e = 0; e < 16; ++e) zero = __builtin_fmaf(o[i][e], 0.0f, zero);
     }
-    if (__syncthreads_or(bad)) {
+    if (__syncthreads_or(zero != 0.0f)) {   // NaN, where one was not finite
 #pragma unroll
         for (int i = 0; i < DB; ++i) o[i] = f32x16{};
         m = kLowest;
@@ -481,7 +552,7 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
             __syncthreads();
             const char* tile = place(it);
             const int j0 = firstKey(it), seen = (it < tilesP ? np : lim) - j0;
-            const int n = it < mine ? min((it < tilesP ? np : nk) - j0, KEYS) : 0;
+            const int n = it < mine ? min((it < tilesP ? np : nk) - j0, S::kKeys) : 0;
             for (int j = 0; j < n; ++j) {
                 float s = 0.0f;
 #pragma unroll
@@ -522,37 +593,78 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : 2) void attentionTiles(Tile
         }
     }
 
+    // Results by whole rows through LDS, each wave its own 32 rows, 16 bytes a
+    // lane (8 bytes of each of 64 rows at a time take 64 cycles a store).
     l += otherHalf(l);
-    if (!valid) return;
-    const int64_t row = token * p.heads + head;
-    if (a.parts > 0) {
-        const int64_t at = static_cast<int64_t>(a.part0 + split) * p.q_rows * p.heads + row;
-        if (hl == 0) a.ml[at] = make_float2(m, l);
-        float* out = a.acc + at * p.dim;
+    if constexpr (KG == 2) {   // the groups' sums joined, a lane's with its like's
+        float* const at = reinterpret_cast<float*>(ldsTiles) + wave % (NW / 2) * (DB * 16 + 2) * 64 + ln;
+        if (wave >= NW / 2) {
+#pragma unroll
+            for (int i = 0; i < DB; ++i) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) at[(i * 16 + e) * 64] = o[i][e];
+            }
+            at[DB * 16 * 64] = m;
+            at[(DB * 16 + 1) * 64] = l;
+        }
+        __syncthreads();
+        if (wave < NW / 2) {
+            const float m1 = at[DB * 16 * 64], top = fmaxf(m, m1), keep = __builtin_amdgcn_exp2f(m - top), keep1 = __builtin_amdgcn_exp2f(m1 - top);
+            m = top;
+            l = l * keep + at[(DB * 16 + 1) * 64] * keep1;
+#pragma unroll
+            for (int i = 0; i < DB; ++i) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) o[i][e] = o[i][e] * keep + at[(i * 16 + e) * 64] * keep1;
+            }
+        }
+        __syncthreads();
+        if (wave >= NW / 2) return;
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    if (hl == 0 && rw + l32 < rows) {
+        const int t = tokenOf(rw + l32), h = rw + l32 - (t + token0) * group + g * group;
+        const int64_t row = (s.q0 + token0 + t) * p.heads + h;
+        if (a.parts > 0) a.ml[static_cast<int64_t>(a.part0 + split) * p.q_rows * p.heads + row] = make_float2(m, l);
+        else if (p.lse != nullptr) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    }
+    auto store = [&](auto zero, float scale, auto rowAt) {
+        using O = decltype(zero);
+        constexpr int OB = RB / static_cast<int>(sizeof(T)) * static_cast<int>(sizeof(O)), OP = OB / 16, PER = 64 / OP;   // bytes and pieces of a row
+        constexpr int SWIZZLE = OP < 16 ? OP - 1 : 15;
+        static_assert(S::kRows * OB <= S::kLds && NW / 2 * (DB * 16 + 2) * 256 <= (KG == 2 ? S::kLds : 1 << 30), "the rows fit LDS");
+        char* const at = ldsTiles + wave * 32 * OB;
 #pragma unroll
         for (int i = 0; i < DB; ++i) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
-                const int d = i * 32 + 2 * e + 4 * hl;
-                if (d < p.dim) *reinterpret_cast<f32x4*>(out + d) = f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+                Vec4<O> v;
+#pragma unroll
+                for (int f = 0; f < 4; ++f) v[f] = static_cast<O>(o[i][e + f] * scale);
+                const int byte = (i * 32 + 2 * e + 4 * hl) * static_cast<int>(sizeof(O));
+                *reinterpret_cast<Vec4<O>*>(at + l32 * OB + (((byte >> 4) ^ (l32 & SWIZZLE)) << 4) + (byte & 15)) = v;
             }
         }
-        return;
-    }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    T* out = static_cast<T*>(p.out) + token * p.out_stride + static_cast<int64_t>(head) * p.dim;
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
-    for (int i = 0; i < DB; ++i) {
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int d = i * 32 + 2 * e + 4 * hl;
-            V4 v;
-#pragma unroll
-            for (int f = 0; f < 4; ++f) v[f] = static_cast<T>(o[i][e + f] * inv);
-            if (d < p.dim) *reinterpret_cast<V4*>(out + d) = v;
+        for (int i = 0; i < 32 / PER; ++i) {
+            const int row = i * PER + ln / OP, piece = ln % OP;
+            const f32x4 v = *reinterpret_cast<const f32x4*>(at + row * OB + ((piece ^ (row & SWIZZLE)) << 4));
+            if (rw + row < rows && piece * 16 < p.dim * static_cast<int>(sizeof(O))) *reinterpret_cast<f32x4*>(rowAt(rw + row) + piece * 16) = v;
         }
+    };
+    if (a.parts > 0) {
+        char* const acc = reinterpret_cast<char*>(a.acc + static_cast<int64_t>(a.part0 + split) * p.q_rows * p.heads * p.dim);
+        store(0.0f, 1.0f, [&](int r) {
+            const int t = tokenOf(r);
+            return acc + ((s.q0 + token0 + t) * p.heads + (r - (t + token0) * group + g * group)) * static_cast<int64_t>(p.dim) * 4;
+        });
+    } else {
+        char* const out = reinterpret_cast<char*>(static_cast<T*>(p.out) + (s.q0 + token0) * p.out_stride);
+        store(static_cast<T>(0.0f), inv, [&](int r) { return out + static_cast<uint64_t>(placeOf(r, p.out_stride)) * sizeof(T); });
     }
-    if (p.lse != nullptr && hl == 0) p.lse[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 
 }  // namespace mlk

@@ -341,6 +341,64 @@ def test_attention_without_allocation(hip, q_lens, k_lens):
     attention_case(hip, q_lens, k_lens, 8, 2, 128, "bf16", noalloc=True, prefix=150, prefix_rows=150)
 
 
+# Row blocks of 32 rows, of eight waves in two groups with 128 rows, and the
+# widest, by the rows and heads at hand: (heads, key/value heads, tokens, keys).
+BLOCKS = {"narrow": (4, 2, [70, 0, 9], [70, 4, 9]), "halves": (80, 40, [129, 70, 0], [200, 70, 5]),
+          "wide": (120, 120, [129, 70, 0], [200, 70, 5]), "halves_long": (32, 16, [200], [777]), "wide_long": (180, 180, [130], [601])}
+
+
+def block_of(name, dtype):
+    return "narrow" if name == "narrow" or (dtype == "f32" and name.startswith("halves")) else name.split("_")[0]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 80, 128, 256])
+@pytest.mark.parametrize("name", BLOCKS)
+def test_attention_row_blocks(hip, dtype, d, name):
+    h, g, q_lens, k_lens = BLOCKS[name]
+    km = op.attention_module(sum(q_lens) + 2, kv_rows=sum(k_lens), sequences=len(q_lens), heads=h, kv_heads=g, dim=d, dtype=dtype)
+    waves, groups = {"narrow": (1, 1), "halves": (8, 2), "wide": (8, 1)}[block_of(name, dtype)]
+    if dtype == "f32" or d == 256:
+        waves, groups = (1, 1) if waves == 1 else (4, 1)
+    step = hip.build(km).step_kernel_name(0)
+    assert f"{max(d, 64) if d != 80 else 96}, {waves}, {groups}, " in step, step
+    attention_case(hip, q_lens, k_lens, h, g, d, dtype, spare=2, causal=d != 64, gap=3, poison=True)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("name", ["halves", "wide"])
+def test_attention_row_blocks_options(hip, dtype, name):
+    # A negative scale; scores far apart, so that the running maximum grows; a
+    # prefix in front of every sequence's keys, its tiles before theirs.
+    h, g, q_lens, k_lens = BLOCKS[name]
+    attention_case(hip, q_lens, k_lens, h, g, 64, dtype, scale=-0.2)
+    attention_case(hip, q_lens, k_lens, h, g, 128, dtype, magnitude=30.0)
+    attention_case(hip, q_lens, k_lens, h, g, 96, dtype, prefix=70, prefix_rows=90, poison=True, gap=1)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("h,g", [(80, 40), (120, 120)])
+def test_attention_row_blocks_hidden_and_infinite(hip, dtype, h, g):
+    # NaN and infinities that the earlier queries do not see, in either group's
+    # keys of a tile, and a key whose scores are -inf before all others.
+    n, d = 150, 64
+    rng = np.random.default_rng(g)
+    q, k, v = (rounded(rng.standard_normal((n, m, d)), dtype) for m in (h, g, g))
+    v[70, 0, 3], v[100, g - 1, 7], k[140, 5, 1] = np.inf, np.nan, np.nan
+    q[:, :, 0] = np.abs(q[:, :, 0]) + 1
+    k[0, 3, 0] = -np.inf
+    got = run(hip, op.attention_module(n, sequences=1, heads=h, kv_heads=g, dim=d, dtype=dtype, lse=True), {"q": q, "k": k, "v": v, "q_offsets": [0, n]})
+    group = h // g
+    for head, first in ((0, 70), ((g - 1) * group, 100), (5 * group, 140)):
+        assert np.isfinite(got["out"][:first, head]).all() and not np.isfinite(got["out"][first:, head]).all()
+    three = slice(3 * group, 4 * group)
+    assert (got["out"][0, three] == 0).all() and (got["lse"][0, three] == -np.inf).all() and np.isfinite(got["out"][1:, three]).all()
+    # Where nothing is seen that is not finite: as without it.
+    clean = {"q": q, "k": np.where(np.isfinite(k), k, 0.0), "v": np.where(np.isfinite(v), v, 0.0)}
+    out, bound, _, _, _ = attention(clean["q"], clean["k"], clean["v"], [0, n], [0], [n], scale=d ** -0.5, causal=True, dtype=dtype)
+    close(got["out"][:70, :3 * group], out[:70, :3 * group], bound[:70, :3 * group])
+
+
 # ---------------------------------------------------------- shared prefixes --
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("q_lens,k_lens", [([1], [1]), ([1, 1, 1], [0, 1, 70]), ([1] * 20, [3] * 20), ([5, 0, 40], [5, 9, 40]),
