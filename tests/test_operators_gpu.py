@@ -344,7 +344,8 @@ def test_attention_without_allocation(hip, q_lens, k_lens):
 # Row blocks of 32 rows, of eight waves in two groups with 128 rows, and the
 # widest, by the rows and heads at hand: (heads, key/value heads, tokens, keys).
 BLOCKS = {"narrow": (4, 2, [70, 0, 9], [70, 4, 9]), "halves": (80, 40, [129, 70, 0], [200, 70, 5]),
-          "wide": (120, 120, [129, 70, 0], [200, 70, 5]), "halves_long": (32, 16, [200], [777]), "wide_long": (180, 180, [130], [601])}
+          "wide": (120, 120, [129, 70, 0], [200, 70, 5]), "halves_long": (32, 16, [200], [777]), "wide_long": (132, 132, [130], [601]),
+          "halves_ranges": (8, 4, [150, 3, 110], [1500, 40, 1101])}
 
 
 def block_of(name, dtype):
