@@ -79,8 +79,8 @@ __global__ __launch_bounds__(256) void attentionRows(mlkd_attention p) {
             const int64_t ks = part == 0 ? p.prefix_k_stride : p.k_stride, vs = part == 0 ? p.prefix_v_stride : p.v_stride;
             const T* k = static_cast<const T*>(part == 0 ? p.prefix_k : p.k) + (part == 0 ? 0 : s.k0 * ks) + g * d;
             const T* v = static_cast<const T*>(part == 0 ? p.prefix_v : p.v) + (part == 0 ? 0 : s.k0 * vs) + g * d;
-            for (int32_t j0 = 0; j0 < n; j0 += 64) {
-                const int seen = min(64, n - j0);
+            for (int64_t j0 = 0; j0 < n; j0 += 64) {
+                const int seen = static_cast<int>(min(int64_t{64}, n - j0));
                 const T* kr = k + (j0 + min(ln, seen - 1)) * ks;
                 float x = 0.0f;
                 for (int c = 0; c < d; ++c) x += lane(c < 64 ? q[0] : c < 128 ? q[1] : c < 192 ? q[2] : q[3], c & 63) * static_cast<float>(kr[c]);
@@ -197,6 +197,9 @@ bool aligned(const void* ptr, int64_t stride, int bytes, int size) {
 bool tilesApply(const mlkd_attention* p) {
     const int size = p->dtype == MLKD_F32 ? 4 : 2;
     if (p->dim % 8 != 0) return false;
+    // A block finds its sequence by reading the lengths 64 at a time from the
+    // batch's end: 64 dependent rounds at most, then by halving, row by row.
+    if (p->sequences > 4096) return false;
     // Rows and keys, with a tile's more, are counted in 32 bits.
     if (p->q_rows * (p->heads / p->kv_heads) >= (int64_t{1} << 30) || std::max(p->kv_rows, p->prefix_rows) > (int64_t{1} << 30)) return false;
     return aligned(p->q, p->q_stride, 16, size) && aligned(p->k, p->k_stride, 16, size) && aligned(p->v, p->v_stride, 16, size) &&

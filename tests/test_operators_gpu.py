@@ -366,6 +366,15 @@ def test_attention_row_blocks(hip, dtype, d, name):
     attention_case(hip, q_lens, k_lens, h, g, d, dtype, spare=2, causal=d != 64, gap=3, poison=True)
 
 
+@pytest.mark.parametrize("n,q,k", [(64, 1, 9), (65, 1, 9), (150, 5, 40), (200, 40, 70), (4096, 1, 2), (4097, 1, 2)])
+@pytest.mark.parametrize("prefix", [None, 50])
+def test_attention_many_sequences(hip, n, q, k, prefix):
+    # Lengths from none to q and k, found 64 sequences at a time up to 4096.
+    rng = np.random.default_rng(n)
+    q_lens, k_lens = [int(x) for x in rng.integers(0, q + 1, n)], [int(x) for x in rng.integers(0, k + 1, n)]
+    attention_case(hip, q_lens, k_lens, 4, 2, 64, "bf16", spare=3, prefix=prefix or 0, prefix_rows=prefix, gap=1, poison=True)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("name", ["halves", "wide"])
 def test_attention_row_blocks_options(hip, dtype, name):
