@@ -502,7 +502,8 @@ def test_host_entry_runs_the_operators(hip):
     assert (out[9:] == KEEP).all() and (got[5].reshape(t, h)[9:] == KEEP).all()
 
 
-CAPTURED = [("decode", [1] * 4, [700, 30, 1500, 1], None), ("prompt", [60, 90], [60, 120], None), ("prefix", [1] * 5, [4, 9, 1, 70, 3], 400)]
+CAPTURED = [("decode", [1] * 4, [700, 30, 1500, 1], None), ("prompt", [60, 90], [60, 120], None), ("prefix", [1] * 5, [4, 9, 1, 70, 3], 400),
+            ("ranges", [100, 50], [1500, 1000], None)]
 
 
 @pytest.mark.parametrize("mode", [0, 2])
