@@ -156,8 +156,11 @@ struct Tiles {
     static_assert(IPW >= 1 && IPW * NW * 1024 == kTile, "a tile is whole loads of the waves");
     static_assert(STAGES == 2 || (STAGES - 2) * 2 * IPW <= 63, "the loads waited on by number fit the counter");
 
+    /// 16 bytes a lane to LDS at `m0` + 16 * lane. A load to LDS takes M0 one
+    /// wait state after a scalar write of it at the earliest; the compiler puts
+    /// none inside asm (s_nop 0).
     static __device__ __forceinline__ void dma(const void* base, uint32_t off, uint32_t m0) {
-        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory");
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory");
     }
 
     static __device__ __forceinline__ int swizzle(int half, int row) {

@@ -866,9 +866,11 @@ __device__ __forceinline__ uint32_t ldsOffset(const void* p) {
 /// preserved, so it is left out. The asm sets M0 itself right before the
 /// load, and in the kernels that use these loads every M0 write comes from
 /// these asm statements (the compiled code holds no other value in M0).
+/// A load to LDS takes M0 one wait state after a scalar write of it at the
+/// earliest, and the compiler puts none inside asm: the s_nop 0.
 __device__ __forceinline__ void dmaLoad16(const _Float16* src, const _Float16* dst) {
     const uint32_t m0 = __builtin_amdgcn_readfirstlane(ldsOffset(dst));
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0) : "memory");
 }
 
 struct DmaFrag {
@@ -1195,7 +1197,7 @@ __global__ __launch_bounds__(512, 1) void gemmF16Dma8(const _Float16* __restrict
 /// per-lane address costs no vector instruction per step.
 /// M0 is handled as in dmaLoad16.
 __device__ __forceinline__ void dmaLoad16s(const void* sbase, uint32_t voff, uint32_t m0) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(m0) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(m0) : "memory");
 }
 
 // ---------------------------------------------------------- f16 ragged ----
@@ -1381,7 +1383,7 @@ __device__ __forceinline__ void dma8sTile(const _Float16* __restrict__ A, const 
                 }
                 const uint32_t m = m0Wave + static_cast<uint32_t>(slot) * (kDmaStage * 2u) + (j & 1) * 1024u +
                                    (j >= 2 ? kDmaA * 2u : 0u);
-                asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m) : "memory");
+                asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m) : "memory");
                 return;
             }
         }
@@ -1618,7 +1620,7 @@ __global__ __launch_bounds__(256, 2) void gemmF16Dma8s(RaggedF16 p) {
             const int left = (j < 2 ? p.ka : p.k) - s * kDmaBK;
             const char* src = j < 2 ? a + gA[j & 1] : b + gB[j & 1];
             if ((j < 2 ? kA[j & 1] : kB[j & 1]) >= left) src = reinterpret_cast<const char*>(kZero16);
-            asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m) : "memory");
+            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m) : "memory");
         } else {
             dmaLoad16s(j < 2 ? a : b, j < 2 ? gA[j & 1] : gB[j & 1], m);
         }
