@@ -44,6 +44,23 @@ __device__ __forceinline__ int64_t tokensOf(const mlkd_norm_rope& p) {
     return min(max(static_cast<int64_t>(p.q_offsets[p.sequences]), int64_t{0}), p.tokens);
 }
 
+/// Heads whose squares f32 does not hold: their sum is past its range, or mean
+/// square and eps are below 2^-90 (squares lose bits from 2^-126 on, and
+/// v_rsq_f32 takes what is below that for 0). The root is then taken of squares
+/// of the elements times a power of two: 2^-70 (elements below 2^128 give
+/// squares below 2^116) or 2^100 (elements below 2^-41 give squares below 2^118,
+/// the smallest, 2^-149, 2^-98).
+struct Rescale {
+    float before, after;   // an element's factors, before and after the product with the root's inverse
+    __device__ __forceinline__ float squares() const { return before * after; }
+    __device__ __forceinline__ float eps(double e) const { return static_cast<float>(e * squares() * squares()); }
+};
+constexpr float kLeastSquare = 0x1p-90f;
+__device__ __forceinline__ bool rescaled(float square) { return square < kLeastSquare || square == INFINITY; }
+__device__ __forceinline__ Rescale rescaleOf(float square) {
+    return {square < kLeastSquare ? 0x1p100f : 1.0f, square == INFINITY ? 0x1p-70f : 1.0f};
+}
+
 /// Orders the lanes' LDS accesses of one wave.
 __device__ __forceinline__ void waveFence() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -79,7 +96,21 @@ __global__ __launch_bounds__(256) void normRopeHeads(mlkd_norm_rope p) {
         if (kind < 2 && p.q_weight != nullptr) {
 #pragma unroll
             for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m, 64);
-            const float r = 1.0f / sqrtf(sum / static_cast<float>(d) + static_cast<float>(p.eps));
+            float square = sum / static_cast<float>(d) + static_cast<float>(p.eps);
+            const bool far = rescaled(square);   // alike in all lanes
+            const Rescale by = rescaleOf(square);
+            if (far) {
+                sum = 0.0f;
+                for (int c = ln; c < d; c += 64) sum += y[c] * by.squares() * (y[c] * by.squares());
+#pragma unroll
+                for (int m = 32; m > 0; m >>= 1) sum += __shfl_xor(sum, m, 64);
+                square = sum / static_cast<float>(d) + by.eps(p.eps);
+            }
+            float r = 1.0f / sqrtf(square);
+            if (far) {
+                for (int c = ln; c < d; c += 64) y[c] = y[c] * by.before * r * by.after;
+                r = 1.0f;
+            }
             const void* w = kind == 0 ? p.q_weight : p.k_weight;
             for (int c = ln; c < d; c += 64) {
                 y[c] = y[c] * r * (p.weight_dtype == MLKD_F32 ? static_cast<const float*>(w)[c] : static_cast<float>(static_cast<const T*>(w)[c]));
@@ -149,7 +180,7 @@ __device__ __forceinline__ float groupSum(float v) {
 /// read and written once, 16 bytes a lane. Four units are read at a time, the
 /// next four (or the next token's first) while these are worked on.
 template <typename T, int LPH, bool INTERLEAVED>
-__global__ __launch_bounds__(256) void normRopeTokens(mlkd_norm_rope p, int per, int chunks) {
+__global__ __launch_bounds__(256, 4) void normRopeTokens(mlkd_norm_rope p, int per, int chunks) {
     using V = Vec8<T>;
     constexpr int HPW = 64 / LPH, PAIRS = INTERLEAVED ? 4 : 8, BATCH = sizeof(T) == 4 ? 2 : 4;
     const int ln = threadIdx.x & 63, at = ln % LPH, d0 = at * 8, sub = ln / LPH;
@@ -235,7 +266,17 @@ __global__ __launch_bounds__(256) void normRopeTokens(mlkd_norm_rope p, int per,
                         sum += y[j] * y[j];
                     }
                     if (normed) {
-                        const float r = __builtin_amdgcn_rsqf(groupSum<LPH>(sum) * mean + eps);
+                        float square = groupSum<LPH>(sum) * mean + eps, r = __builtin_amdgcn_rsqf(square);
+                        if (__any(rescaled(square))) {   // the other heads times 1
+                            const Rescale by = rescaleOf(square);
+                            sum = 0.0f;
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) sum += y[j] * by.squares() * (y[j] * by.squares());
+                            r = __builtin_amdgcn_rsqf(groupSum<LPH>(sum) * mean + by.eps(p.eps));
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) y[j] = y[j] * by.before * r * by.after;
+                            r = 1.0f;
+                        }
 #pragma unroll
                         for (int j = 0; j < 8; ++j) y[j] = y[j] * r * (kind == 0 ? wq[j] : wk[j]);
                     }
