@@ -153,6 +153,8 @@ struct Tiles {
     static constexpr int kRows = 32 * NW / KG;
     static constexpr int IPW = kTile / 1024 / NW;                    // 1024-byte loads of a wave, for keys and again for values
     static constexpr int kKeys = KEYS / KG, KB = kKeys / 32;         // keys of a tile that a wave takes
+    /// log2 of a largest weight when the weights' reference is set: see attentionTiles.
+    static constexpr float kTop = std::is_same_v<T, _Float16> ? 7.0f : 0.0f;
     static_assert(IPW >= 1 && IPW * NW * 1024 == kTile, "a tile is whole loads of the waves");
     static_assert(STAGES == 2 || (STAGES - 2) * 2 * IPW <= 63, "the loads waited on by number fit the counter");
 
@@ -211,8 +213,10 @@ struct Tiles {
 /// transposing reads. The maximum that the weights are taken relative to
 /// follows the running one only when that has grown by 2^8: sums of weights
 /// up to 2^8 lose nothing in f32, and out is rescaled in few tiles. Weights are
-/// rounded to the type (half a step, relative) as the product's operand, their
-/// sum is of the f32 values.
+/// rounded to the type as the product's operand, half a step, relative, their
+/// sum is of the f32 values. f16 has such steps from 2^-14 on and 0 below 2^-25:
+/// its weights are 2^7 to 2^15 at the row's maximum instead of 1 to 2^8, so that
+/// only weights below 2^-32 of the largest, not 2^-25, are in the sum alone.
 ///
 /// What bounds it: 16-bit types of 128 columns, the products (a wave's 32 of a
 /// 64-key tile take 1024 cycles and more with the LDS reads that feed them)
@@ -361,7 +365,7 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : DT == 64 && sizeof(T) == 2 
     }
 
     f32x16 o[DB] = {};
-    float m = kLowest, l = 0.0f;   // of this lane's query; l of this lane's keys
+    float m = kLowest, l = 0.0f;   // what the weights of this lane's query are relative to; of this lane's keys, their sum
     auto place = [&](int it) { return ldsTiles + (it - first) % STAGES * S::kStage + key0 * RB; };
     auto firstKey = [&](int it) { return (it < tilesP ? it : it - tilesP) * KEYS + key0; };
     // Scores of a tile.
@@ -397,7 +401,7 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : DT == 64 && sizeof(T) == 2 
 #pragma unroll
             for (int e = 0; e < 16; ++e) top = fmaxf(top, x[kb][e]);
         }
-        top = fmaxf(top, otherHalf(top)) * c;
+        top = __builtin_fmaf(fmaxf(top, otherHalf(top)), c, -S::kTop);
         while (__any(top > m + 8.0f)) {   // once at most; as an if it has out copied in every tile
             const float base = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - base);
             m = base;
@@ -588,8 +592,8 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : DT == 64 && sizeof(T) == 2 
                 }
                 s += otherHalf(s);
                 if (j >= seen) s = -INFINITY;
-                const float top = fmaxf(m, s * c), keep = __builtin_amdgcn_exp2f(m - top);
-                const float u = __builtin_amdgcn_exp2f(s * c - top);
+                const float x = s * c, top = fmaxf(m, x - S::kTop), keep = __builtin_amdgcn_exp2f(m - top);
+                const float u = __builtin_amdgcn_exp2f(x - top);
                 m = top;
                 l = l * keep + (hl == 0 ? u : 0.0f);
                 const float ut = static_cast<float>(static_cast<T>(u));

@@ -34,3 +34,41 @@ def test_norm_of_heads_far_from_one(hip, dtype, d, eps, magnitudes):
         want, bound = norm_rope(x[:, heads], weights[f"{name}_weight"], pos, **args)
         close(got[name], want, bound, name)
     assert (got["v"] == x[:, h + g:]).all()
+
+
+# ---------------------------------------------------------------- attention --
+# Row blocks and key ranges: (heads, key/value heads, queries, keys).
+TAILS = {"narrow": (4, 2, 1, 300), "ranges": (4, 1, 1, 20000), "halves": (32, 16, 200, 5000), "halves_ranges": (4, 1, 300, 20000),
+         "wide": (132, 132, 130, 601)}
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("name,hidden", [(n, b) for n in TAILS for b in (False, True) if not b or TAILS[n][2] > 1])
+def test_f16_tail_behind_one_key(hip, d, name, hidden):
+    """One key with the largest score and no value, all others 2^-26 of it, with
+    values about 1: what is left of a tail in f16 weights. `hidden`: a NaN that
+    the first queries do not see, so that keys are taken one by one.
+
+    Bound, scores being exact products: a weight relative to the largest is
+    within 2^-11 of itself or 2^-25 2^-7, its exponential and the running sums
+    within (n + 64) 2^-24, and out is rounded once."""
+    h, g, nq, nk = TAILS[name]
+    rng = np.random.default_rng(nk)
+    q, k = np.zeros((nq, h, d)), np.zeros((nk, g, d))
+    q[..., 0], k[..., 0], k[nk // 3, :, 0] = 1.0, -18.0, 0.0
+    v = rounded(0.5 + rng.random((nk, g, d)), "f16")
+    v[nk // 3] = 0.0
+    if hidden:
+        v[nk - 1, :, 0] = np.nan
+    km = op.attention_module(nq, kv_rows=nk, sequences=1, heads=h, kv_heads=g, dim=d, dtype="f16", causal=hidden, scale=1.0, lse=True)
+    got = run(hip, km, {"q": q, "k": k, "v": v, "q_offsets": [0, nq], "kv_start": [0], "kv_len": [nk]})
+    rows = nq - 1 if hidden else nq
+    seen = nk - nq + 1 + np.arange(rows) if hidden else np.full(rows, nk)
+    w = np.exp(k[:, 0, 0])
+    total, sums = np.cumsum(w)[seen - 1], np.cumsum(w[:, None, None] * np.where(np.isnan(v), 0.0, v), 0)[seen - 1]
+    top = np.cumsum(np.where(np.isnan(v), 0.0, v), 0)[seen - 1]   # sums of the tail's values
+    want = np.repeat(sums / total[:, None, None], h // g, 1)
+    sum_error = (nk + 64) * 2.0 ** -24
+    bound = want * (2.0 ** -11 + sum_error) * 2 + np.repeat(top, h // g, 1) * 2.0 ** -32 + 2.0 ** -25
+    close(got["out"][:rows], want, bound)
+    close(got["lse"][:rows], np.repeat(np.log(total)[:, None], h, 1), sum_error + 2.0 ** -22)
