@@ -21,6 +21,7 @@ template <typename T>
 using Piece = T __attribute__((ext_vector_type(16 / sizeof(T))));
 
 constexpr float kLowest = -3.402823466e38f;   // a running maximum before any score
+constexpr float kFar = 16777216.0f;           // 2^24
 
 /// c += a b over the columns of a piece in either half wave: 16 of f16 and
 /// bf16, 8 of f32.
@@ -556,8 +557,11 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : DT == 64 && sizeof(T) == 2 
         if (PING && !late) barrier();
     }
     // A weight of 0 takes an infinite or NaN value to NaN: where a row came out
-    // non-finite, the block is summed again key by key, hidden keys left out.
-    float zero = 0.0f * l;
+    // non-finite, the block is summed again key by key, hidden keys left out. Also
+    // where f32 holds the maximum in steps of 2 or more: it is off the score it
+    // was rounded from by up to half a step, and all weights by as many powers of
+    // two. Key by key they are relative to scores rounded alike.
+    float zero = fabsf(m) < kFar || m == kLowest ? 0.0f * l : NAN;
 #pragma unroll
     for (int i = 0; i < DB; ++i) {
 #pragma unroll

@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 
 from mlk2_amd import operators as op
-from operators_ref import norm_rope, rounded
-from test_operators_gpu import close, run
+from operators_ref import TINY, U, U32, norm_rope, rounded
+from test_operators_gpu import TYPES, close, run
 
 pytestmark = pytest.mark.gpu
 
@@ -72,3 +72,37 @@ def test_f16_tail_behind_one_key(hip, d, name, hidden):
     bound = want * (2.0 ** -11 + sum_error) * 2 + np.repeat(top, h // g, 1) * 2.0 ** -32 + 2.0 ** -25
     close(got["out"][:rows], want, bound)
     close(got["lse"][:rows], np.repeat(np.log(total)[:, None], h, 1), sum_error + 2.0 ** -22)
+
+
+SHAPES = {"narrow": (4, 2, 1, 300), "ranges": (4, 1, 1, 5000), "halves": (32, 16, 200, 500), "halves_ranges": (4, 1, 300, 3000),
+          "wide": (132, 132, 130, 601)}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 256, 20])
+@pytest.mark.parametrize("name", SHAPES)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("size", [23, 26, 31, 40, 60])
+def test_scores_far_from_zero(hip, dtype, d, name, sign, size):
+    """Scores of about 2^size: the keys with the largest share the weight.
+
+    Scores are one product, the same for the same operands, and an eighth and
+    more apart, which is 2^20 and more; so the result is a mean of n values,
+    each product and sum within 2^-24 n, the weights and out rounded once."""
+    h, g, nq, nk = SHAPES[name]
+    rng = np.random.default_rng(nk)
+    q, k = np.zeros((nq, h, d)), np.zeros((nk, g, d))
+    q[..., 1] = 1.37 * 2.0 ** 8
+    k[..., 1] = sign * rng.choice([1.25, 1.3828125, 1.5] if sign > 0 else [1.8671875, 1.99], (nk, g)) * 2.0 ** 8
+    best = sorted(rng.choice(nk, 7, replace=False))
+    k[best, :, 1] = sign * 1.7109375 * 2.0 ** 8
+    q, k = rounded(q, dtype), rounded(k, dtype)
+    v = rounded(rng.standard_normal((nk, g, d)), dtype)
+    scale = 2.0 ** (size - 17)
+    km = op.attention_module(nq, kv_rows=nk, sequences=1, heads=h, kv_heads=g, dim=d, dtype=dtype, causal=False, scale=scale, lse=True)
+    got = run(hip, km, {"q": q, "k": k, "v": v, "q_offsets": [0, nq], "kv_start": [0], "kv_len": [nk]})
+    want = np.repeat(v[best].mean(0), h // g, 0)
+    size_of = np.repeat(np.abs(v[best]).mean(0), h // g, 0)
+    close(got["out"], np.broadcast_to(want, got["out"].shape), (U[dtype] + 64 * U32) * size_of + U[dtype] * np.abs(want) + TINY[dtype])
+    lse = q[0, 0, 1] * k[best[0], 0, 1] * scale + np.log(len(best))
+    close(got["lse"], np.full(got["lse"].shape, lse), 8 * U32 * abs(lse))
