@@ -70,7 +70,7 @@ __device__ __forceinline__ int operator/(int n, const Divider& d) {
 struct TileArgs {
     mlkd_attention p;
     int keys;         // 1: the prefix, 2: the sequences' own, 3: both
-    int all_rows;     // 1: rows of all sequences together (prefix keys only)
+    int all_rows;     // 1: the rows that sequences hold, all together (prefix keys only)
     int splits;       // key ranges of each row block
     int part0;        // partial results: the first range's index ...
     int parts;        // ... of so many (0: results go straight to out)
@@ -246,9 +246,14 @@ __global__ __launch_bounds__(NW * 64, DT > 128 ? 1 : DT == 64 && sizeof(T) == 2 
     const int id = static_cast<int>(blockIdx.x), of = id / a.by_kv_heads, g = id - of * p.kv_heads;
     const int rest = of / a.by_splits, split = of - rest * a.splits, group = p.heads / p.kv_heads;
     int np = (a.keys & 1) != 0 ? prefixOf(p) : 0;
-    SeqSpan s{0, 0, static_cast<int32_t>(p.q_rows), 0};
+    SeqSpan s{};
     int r0 = rest * S::kRows;
-    if (a.all_rows != 0 ? r0 >= s.nq * group : !rowBlock<S::kRows>(p, group, rest, s, r0)) return;
+    if (a.all_rows != 0) {
+        s = heldRows(p);
+        if (r0 >= s.nq * group) return;
+    } else if (!rowBlock<S::kRows>(p, group, rest, s, r0)) {
+        return;
+    }
     s = SeqSpan{uniform(s.q0), uniform(s.k0), static_cast<int32_t>(uniform(s.nq)), static_cast<int32_t>(uniform(s.nk))};
     r0 = __builtin_amdgcn_readfirstlane(r0);
     np = __builtin_amdgcn_readfirstlane(np);

@@ -3,9 +3,11 @@ magnitudes, long tails, rows that no sequence holds, many tokens to a wave."""
 import numpy as np
 import pytest
 
+from attention_abi import Attention
 from mlk2_amd import operators as op
-from operators_ref import TINY, U, U32, norm_rope, rounded
-from test_operators_gpu import TYPES, close, run
+from mlk2_amd.backend import DeviceBuffer
+from operators_ref import TINY, U, U32, attention, norm_rope, rounded
+from test_operators_gpu import KEEP, TYPES, close, run
 
 pytestmark = pytest.mark.gpu
 
@@ -106,3 +108,47 @@ def test_scores_far_from_zero(hip, dtype, d, name, sign, size):
     close(got["out"], np.broadcast_to(want, got["out"].shape), (U[dtype] + 64 * U32) * size_of + U[dtype] * np.abs(want) + TINY[dtype])
     lse = q[0, 0, 1] * k[best[0], 0, 1] * scale + np.log(len(best))
     close(got["lse"], np.full(got["lse"].shape, lse), 8 * U32 * abs(lse))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offsets", [[10] + list(range(11, 51)), [0] * 20 + list(range(21)), [300] * 41, [0] * 41, [5, 50] + [7] * 38 + [40]])
+def test_rows_of_no_sequence_take_no_part_behind_a_prefix(hip, dtype, offsets):
+    # Rows before, behind and past the sequences hold NaN and infinities: neither
+    # partial results nor outputs are written for them, and the others are whole.
+    h, g, d, rows, prefix, keys = 4, 1, 64, 300, 700, 3
+    n = len(offsets) - 1
+    rng = np.random.default_rng(3)
+    first, end = min(offsets), min(max(offsets), rows)
+    q = rng.standard_normal((rows, h, d))
+    q[:first], q[end:] = np.nan, np.inf
+    q = rounded(q, dtype)
+    k, v = (rounded(rng.standard_normal((n * keys, g, d)), dtype) for _ in range(2))
+    pk, pv = (rounded(rng.standard_normal((prefix, g, d)), dtype) for _ in range(2))
+    start, lens = np.arange(n) * keys, np.full(n, keys)
+    p = Attention.of(heads=h, kv_heads=g, dim=d, sequences=n, q_rows=rows, kv_rows=n * keys, prefix_rows=prefix, dtype=dtype)
+    parts = p.ranges()
+    assert parts > 1
+    bufs = {name: DeviceBuffer.from_array(np.asarray(a), dtype) for name, a in
+            {"q": q, "k": k, "v": v, "prefix_k": pk, "prefix_v": pv, "out": np.full((rows, h, d), KEEP)}.items()}
+    bufs.update({name: DeviceBuffer.from_array(np.asarray(a), "i32") for name, a in
+                 {"q_offsets": offsets, "kv_start": start, "kv_len": lens}.items()})
+    bufs["lse"] = DeviceBuffer.from_array(np.full((rows, h), KEEP), "f32")
+    bufs["work"] = DeviceBuffer.from_array(np.full(p.work_needed() // 4, KEEP), "f32")
+    for name, b in bufs.items():
+        setattr(p, name, b.ptr)
+    p.work_bytes = bufs["work"].nbytes
+    p.launch()
+    work = bufs["work"].to_numpy()
+    sums = work[:parts * rows * h * d].reshape(parts, rows, h * d)
+    stats = work[parts * rows * h * d:].reshape(parts, rows, 2 * h)
+    for part in (sums, stats):
+        assert (part[:, :first] == KEEP).all() and (part[:, end:] == KEEP).all()
+    out, lse = bufs["out"].to_numpy().reshape(rows, h, d), bufs["lse"].to_numpy().reshape(rows, h)
+    assert (out[:first] == KEEP).all() and (out[end:] == KEEP).all() and (lse[:first] == KEEP).all() and (lse[end:] == KEEP).all()
+    if list(offsets) != sorted(offsets):
+        assert np.isfinite(out[first:end]).all()   # rows in two sequences: either's keys
+        return
+    want, bound, want_lse, lse_bound, written = attention(q, k, v, np.minimum(offsets, rows), start, lens, scale=d ** -0.5, causal=True,
+                                                          dtype=dtype, prefix_k=pk, prefix_v=pv)
+    close(out[written], want[written], bound[written], "out")
+    close(lse[written], want_lse[written], lse_bound[written], "lse")
