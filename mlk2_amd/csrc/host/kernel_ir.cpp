@@ -382,7 +382,8 @@ Result<KernelModule> parseKernelModule(const char* text, size_t len) {
         const uint32_t ops = rd.member(n, "operands");
         if (ops != kInvalidId && rd.at(ops).type == JNode::Object) {
             for (const uint32_t m : rd.at(ops).items) {
-                kn.operands.emplace_back(rd.at(m).text, static_cast<uint32_t>(d.integer(rd.at(m).items[0], -1)));
+                const int64_t id = d.integer(rd.at(m).items[0], -1);
+                kn.operands.emplace_back(rd.at(m).text, id >= 0 && id < kInvalidId ? static_cast<uint32_t>(id) : kInvalidId);
             }
         }
         const uint32_t attrs = rd.member(n, "attrs");
