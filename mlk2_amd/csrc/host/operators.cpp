@@ -2,6 +2,7 @@
 // shared_prefix_attention. Their operands are buffers by name, their options
 // numbers by name; everything the kernels assume of either is checked here,
 // before any device work.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 #include <string>
@@ -59,10 +60,10 @@ public:
                 return fail("operand '" + name + "' is neither an input nor an output");
             }
             if (b.dims.empty()) return fail("operand '" + name + "' has no dims");
-            int64_t total = 1;
+            int64_t total = 1;   // of the dims that are not 0, so that every part of the product fits
             for (const int64_t d : b.dims) {
                 if (d < 0 || (d > 0 && total > (int64_t{1} << 44) / d)) return fail("operand '" + name + "' is too large");
-                total *= d;
+                total *= std::max<int64_t>(d, 1);
             }
         }
         for (size_t i = 0; i < n_.attrs.size(); ++i) {
