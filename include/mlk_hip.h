@@ -227,9 +227,11 @@ int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* bind
  * in pairs (i, i + rot/2), or (2i, 2i+1) if interleaved, by the angle
  * positions[axis, t] * theta^(-2i/rot); the first section_0 pairs take axis
  * 0, the next section_1 axis 1, the last section_2 axis 2. Angles are reduced
- * in f64. k_out and v_out hold token t in row slots[t], or in row t without
- * slots; a slot outside the rows stores nothing, and slots that name a row
- * twice leave one of its tokens there. With q_offsets (i32 [n + 1], n
+ * in f64. Means and products are held in f32; a head's size does not matter to
+ * its norm. k_out and v_out hold token t in row slots[t], or in row t without
+ * slots; a slot outside the rows stores nothing. Tokens whose slots name the
+ * same row store there in no order: each 16 bytes and less of the row are one
+ * of theirs, not all the same one's. With q_offsets (i32 [n + 1], n
  * sequences) the tokens from its last element on are left alone. q_out may
  * take q's place, and without slots k_out k's and v_out v's.
  *
@@ -243,7 +245,29 @@ int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* bind
  * keys, does not reach its result, whatever its bits. A query without keys,
  * or with -inf scores alone, gets zeros and an lse of -inf. lse (f32 [rows,
  * heads]) is the log of the sum of exp(scale q k^T). Rows behind the last
- * sequence are left alone; offsets and lengths are clipped to the buffers.
+ * sequence are left alone; offsets and lengths are clipped to the buffers
+ * (offsets are meant to rise: a row that two sequences hold is written by both).
+ *
+ * Scores, weights, their sums and those of the values are held in f32: q k^T,
+ * scale q k^T and the sum of weights (each up to 2^8) times values have to stay
+ * in its range. f16 and bf16 weights are rounded to the type for their product
+ * with v, by half a step of themselves or, f16, 2^-32 of the row's largest if
+ * that is more; their sum, and so lse, is of the f32 values. The error against
+ * 64 bits is 1.1 to 1.4 times that of f32 weights rounded once at the end. Rows
+ * off 16 bytes (below) have f32 weights throughout.
+ *
+ * Time: buffers' sizes, not the lengths in them, decide the form: row blocks
+ * and key ranges are those of q's rows and k's rows over the number of
+ * sequences. Build a module per size that is run often (one of 8192 rows runs
+ * 64 single tokens in blocks and ranges meant for prompts), and expect one long
+ * sequence among short ones to take as many ranges as they do. The matrix-core
+ * kernels take rows of whole 16-byte pieces (dim a multiple of 8, columns,
+ * widths and addresses of 16 bytes), widths below 2^22 elements and at most
+ * 4096 sequences by q_offsets' size; other Calls run a wave to a row, 50 times
+ * slower for single tokens and 200 for prompts (32 over up to 8192 keys at dim
+ * 127: 7.6 ms; 2048 tokens: 11.2). Where a row's result is not finite, or its
+ * scores are past 1e7 in size, its block of rows is summed key by key (2048
+ * tokens, one such row: 108 us instead of 56; all of them: 2 ms).
  *
  * shared_prefix_attention (attention's operands, prefix_k, prefix_v;
  * prefix_len): every sequence's keys follow prefix_k and prefix_v rows 0 ..

@@ -228,7 +228,7 @@ struct Tiles {
 /// 64 columns fit a compute unit at 128 registers (16 sequences of up to 1024,
 /// 16 heads: 78 -> 64 us).
 /// Measured (bf16, 32 and 8 heads of 128, causal): 8 packed prompts of up to
-/// 4096 tokens 544 us, 950 TFLOP/s; one of 2048, by halves, 56 us, 610
+/// 4096 tokens 546 us, 945 TFLOP/s; one of 2048, by halves, 56 us, 610
 /// TFLOP/s; 32 single tokens over up to 8192 keys 148 us, 4.2 TB/s. f32, two
 /// sequences of 1001, 8 heads of 64: 46 us.
 template <typename T, int DT, int NW, int KG, int KEYS, int STAGES>

@@ -13,7 +13,8 @@ the outputs. The operators and their operands:
     theta^(-2 i / rot) (pair i is elements i and i + rot/2, or 2i and 2i + 1
     with ``interleaved``; ``sections`` counts the pairs of each position axis).
     k_out and v_out take token t at row ``slots[t]`` (row t without slots); a
-    slot outside the rows stores nothing. With ``q_offsets`` the tokens from
+    slot outside the rows stores nothing, one that names a row again leaves
+    pieces of either token there. With ``q_offsets`` the tokens from
     q_offsets[-1] on are left alone.
 ``attention``
     out = softmax(scale q k^T) v over packed sequences: sequence b has the
@@ -28,7 +29,10 @@ the outputs. The operators and their operands:
 
 Types: f16, bf16 or f32, the same for all rows; sums are held in f32 and each
 output is rounded once. Attention's weights are rounded to the type of v before
-they meet it, so that f16 and bf16 run on the matrix cores.
+they meet it, so that f16 and bf16 run on the matrix cores; their sum is of the
+f32 values. Buffers' sizes decide how an attention runs, not the lengths in them,
+and rows off 16 bytes or more than 4096 sequences run a wave to a row (see
+include/mlk_hip.h).
 """
 from __future__ import annotations
 
