@@ -5,12 +5,14 @@ instructions, but puts none inside inline assembly or for its sake:
 - a scalar write of M0, then a load to LDS that takes its place from M0: one;
 - a vector write of a scalar register, then a memory access that reads it: five.
 """
+import os
+
 import pytest
 
 import isa
 from mlk2_amd.backend import LIB_PATH
 
-CODE = list(isa.code_objects(LIB_PATH))
+CODE = list(isa.code_objects(LIB_PATH)) if os.path.exists(LIB_PATH) else []
 
 
 @pytest.mark.parametrize("n", range(len(CODE)))
@@ -32,5 +34,5 @@ def test_waits(n):
 
 
 def test_direct_loads_are_there():
-    # What the first rule is about: the library does load to LDS.
+    # What the first rule is about: the library is built and does load to LDS.
     assert sum("_lds_" in i.op for code in CODE for i in isa.disassembled(code)[0]) > 100
