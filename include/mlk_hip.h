@@ -40,8 +40,10 @@ enum {
 };
 
 /* Device element types (KernelBuffer::dtype subset). */
-/* MLKHIP_BF16 and MLKHIP_I32 are the operators' (see below). */
-enum { MLKHIP_F32 = 0, MLKHIP_F16 = 1, MLKHIP_F64 = 2, MLKHIP_BF16 = 3, MLKHIP_I32 = 4 };
+/* MLKHIP_BF16 and those after it are the operators' (see below). */
+enum {
+    MLKHIP_F32 = 0, MLKHIP_F16 = 1, MLKHIP_F64 = 2, MLKHIP_BF16 = 3, MLKHIP_I32 = 4, MLKHIP_I8 = 5, MLKHIP_U8 = 6
+};
 
 typedef struct mlkhip_artifact mlkhip_artifact;
 

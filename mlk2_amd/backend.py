@@ -24,10 +24,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("MLK_HIP_LIB") or os.path.join(HERE, "lib", "libmlk_hip.so")
 
 OK, NEG_STORE, RUNTIME, LAUNCH, NO_DEVICE, BAD_BINDING, REFUSED = 0, 1, 2, 3, 4, 6, 7
-F32, F16, F64, BF16, I32 = 0, 1, 2, 3, 4
-DTYPE_CODE = {"f32": F32, "f16": F16, "f64": F64, "bf16": BF16, "i32": I32}
+F32, F16, F64, BF16, I32, I8, U8 = 0, 1, 2, 3, 4, 5, 6
+DTYPE_CODE = {"f32": F32, "f16": F16, "f64": F64, "bf16": BF16, "i32": I32, "i8": I8, "u8": U8}
 # numpy has no bfloat16: its device elements are their 16 bits here.
-NP_OF_CODE = {F32: np.float32, F16: np.float16, F64: np.float64, BF16: np.uint16, I32: np.int32}
+NP_OF_CODE = {F32: np.float32, F16: np.float16, F64: np.float64, BF16: np.uint16, I32: np.int32, I8: np.int8,
+              U8: np.uint8}
 
 
 def bf16_bits(a) -> np.ndarray:

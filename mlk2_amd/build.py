@@ -30,7 +30,7 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 CLANG = os.path.join(ROCM, "llvm", "bin", "clang++")
 
 DEVICE_SOURCES = ["runtime.hip", "jit.hip", "softmax.hip", "gemm.hip", "gemm_general.hip", "score_softmax.hip", "attention.hip",
-                  "norm_rope.hip", "probe.hip"]
+                  "norm_rope.hip", "rows_i8.hip", "matmul_i8.hip", "kv4_rows.hip", "attention_kv4.hip", "probe.hip"]
 HOST_SOURCES = ["kernel_ir.cpp", "planner.cpp", "codegen.cpp", "nestgen.cpp", "canonical.cpp", "operators.cpp", "driver.cpp",
                 "tune.cpp", "artifact.cpp"]
 

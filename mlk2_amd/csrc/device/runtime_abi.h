@@ -139,6 +139,19 @@ int64_t mlkd_attention_work_bytes(const mlkd_attention* p);
 /// The kernels mlkd_launch_attention runs for `p`, joined by '+' (valid until
 /// this thread's next call).
 const char* mlkd_attention_kernel_names(const mlkd_attention* p);
+/// Likewise for the operators in 8 and 4 bits.
+int mlkd_launch_quantize_rows(const mlkd_quantize_rows* p, void* stream);
+const char* mlkd_quantize_rows_kernel_name(const mlkd_quantize_rows* p);
+int mlkd_launch_matmul_i8(const mlkd_matmul_i8* p, void* stream);
+int64_t mlkd_matmul_i8_work_bytes(const mlkd_matmul_i8* p);
+const char* mlkd_matmul_i8_kernel_names(const mlkd_matmul_i8* p);
+int mlkd_launch_store_kv4(const mlkd_kv4_rows* p, void* stream);
+const char* mlkd_store_kv4_kernel_name(const mlkd_kv4_rows* p);
+int mlkd_launch_load_kv4(const mlkd_kv4_rows* p, void* stream);
+const char* mlkd_load_kv4_kernel_name(const mlkd_kv4_rows* p);
+int mlkd_launch_attention_kv4(const mlkd_attention_kv4* p, void* stream);
+int64_t mlkd_attention_kv4_work_bytes(const mlkd_attention_kv4* p);
+const char* mlkd_attention_kv4_kernel_names(const mlkd_attention_kv4* p);
 
 /// Measured HBM bandwidth (streaming copy of 256 MiB) and f16 MFMA
 /// throughput (register-only MFMAs, one wave per SIMD) of the current

@@ -11,8 +11,8 @@ extern "C" {
 
 /// Element types a device buffer may hold (KernelBuffer::dtype subset,
 /// compiler/include/mlk/type/domain.h:53-60).
-/// BF16 and I32 are the operators' (mlkd_norm_rope, mlkd_attention).
-enum mlkd_dtype { MLKD_F32 = 0, MLKD_F16 = 1, MLKD_F64 = 2, MLKD_BF16 = 3, MLKD_I32 = 4 };
+/// BF16, I32, I8 and U8 are the operators' (mlkd_norm_rope and the ones below it).
+enum mlkd_dtype { MLKD_F32 = 0, MLKD_F16 = 1, MLKD_F64 = 2, MLKD_BF16 = 3, MLKD_I32 = 4, MLKD_I8 = 5, MLKD_U8 = 6 };
 
 /// Runtime scalar parameters of a chain (ScalarParam operands,
 /// kernel_ir.h:58-70); indices past the bound table read 0.0 like the
@@ -124,6 +124,60 @@ typedef struct mlkd_attention {
     void* work;                          /* mlkd_attention_work_bytes, or NULL: no key ranges */
     int64_t work_bytes;
 } mlkd_attention;
+
+/// Rows in 8-bit integers: scale[t] = max |x[t, :]| / 127, codes[t, :] =
+/// x[t, :] / scale[t] rounded to the nearest, half way to the even one, kept
+/// within -127 .. 127. A row of zeros has scale 0 and codes 0, one that holds a
+/// value that is not finite scale NaN and codes 0.
+typedef struct mlkd_quantize_rows {
+    const void* x;
+    int8_t* codes;
+    float* scale;                        /* [rows] */
+    int32_t dtype, pad;                  /* of x */
+    int64_t rows, cols;
+    int64_t x_stride, codes_stride;      /* elements from row to row */
+} mlkd_quantize_rows;
+
+/// out[t, n] = (sum_k a[t, k] b[n, k]) a_scale[t] b_scale[n] + bias[n]; the sum
+/// is exact (k < 2^17).
+typedef struct mlkd_matmul_i8 {
+    const int8_t *a, *b;
+    const float *a_scale, *b_scale;      /* [m], [n] */
+    const float* bias;                   /* [n], or NULL */
+    void* out;
+    int32_t dtype, pad;                  /* of out */
+    int64_t m, n, k;
+    int64_t lda, ldb, ldo;               /* elements from row to row */
+    void* work;                          /* mlkd_matmul_i8_work_bytes, or NULL: no ranges of k */
+    int64_t work_bytes;
+} mlkd_matmul_i8;
+
+/// Heads of k and v to and from the rows of a cache in 4 bits: a scale for each
+/// row and head, max |x| / 6, and the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 to
+/// |x| / scale, half way between two the one of the even code. A code is that
+/// number's place, 0 .. 7, and 8 more where x has its sign bit set; element 2i
+/// has the low half of byte i. A head of zeros has scale 0, one that holds a
+/// value that is not finite scale NaN and codes 0. Token t takes row slots[t]
+/// (row t without slots; rows outside the cache are left out), tokens below
+/// q_offsets[sequences] only.
+typedef struct mlkd_kv4_rows {
+    void *k, *v;                         /* read by the store, written by the load */
+    uint8_t *k_codes, *v_codes;
+    float *k_scale, *v_scale;            /* [cache_rows, kv_heads] */
+    const int32_t* slots;                /* [tokens], or NULL */
+    const int32_t* q_offsets;            /* [sequences + 1], or NULL */
+    int32_t dtype, kv_heads, dim, sequences;
+    int64_t tokens, cache_rows;
+    int64_t k_stride, v_stride;          /* elements from row to row */
+    int64_t k_codes_stride, v_codes_stride;   /* bytes from row to row */
+} mlkd_kv4_rows;
+
+/// mlkd_attention over such a cache: `a` with k and v the codes (strides in
+/// bytes) and no prefix.
+typedef struct mlkd_attention_kv4 {
+    mlkd_attention a;
+    const float *k_scale, *v_scale;      /* [kv_rows, kv_heads] */
+} mlkd_attention_kv4;
 
 #ifdef __cplusplus
 }

@@ -49,7 +49,7 @@ std::vector<bool> storedBuffers(const KernelModule& km) {
         }
         if (!isOperatorCall(n)) continue;
         for (const auto& [name, b] : n.operands) {   // outputs by their names
-            const bool out = name == "out" || name == "lse" || name == "q_out" || name == "k_out" || name == "v_out";
+            const bool out = name == "out" || name == "lse" || (name.size() > 4 && name.compare(name.size() - 4, 4, "_out") == 0);
             if (out && b < km.buffers.size()) w[b] = true;
         }
     }

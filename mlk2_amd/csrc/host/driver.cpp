@@ -8,6 +8,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <limits>
 #include <memory>
 #include <new>
 #include <unordered_map>
@@ -25,6 +26,8 @@ int dtypeCode(Dtype d) {
         case Dtype::F16: return MLKD_F16;
         case Dtype::BF16: return MLKD_BF16;
         case Dtype::I32: return MLKD_I32;
+        case Dtype::I8: return MLKD_I8;
+        case Dtype::U8: return MLKD_U8;
         default: return MLKD_F64;
     }
 }
@@ -67,6 +70,12 @@ int32_t toInt32(double d) {
     if (d <= -2147483648.0) return INT32_MIN;
     if (d >= 2147483647.0) return INT32_MAX;
     return static_cast<int32_t>(d);
+}
+
+/// f64 -> an integer of 8 bits, likewise.
+template <typename T>
+T toInt8(double d) {
+    return static_cast<T>(std::clamp<int32_t>(toInt32(d), std::numeric_limits<T>::min(), std::numeric_limits<T>::max()));
 }
 
 double fromHalfBits(uint16_t bits) {
@@ -141,6 +150,16 @@ void narrowTo(void* out, const double* src, int64_t cnt, Dtype dt) {
         parallelRange(cnt, [&](int64_t b, int64_t e) {
             for (int64_t x = b; x < e; ++x) o[x] = toInt32(src[x]);
         });
+    } else if (dt == Dtype::I8) {
+        int8_t* o = static_cast<int8_t*>(out);
+        parallelRange(cnt, [&](int64_t b, int64_t e) {
+            for (int64_t x = b; x < e; ++x) o[x] = toInt8<int8_t>(src[x]);
+        });
+    } else if (dt == Dtype::U8) {
+        uint8_t* o = static_cast<uint8_t*>(out);
+        parallelRange(cnt, [&](int64_t b, int64_t e) {
+            for (int64_t x = b; x < e; ++x) o[x] = toInt8<uint8_t>(src[x]);
+        });
     } else {
         uint16_t* o = static_cast<uint16_t*>(out);
         parallelRange(cnt, [&](int64_t b, int64_t e) {
@@ -173,6 +192,16 @@ void widenFrom(double* dst, const void* in, int64_t cnt, Dtype dt) {
         });
     } else if (dt == Dtype::I32) {
         const int32_t* s = static_cast<const int32_t*>(in);
+        parallelRange(cnt, [&](int64_t b, int64_t e) {
+            for (int64_t x = b; x < e; ++x) dst[x] = s[x];
+        });
+    } else if (dt == Dtype::I8) {
+        const int8_t* s = static_cast<const int8_t*>(in);
+        parallelRange(cnt, [&](int64_t b, int64_t e) {
+            for (int64_t x = b; x < e; ++x) dst[x] = s[x];
+        });
+    } else if (dt == Dtype::U8) {
+        const uint8_t* s = static_cast<const uint8_t*>(in);
         parallelRange(cnt, [&](int64_t b, int64_t e) {
             for (int64_t x = b; x < e; ++x) dst[x] = s[x];
         });
@@ -462,6 +491,30 @@ const char* HipLoadedKernel::stepKernelName(size_t si) const {
                 p.work_bytes = need;
             }
             name = mlkd_attention_kernel_names(&p);
+        } else if (st.kind == StepKind::QuantizeRows) {
+            mlkd_quantize_rows p;
+            fillQuantizeRows(km_, st, ptr, p);
+            name = mlkd_quantize_rows_kernel_name(&p);
+        } else if (st.kind == StepKind::MatmulI8) {
+            mlkd_matmul_i8 p;
+            fillMatmulI8(km_, st, ptr, p);
+            if (const int64_t need = mlkd_matmul_i8_work_bytes(&p); need > 0) {
+                p.work = ptr[0];   // runDevice gives such a step its workspace
+                p.work_bytes = need;
+            }
+            name = mlkd_matmul_i8_kernel_names(&p);
+        } else if (st.kind == StepKind::StoreKv4 || st.kind == StepKind::LoadKv4) {
+            mlkd_kv4_rows p;
+            fillKv4Rows(km_, st, ptr, p);
+            name = st.kind == StepKind::StoreKv4 ? mlkd_store_kv4_kernel_name(&p) : mlkd_load_kv4_kernel_name(&p);
+        } else if (st.kind == StepKind::AttentionKv4) {
+            mlkd_attention_kv4 p;
+            fillAttentionKv4(km_, st, ptr, p);
+            if (const int64_t need = mlkd_attention_kv4_work_bytes(&p); need > 0) {
+                p.a.work = ptr[0];   // runDevice gives such a step its workspace
+                p.a.work_bytes = need;
+            }
+            name = mlkd_attention_kv4_kernel_names(&p);
         }
     }
     std::lock_guard<std::mutex> g(scratchLock_);
@@ -559,6 +612,14 @@ int HipLoadedKernel::arenaLayout(const DeviceBinding* binds, int64_t elements, c
             mlkd_attention p;
             fillAttention(km_, st, ptr, p);
             pad = mlkd_attention_work_bytes(&p);
+        } else if (st.kind == StepKind::MatmulI8) {
+            mlkd_matmul_i8 p;
+            fillMatmulI8(km_, st, ptr, p);
+            pad = mlkd_matmul_i8_work_bytes(&p);
+        } else if (st.kind == StepKind::AttentionKv4) {
+            mlkd_attention_kv4 p;
+            fillAttentionKv4(km_, st, ptr, p);
+            pad = mlkd_attention_kv4_work_bytes(&p);
         }
         if (pad > 0 && align256(static_cast<size_t>(pad)) <= arena.bytes - used) {
             padOff[si] = used;
@@ -643,6 +704,15 @@ int HipLoadedKernel::runDevice(const DeviceBinding* binds, int n, const double* 
     for (size_t si = 0; si < plan_.steps.size(); ++si) {
         const Step& st = plan_.steps[si];
         int rc = 0;
+        // A workspace of `need` bytes that the step can do without: its size
+        // where there is one, else 0.
+        auto workspace = [&](int64_t need, void** work) -> int64_t {
+            if (need == 0) return 0;
+            if (arena == nullptr) return stepScratch(*rs, si, 0, need, stream, work);
+            if (padOff[si] == SIZE_MAX) return 0;
+            *work = arena->base + padOff[si];
+            return need;
+        };
         switch (st.kind) {
             case StepKind::Fail:
                 if (st.failCode != 0) {
@@ -814,6 +884,34 @@ int HipLoadedKernel::runDevice(const DeviceBinding* binds, int n, const double* 
                     p.work_bytes = stepScratch(*rs, si, 0, need, stream, &p.work);
                 }
                 rc = mlkd_launch_attention(&p, stream);
+                break;
+            }
+            case StepKind::QuantizeRows: {
+                mlkd_quantize_rows p;
+                fillQuantizeRows(km_, st, ptr, p);
+                rc = mlkd_launch_quantize_rows(&p, stream);
+                break;
+            }
+            case StepKind::MatmulI8: {
+                mlkd_matmul_i8 p;
+                fillMatmulI8(km_, st, ptr, p);
+                // Without the workspace the step runs in one range of k.
+                p.work_bytes = workspace(mlkd_matmul_i8_work_bytes(&p), &p.work);
+                rc = mlkd_launch_matmul_i8(&p, stream);
+                break;
+            }
+            case StepKind::StoreKv4:
+            case StepKind::LoadKv4: {
+                mlkd_kv4_rows p;
+                fillKv4Rows(km_, st, ptr, p);
+                rc = st.kind == StepKind::StoreKv4 ? mlkd_launch_store_kv4(&p, stream) : mlkd_launch_load_kv4(&p, stream);
+                break;
+            }
+            case StepKind::AttentionKv4: {
+                mlkd_attention_kv4 p;
+                fillAttentionKv4(km_, st, ptr, p);
+                p.a.work_bytes = workspace(mlkd_attention_kv4_work_bytes(&p), &p.a.work);
+                rc = mlkd_launch_attention_kv4(&p, stream);
                 break;
             }
         }

@@ -206,7 +206,10 @@ MathOp mathFromName(const std::string& s) {
                   {"gelu", MathOp::Gelu}, {"matmul", MathOp::MatMul},
                   {"reduce_sum", MathOp::ReduceSum}, {"softmax", MathOp::Softmax},
                   {"qk_norm_rope", MathOp::QkNormRope}, {"attention", MathOp::Attention},
-                  {"shared_prefix_attention", MathOp::SharedPrefixAttention}};
+                  {"shared_prefix_attention", MathOp::SharedPrefixAttention},
+                  {"quantize_rows", MathOp::QuantizeRows}, {"matmul_i8", MathOp::MatmulI8},
+                  {"store_kv4", MathOp::StoreKv4}, {"load_kv4", MathOp::LoadKv4},
+                  {"attention_kv4", MathOp::AttentionKv4}};
     for (const auto& e : kNames) {
         if (s == e.name) return e.op;
     }
@@ -237,6 +240,8 @@ Dtype dtypeFromName(const std::string& s) {
     if (s == "f64") return Dtype::F64;
     if (s == "bf16") return Dtype::BF16;
     if (s == "i32") return Dtype::I32;
+    if (s == "i8") return Dtype::I8;
+    if (s == "u8") return Dtype::U8;
     return Dtype::Other;
 }
 
@@ -456,6 +461,8 @@ int dtypeBytes(Dtype d) {
         case Dtype::F64: return 8;
         case Dtype::BF16: return 2;
         case Dtype::I32: return 4;
+        case Dtype::I8: return 1;
+        case Dtype::U8: return 1;
         case Dtype::Other: return 0;
     }
     return 0;
@@ -465,13 +472,19 @@ const char* mathOpName(MathOp op) {
     static const char* kNames[] = {"add", "sub", "mul", "div", "neg", "pow", "exp", "log",
                                    "sin", "cos", "tan", "tanh", "sqrt", "rsqrt", "erf", "gelu",
                                    "matmul", "reduce_sum", "softmax", "?",
-                                   "qk_norm_rope", "attention", "shared_prefix_attention"};
+                                   "qk_norm_rope", "attention", "shared_prefix_attention",
+                                   "quantize_rows", "matmul_i8", "store_kv4", "load_kv4", "attention_kv4"};
     return kNames[static_cast<int>(op)];
 }
 
 bool isOperatorCall(const KernelNode& n) {
-    return n.op == KernelOp::Call && (n.math == MathOp::QkNormRope || n.math == MathOp::Attention ||
-                                      n.math == MathOp::SharedPrefixAttention);
+    switch (n.math) {
+        case MathOp::QkNormRope: case MathOp::Attention: case MathOp::SharedPrefixAttention:
+        case MathOp::QuantizeRows: case MathOp::MatmulI8: case MathOp::StoreKv4:
+        case MathOp::LoadKv4: case MathOp::AttentionKv4:
+            return n.op == KernelOp::Call;
+        default: return false;
+    }
 }
 
 bool isUnaryMath(MathOp op) {

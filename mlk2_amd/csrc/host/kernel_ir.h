@@ -25,12 +25,12 @@ enum class MathOp : uint8_t {
     Add, Sub, Mul, Div, Neg, Pow, Exp, Log, Sin, Cos, Tan, Tanh, Sqrt, Rsqrt, Erf, Gelu,
     MatMul, ReduceSum, Softmax, Other,
     // Operators of this backend (Call nodes with named operands and attributes).
-    QkNormRope, Attention, SharedPrefixAttention
+    QkNormRope, Attention, SharedPrefixAttention, QuantizeRows, MatmulI8, StoreKv4, LoadKv4, AttentionKv4
 };
 
 enum class AccumMode : uint8_t { None, Add, Max };
-/// BF16 and I32 buffers are read and written by operator Calls only.
-enum class Dtype : uint8_t { F32, F16, F64, Other, BF16, I32 };
+/// BF16, I32, I8 and U8 buffers are read and written by operator Calls only.
+enum class Dtype : uint8_t { F32, F16, F64, Other, BF16, I32, I8, U8 };
 
 struct KernelOperand {
     enum class Kind : uint8_t { Const, ElemA, ElemB, ScalarParam, Temp, ElemIdx };

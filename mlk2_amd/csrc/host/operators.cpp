@@ -1,5 +1,5 @@
-// Operator Calls of a module: qk_norm_rope, attention and
-// shared_prefix_attention. Their operands are buffers by name, their options
+// Operator Calls of a module: qk_norm_rope, attention, shared_prefix_attention,
+// and those in 8 and 4 bits. Their operands are buffers by name, their options
 // numbers by name; everything the kernels assume of either is checked here,
 // before any device work.
 #include <algorithm>
@@ -17,10 +17,13 @@ namespace {
 
 constexpr const char* kSlotNames[kOperandSlots] = {
     "q",          "k",       "v",          "prefix_k", "prefix_v", "q_weight", "k_weight", "positions", "slots", "q_offsets",
-    "kv_start",   "kv_len",  "prefix_len", "q_out",    "k_out",    "v_out",    "out",      "lse"};
+    "kv_start",   "kv_len",  "prefix_len", "x",        "a",        "a_scale",  "b",        "b_scale",   "bias",  "k_codes",
+    "k_scale",    "v_codes", "v_scale",    "q_out",    "k_out",    "v_out",    "out",      "lse",       "codes_out",
+    "scale_out",  "k_codes_out", "k_scale_out", "v_codes_out", "v_scale_out"};
 
 constexpr int64_t kMaxRows = INT32_MAX;   // rows are named by i32 buffers
 constexpr int kMaxDim = 256, kMaxHeads = 4096;
+constexpr int64_t kMaxInner = (1 << 17) - 1;   // of a product in 8 bits: 2^14 a term, sums below 2^31
 
 int operandCode(Dtype d) {
     switch (d) {
@@ -28,6 +31,8 @@ int operandCode(Dtype d) {
         case Dtype::F16: return MLKD_F16;
         case Dtype::BF16: return MLKD_BF16;
         case Dtype::I32: return MLKD_I32;
+        case Dtype::I8: return MLKD_I8;
+        case Dtype::U8: return MLKD_U8;
         default: return MLKD_F64;
     }
 }
@@ -70,7 +75,7 @@ public:
             const std::string& name = n_.attrs[i].first;
             bool known = false;
             for (const char* a : attrs) known = known || name == a;
-            // "<operand>_at" for the operands that are rows of heads.
+            // "<operand>_at" for the operands that are rows of heads or columns.
             for (const int s : slots) known = known || (rowsOfHeads(s) && name == std::string(kSlotNames[s]) + "_at");
             if (!known) return fail("unknown attribute '" + name + "'");
             for (size_t j = 0; j < i; ++j) {
@@ -111,7 +116,9 @@ public:
     bool heads(int slot, int64_t heads, int64_t dim, Dtype want, Operand& o) {
         if (!has(slot)) return fail(std::string("operand '") + kSlotNames[slot] + "' is missing");
         const KernelBuffer& b = km_.buffers[id(slot)];
-        if (b.dtype != want) return fail(std::string("'") + kSlotNames[slot] + "' has another dtype than 'q'");
+        if (b.dtype != want) {
+            return fail(std::string("'") + kSlotNames[slot] + (want == Dtype::U8 ? "' must be u8" : want == Dtype::I8 ? "' must be i8" : "' has another dtype than 'q'"));
+        }
         o.buffer = id(slot);
         o.rows = b.dims[0];
         o.width = 1;
@@ -127,6 +134,7 @@ public:
 
     /// Operand `slot` as a dense array of exactly `elements` (-1: any number).
     bool dense(int slot, Dtype want, int64_t elements, const char* type, Operand& o) {
+        if (!has(slot)) return fail(std::string("operand '") + kSlotNames[slot] + "' is missing");
         const KernelBuffer& b = km_.buffers[id(slot)];
         o.buffer = id(slot);
         o.rows = 1;
@@ -141,7 +149,8 @@ public:
 
 private:
     static bool rowsOfHeads(int s) {
-        return s <= kOpPrefixV || s == kOpQOut || s == kOpKOut || s == kOpVOut || s == kOpOut;
+        return s <= kOpPrefixV || s == kOpQOut || s == kOpKOut || s == kOpVOut || s == kOpOut || s == kOpX || s == kOpA || s == kOpB ||
+               s == kOpKCodes || s == kOpVCodes || s == kOpCodesOut || s == kOpKCodesOut || s == kOpVCodesOut;
     }
     const KernelModule& km_;
     const KernelNode& n_;
@@ -260,6 +269,31 @@ bool normRope(Reader& r, OperatorStep& o) {
     return disjoint(r, o, columns, inPlace);
 }
 
+/// What attention's forms have alike: the sequences, lse, the options. `keys`
+/// rows of `what`; columns(slot) of each operand.
+template <typename F>
+bool attentionRest(Reader& r, OperatorStep& o, int64_t rows, int64_t keys, const char* what, const F& columns) {
+    if (o.op[kOpOut].rows != rows) return r.fail("'q' and 'out' must have the same rows");
+    if (!sequences(r, o)) return false;
+    if (r.has(kOpKvStart) != r.has(kOpKvLen)) return r.fail("'kv_start' and 'kv_len' come together");
+    if (r.has(kOpKvStart)) {
+        if (!r.dense(kOpKvStart, Dtype::I32, o.sequences, "i32", o.op[kOpKvStart]) ||
+            !r.dense(kOpKvLen, Dtype::I32, o.sequences, "i32", o.op[kOpKvLen])) {
+            return false;
+        }
+    } else if (keys != rows) {
+        return r.fail(std::string(what) + " must have the rows of 'q' where there is no 'kv_start'");
+    }
+    if (r.has(kOpLse) && !r.dense(kOpLse, Dtype::F32, rows * o.heads, "f32", o.op[kOpLse])) return false;
+    int64_t causal = 0;
+    if (!r.real("scale", 1.0 / std::sqrt(static_cast<double>(o.dim)), o.scale) || !r.whole("causal", 1, 0, 1, causal)) return false;
+    if (!(std::fabs(o.scale) >= 1e-20 && std::fabs(o.scale) <= 1e20)) return r.fail("scale must be of 1e-20 .. 1e20 in size");
+    o.causal = causal != 0;
+    int64_t of[kOperandSlots];
+    for (int s = 0; s < kOperandSlots; ++s) of[s] = columns(s);
+    return disjoint(r, o, of, {});
+}
+
 bool attention(Reader& r, OperatorStep& o, bool prefix) {
     bool ok = prefix ? r.names({kOpQ, kOpK, kOpV, kOpPrefixK, kOpPrefixV, kOpPrefixLen, kOpQOffsets, kOpKvStart, kOpKvLen, kOpOut, kOpLse},
                                {"heads", "kv_heads", "dim", "scale", "causal"})
@@ -271,34 +305,113 @@ bool attention(Reader& r, OperatorStep& o, bool prefix) {
     if (!r.heads(kOpK, g, d, dt, o.op[kOpK]) || !r.heads(kOpV, g, d, dt, o.op[kOpV]) || !r.heads(kOpOut, h, d, dt, o.op[kOpOut])) {
         return false;
     }
-    if (o.op[kOpOut].rows != rows) return r.fail("'q' and 'out' must have the same rows");
     if (o.op[kOpV].rows != o.op[kOpK].rows) return r.fail("'k' and 'v' must have the same rows");
-    if (!r.has(kOpQOffsets)) return r.fail("operand 'q_offsets' is missing");
-    if (!sequences(r, o)) return false;
-    if (r.has(kOpKvStart) != r.has(kOpKvLen)) return r.fail("'kv_start' and 'kv_len' come together");
-    if (r.has(kOpKvStart)) {
-        if (!r.dense(kOpKvStart, Dtype::I32, o.sequences, "i32", o.op[kOpKvStart]) ||
-            !r.dense(kOpKvLen, Dtype::I32, o.sequences, "i32", o.op[kOpKvLen])) {
-            return false;
-        }
-    } else if (o.op[kOpK].rows != rows) {
-        return r.fail("'k' must have the rows of 'q' where there is no 'kv_start'");
-    }
     if (prefix) {
         if (!r.heads(kOpPrefixK, g, d, dt, o.op[kOpPrefixK]) || !r.heads(kOpPrefixV, g, d, dt, o.op[kOpPrefixV])) return false;
         if (o.op[kOpPrefixV].rows != o.op[kOpPrefixK].rows) return r.fail("'prefix_k' and 'prefix_v' must have the same rows");
         if (r.has(kOpPrefixLen) && !r.dense(kOpPrefixLen, Dtype::I32, 1, "i32", o.op[kOpPrefixLen])) return false;
     }
-    if (r.has(kOpLse) && !r.dense(kOpLse, Dtype::F32, rows * h, "f32", o.op[kOpLse])) return false;
-    int64_t causal = 0;
-    if (!r.real("scale", 1.0 / std::sqrt(static_cast<double>(d)), o.scale) || !r.whole("causal", 1, 0, 1, causal)) return false;
-    if (!(std::fabs(o.scale) >= 1e-20 && std::fabs(o.scale) <= 1e20)) return r.fail("scale must be of 1e-20 .. 1e20 in size");
-    o.causal = causal != 0;
+    return attentionRest(r, o, rows, o.op[kOpK].rows, "'k'", [&](int s) {
+        return s == kOpQ || s == kOpOut ? h * d : s <= kOpPrefixV ? g * d : o.op[s].width;
+    });
+}
+
+/// Rows of `cols` columns of x in 8-bit integers.
+bool quantizeRows(Reader& r, OperatorStep& o) {
+    int64_t cols = 0;
+    if (!r.names({kOpX, kOpCodesOut, kOpScaleOut}, {"cols"}) || !r.whole("cols", 0, 1, INT32_MAX, cols)) return false;
+    if (!r.has(kOpX)) return r.fail("operand 'x' is missing");
+    if (!floatType(r.dtype(kOpX))) return r.fail("'x' must be f16, bf16 or f32");
+    o.cols = cols;
+    if (!r.heads(kOpX, 1, cols, r.dtype(kOpX), o.op[kOpX]) || !r.heads(kOpCodesOut, 1, cols, Dtype::I8, o.op[kOpCodesOut])) return false;
+    const int64_t rows = o.op[kOpX].rows;
+    if (o.op[kOpCodesOut].rows != rows) return r.fail("'x' and 'codes_out' must have the same rows");
+    if (!r.dense(kOpScaleOut, Dtype::F32, rows, "f32", o.op[kOpScaleOut])) return false;
     int64_t columns[kOperandSlots];
-    for (int s = 0; s < kOperandSlots; ++s) {
-        columns[s] = s == kOpQ || s == kOpOut ? h * d : s <= kOpPrefixV ? g * d : o.op[s].width;
-    }
+    for (int s = 0; s < kOperandSlots; ++s) columns[s] = s == kOpX || s == kOpCodesOut ? cols : o.op[s].width;
     return disjoint(r, o, columns, {});
+}
+
+/// out [m, n] of a [m, inner] and b [n, inner].
+bool matmulI8(Reader& r, OperatorStep& o) {
+    int64_t cols = 0, inner = 0;
+    if (!r.names({kOpA, kOpAScale, kOpB, kOpBScale, kOpBias, kOpOut}, {"cols", "inner"}) || !r.whole("cols", 0, 1, INT32_MAX, cols) ||
+        !r.whole("inner", 0, 1, kMaxInner, inner)) {
+        return false;
+    }
+    o.cols = cols;
+    o.inner = inner;
+    if (!r.heads(kOpA, 1, inner, Dtype::I8, o.op[kOpA]) || !r.heads(kOpB, 1, inner, Dtype::I8, o.op[kOpB])) return false;
+    if (!r.has(kOpOut)) return r.fail("operand 'out' is missing");
+    if (!floatType(r.dtype(kOpOut))) return r.fail("'out' must be f16, bf16 or f32");
+    if (!r.heads(kOpOut, 1, cols, r.dtype(kOpOut), o.op[kOpOut])) return false;
+    if (o.op[kOpB].rows != cols) return r.fail("'b' must have " + std::to_string(cols) + " rows");
+    const int64_t rows = o.op[kOpA].rows;
+    if (o.op[kOpOut].rows != rows) return r.fail("'a' and 'out' must have the same rows");
+    if (!r.dense(kOpAScale, Dtype::F32, rows, "f32", o.op[kOpAScale]) || !r.dense(kOpBScale, Dtype::F32, cols, "f32", o.op[kOpBScale])) {
+        return false;
+    }
+    if (r.has(kOpBias) && !r.dense(kOpBias, Dtype::F32, cols, "f32", o.op[kOpBias])) return false;
+    int64_t columns[kOperandSlots];
+    for (int s = 0; s < kOperandSlots; ++s) columns[s] = s == kOpOut ? cols : s == kOpA || s == kOpB ? inner : o.op[s].width;
+    return disjoint(r, o, columns, {});
+}
+
+/// kv_heads and an even dim of a cache in 4 bits.
+bool packedShape(Reader& r, OperatorStep& o) {
+    int64_t g = 0, d = 0;
+    if (!r.whole("kv_heads", 0, 1, kMaxHeads, g) || !r.whole("dim", 0, 2, kMaxDim, d)) return false;
+    if (d % 2 != 0) return r.fail("dim must be even");
+    o.kvHeads = static_cast<int32_t>(g);
+    o.dim = static_cast<int32_t>(d);
+    return true;
+}
+
+/// The cache's four buffers, from slot `codes` on: codes and scales of k, of v.
+bool packedCache(Reader& r, OperatorStep& o, int codes) {
+    for (const int s : {codes, codes + 2}) {
+        if (!r.heads(s, o.kvHeads, o.dim / 2, Dtype::U8, o.op[s])) return false;
+        if (!r.dense(s + 1, Dtype::F32, o.op[s].rows * o.kvHeads, "f32", o.op[s + 1])) return false;
+    }
+    return o.op[codes].rows == o.op[codes + 2].rows || r.fail("the codes of k and v must have the same rows");
+}
+static_assert(kOpKScale == kOpKCodes + 1 && kOpVCodes == kOpKCodes + 2 && kOpVScale == kOpKCodes + 3, "");
+static_assert(kOpKScaleOut == kOpKCodesOut + 1 && kOpVCodesOut == kOpKCodesOut + 2 && kOpVScaleOut == kOpKCodesOut + 3, "");
+
+bool kv4Rows(Reader& r, OperatorStep& o, bool store) {
+    const int k = store ? kOpK : kOpKOut, v = store ? kOpV : kOpVOut, codes = store ? kOpKCodesOut : kOpKCodes;
+    if (!r.names({k, v, kOpSlots, kOpQOffsets, codes, codes + 1, codes + 2, codes + 3}, {"kv_heads", "dim"}) || !packedShape(r, o)) return false;
+    const int64_t g = o.kvHeads, d = o.dim;
+    if (!r.has(k)) return r.fail(std::string("operand '") + kSlotNames[k] + "' is missing");
+    if (!floatType(r.dtype(k))) return r.fail(std::string("'") + kSlotNames[k] + "' must be f16, bf16 or f32");
+    if (!r.heads(k, g, d, r.dtype(k), o.op[k])) return false;
+    if (r.has(v) && r.dtype(v) != r.dtype(k)) return r.fail("k and v must be of one dtype");
+    if (!r.heads(v, g, d, r.dtype(k), o.op[v]) || !packedCache(r, o, codes)) return false;
+    const int64_t rows = o.op[k].rows;
+    if (o.op[v].rows != rows) return r.fail("k and v must have the same rows");
+    if (r.has(kOpSlots)) {
+        if (!r.dense(kOpSlots, Dtype::I32, rows, "i32", o.op[kOpSlots])) return false;
+    } else if (o.op[codes].rows != rows) {
+        return r.fail("the codes must have the rows of k where there are no slots");
+    }
+    if (r.has(kOpQOffsets) && !sequences(r, o)) return false;
+    int64_t columns[kOperandSlots];
+    for (int s = 0; s < kOperandSlots; ++s) columns[s] = s == k || s == v ? g * d : s == codes || s == codes + 2 ? g * d / 2 : o.op[s].width;
+    return disjoint(r, o, columns, {});
+}
+
+bool attentionKv4(Reader& r, OperatorStep& o) {
+    if (!r.names({kOpQ, kOpKCodes, kOpKScale, kOpVCodes, kOpVScale, kOpQOffsets, kOpKvStart, kOpKvLen, kOpOut, kOpLse},
+                 {"heads", "kv_heads", "dim", "scale", "causal"}) ||
+        !shape(r, o)) {
+        return false;
+    }
+    if (o.dim % 2 != 0) return r.fail("dim must be even");
+    const int64_t h = o.heads, d = o.dim, rows = o.op[kOpQ].rows;
+    if (!packedCache(r, o, kOpKCodes) || !r.heads(kOpOut, h, d, r.dtype(kOpQ), o.op[kOpOut])) return false;
+    return attentionRest(r, o, rows, o.op[kOpKCodes].rows, "'k_codes'", [&](int s) {
+        return s == kOpQ || s == kOpOut ? h * d : s == kOpKCodes || s == kOpVCodes ? o.kvHeads * d / 2 : o.op[s].width;
+    });
 }
 
 void* place(const Step& st, int slot, const std::vector<void*>& ptr, int bytes) {
@@ -309,7 +422,28 @@ void* place(const Step& st, int slot, const std::vector<void*>& ptr, int bytes) 
 
 }  // namespace
 
-bool isOperator(const Step& st) { return st.kind == StepKind::NormRope || st.kind == StepKind::Attention; }
+bool isOperator(const Step& st) { return st.kind >= StepKind::NormRope; }
+
+Dtype operatorDtype(const KernelModule& km, const Step& st) {
+    const Operand* op = st.oper.op;
+    const int slot = st.kind == StepKind::QuantizeRows ? kOpX
+                     : st.kind == StepKind::MatmulI8   ? kOpOut
+                     : st.kind == StepKind::StoreKv4   ? kOpK
+                     : st.kind == StepKind::LoadKv4    ? kOpKOut
+                                                       : kOpQ;
+    return km.buffers[op[slot].buffer].dtype;
+}
+
+int64_t operatorRows(const Step& st) {
+    const Operand* op = st.oper.op;
+    switch (st.kind) {
+        case StepKind::QuantizeRows: return op[kOpX].rows;
+        case StepKind::StoreKv4: return op[kOpK].rows;
+        case StepKind::LoadKv4: return op[kOpKOut].rows;
+        case StepKind::MatmulI8: return op[kOpOut].rows;
+        default: return op[kOpQ].rows;
+    }
+}
 
 Result<Step> operatorStep(const KernelModule& km, const KernelNode& call) {
     Step st;
@@ -319,6 +453,23 @@ Result<Step> operatorStep(const KernelModule& km, const KernelNode& call) {
         st.kind = StepKind::NormRope;
         st.what = "qk-norm-rope";
         ok = normRope(r, st.oper);
+    } else if (call.math == MathOp::QuantizeRows) {
+        st.kind = StepKind::QuantizeRows;
+        st.what = "quantize-rows";
+        ok = quantizeRows(r, st.oper);
+    } else if (call.math == MathOp::MatmulI8) {
+        st.kind = StepKind::MatmulI8;
+        st.what = "matmul-i8";
+        ok = matmulI8(r, st.oper);
+    } else if (call.math == MathOp::StoreKv4 || call.math == MathOp::LoadKv4) {
+        const bool store = call.math == MathOp::StoreKv4;
+        st.kind = store ? StepKind::StoreKv4 : StepKind::LoadKv4;
+        st.what = store ? "store-kv4" : "load-kv4";
+        ok = kv4Rows(r, st.oper, store);
+    } else if (call.math == MathOp::AttentionKv4) {
+        st.kind = StepKind::AttentionKv4;
+        st.what = "attention-kv4";
+        ok = attentionKv4(r, st.oper);
     } else {
         const bool prefix = call.math == MathOp::SharedPrefixAttention;
         st.kind = StepKind::Attention;
@@ -399,6 +550,78 @@ void fillAttention(const KernelModule& km, const Step& st, const std::vector<voi
     p.prefix_v_stride = o.op[kOpPrefixV].width;
     p.out_stride = o.op[kOpOut].width;
     p.scale = o.scale;
+}
+
+void fillQuantizeRows(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_quantize_rows& p) {
+    p = {};
+    const OperatorStep& o = st.oper;
+    const Dtype dt = operatorDtype(km, st);
+    p.x = place(st, kOpX, ptr, dtypeBytes(dt));
+    p.codes = static_cast<int8_t*>(place(st, kOpCodesOut, ptr, 1));
+    p.scale = static_cast<float*>(place(st, kOpScaleOut, ptr, 0));
+    p.dtype = operandCode(dt);
+    p.rows = o.op[kOpX].rows;
+    p.cols = o.cols;
+    p.x_stride = o.op[kOpX].width;
+    p.codes_stride = o.op[kOpCodesOut].width;
+}
+
+void fillMatmulI8(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_matmul_i8& p) {
+    p = {};
+    const OperatorStep& o = st.oper;
+    const Dtype dt = operatorDtype(km, st);
+    p.a = static_cast<const int8_t*>(place(st, kOpA, ptr, 1));
+    p.b = static_cast<const int8_t*>(place(st, kOpB, ptr, 1));
+    p.a_scale = static_cast<const float*>(place(st, kOpAScale, ptr, 0));
+    p.b_scale = static_cast<const float*>(place(st, kOpBScale, ptr, 0));
+    p.bias = static_cast<const float*>(place(st, kOpBias, ptr, 0));
+    p.out = place(st, kOpOut, ptr, dtypeBytes(dt));
+    p.dtype = operandCode(dt);
+    p.m = o.op[kOpA].rows;
+    p.n = o.cols;
+    p.k = o.inner;
+    p.lda = o.op[kOpA].width;
+    p.ldb = o.op[kOpB].width;
+    p.ldo = o.op[kOpOut].width;
+}
+
+void fillKv4Rows(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_kv4_rows& p) {
+    p = {};
+    const OperatorStep& o = st.oper;
+    const bool store = st.kind == StepKind::StoreKv4;
+    const int k = store ? kOpK : kOpKOut, v = store ? kOpV : kOpVOut, codes = store ? kOpKCodesOut : kOpKCodes;
+    const Dtype dt = operatorDtype(km, st);
+    p.k = place(st, k, ptr, dtypeBytes(dt));
+    p.v = place(st, v, ptr, dtypeBytes(dt));
+    p.k_codes = static_cast<uint8_t*>(place(st, codes, ptr, 1));
+    p.k_scale = static_cast<float*>(place(st, codes + 1, ptr, 0));
+    p.v_codes = static_cast<uint8_t*>(place(st, codes + 2, ptr, 1));
+    p.v_scale = static_cast<float*>(place(st, codes + 3, ptr, 0));
+    p.slots = static_cast<const int32_t*>(place(st, kOpSlots, ptr, 0));
+    p.q_offsets = static_cast<const int32_t*>(place(st, kOpQOffsets, ptr, 0));
+    p.dtype = operandCode(dt);
+    p.kv_heads = o.kvHeads;
+    p.dim = o.dim;
+    p.sequences = o.sequences;
+    p.tokens = o.op[k].rows;
+    p.cache_rows = o.op[codes].rows;
+    p.k_stride = o.op[k].width;
+    p.v_stride = o.op[v].width;
+    p.k_codes_stride = o.op[codes].width;
+    p.v_codes_stride = o.op[codes + 2].width;
+}
+
+void fillAttentionKv4(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_attention_kv4& p) {
+    p = {};
+    const OperatorStep& o = st.oper;
+    fillAttention(km, st, ptr, p.a);   // all but the keys and values
+    p.a.k = place(st, kOpKCodes, ptr, 1);
+    p.a.v = place(st, kOpVCodes, ptr, 1);
+    p.a.kv_rows = o.op[kOpKCodes].rows;
+    p.a.k_stride = o.op[kOpKCodes].width;
+    p.a.v_stride = o.op[kOpVCodes].width;
+    p.k_scale = static_cast<const float*>(place(st, kOpKScale, ptr, 0));
+    p.v_scale = static_cast<const float*>(place(st, kOpVScale, ptr, 0));
 }
 
 }  // namespace mlk::hip

@@ -1080,9 +1080,7 @@ void markTemps(const KernelModule& km, const Step& st, std::vector<bool>& need) 
         case StepKind::Nest:
             for (const uint32_t b : st.nestBufs) mark(b);
             break;
-        case StepKind::NormRope:
-        case StepKind::Attention:   // no temps among their operands
-        case StepKind::Fail:
+        default:   // Fail, and operators: no temps among their operands
             break;
     }
 }
@@ -1118,13 +1116,12 @@ void stepIO(const Step& st, std::vector<uint32_t>& reads, std::vector<uint32_t>&
             reads.push_back(st.bias);
             writes.push_back(st.s);
             break;
-        case StepKind::NormRope:
-        case StepKind::Attention:
+        case StepKind::Fail: break;
+        default:
             for (int i = 0; i < kOperandSlots; ++i) {
                 if (st.oper.op[i].buffer != kInvalidId) (i < kFirstOpOutput ? reads : writes).push_back(st.oper.op[i].buffer);
             }
             break;
-        case StepKind::Fail: break;
     }
 }
 
@@ -1220,11 +1217,8 @@ std::string policyFor(const KernelModule& km, const std::vector<Step>& steps) {
                 else gemm32 = true;
                 break;
             case StepKind::ScoreSoftmax: score = true; break;
-            case StepKind::NormRope:
-            case StepKind::Attention:
-                (km.buffers[st.oper.op[kOpQ].buffer].dtype == Dtype::F32 ? oper32 : oper16) = true;
-                break;
             case StepKind::Fail: break;
+            default: (operatorDtype(km, st) == Dtype::F32 ? oper32 : oper16) = true; break;
         }
     }
     bool crossF16 = false;
@@ -1353,7 +1347,7 @@ Result<Plan> planModule(const KernelModule& input) {
             plan.steps.push_back(std::move(*ns));
         }
     }
-    // Only the operators read and write bf16 and i32 buffers.
+    // Only the operators read and write these types.
     std::vector<uint32_t> reads, writes;
     for (const Step& st : plan.steps) {
         if (isOperator(st)) continue;
@@ -1361,7 +1355,7 @@ Result<Plan> planModule(const KernelModule& input) {
         reads.insert(reads.end(), writes.begin(), writes.end());
         reads.insert(reads.end(), st.nestBufs.begin(), st.nestBufs.end());
         for (const uint32_t b : reads) {
-            if (b < km.buffers.size() && (km.buffers[b].dtype == Dtype::BF16 || km.buffers[b].dtype == Dtype::I32)) {
+            if (b < km.buffers.size() && km.buffers[b].dtype > Dtype::Other) {
                 return err(ErrorCode::UnsupportedCapability, "buffer dtype outside f16/f32/f64: " + km.buffers[b].name);
             }
         }

@@ -13,12 +13,18 @@
 
 namespace mlk::hip {
 
-enum class StepKind : uint8_t { Elementwise, Softmax, Gemm, RowSum, ScoreSoftmax, Nest, Fail, NormRope, Attention };
+enum class StepKind : uint8_t {
+    Elementwise, Softmax, Gemm, RowSum, ScoreSoftmax, Nest, Fail,
+    // Operator Calls.
+    NormRope, Attention, QuantizeRows, MatmulI8, StoreKv4, LoadKv4, AttentionKv4
+};
 
 /// Operands of the operator Calls; each names a buffer of the module.
 enum OperandSlot : int {
     kOpQ, kOpK, kOpV, kOpPrefixK, kOpPrefixV, kOpQWeight, kOpKWeight, kOpPositions, kOpSlots, kOpQOffsets, kOpKvStart,
-    kOpKvLen, kOpPrefixLen, kOpQOut, kOpKOut, kOpVOut, kOpOut, kOpLse, kOperandSlots
+    kOpKvLen, kOpPrefixLen, kOpX, kOpA, kOpAScale, kOpB, kOpBScale, kOpBias, kOpKCodes, kOpKScale, kOpVCodes, kOpVScale,
+    kOpQOut, kOpKOut, kOpVOut, kOpOut, kOpLse, kOpCodesOut, kOpScaleOut, kOpKCodesOut, kOpKScaleOut, kOpVCodesOut,
+    kOpVScaleOut, kOperandSlots
 };
 constexpr int kFirstOpOutput = kOpQOut;
 
@@ -33,6 +39,7 @@ struct Operand {
 struct OperatorStep {
     Operand op[kOperandSlots];
     int32_t heads{0}, kvHeads{0}, dim{0}, sequences{0};
+    int64_t cols{0}, inner{0};
     int32_t rot{0}, axes{1}, sections[3]{0, 0, 0};
     bool interleaved{false}, causal{true};
     double scale{0.0}, eps{0.0};
@@ -120,7 +127,7 @@ struct Step {
     bool narrowRoundTrip{false};
     bool touchesF16{false};
 
-    // NormRope / Attention.
+    // Operator Calls.
     OperatorStep oper;
 
     // Launch form of a hand-written kernel (-1: the kernel's default); set
@@ -176,6 +183,14 @@ bool isOperator(const Step& st);
 /// Launch descriptors of an operator step; `ptr` holds an address per buffer id.
 void fillNormRope(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_norm_rope& p);
 void fillAttention(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_attention& p);
+void fillQuantizeRows(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_quantize_rows& p);
+void fillMatmulI8(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_matmul_i8& p);
+void fillKv4Rows(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_kv4_rows& p);
+void fillAttentionKv4(const KernelModule& km, const Step& st, const std::vector<void*>& ptr, mlkd_attention_kv4& p);
+/// Rows of an operator's results.
+int64_t operatorRows(const Step& st);
+/// The rows' dtype of an operator step: what its results are rounded to.
+Dtype operatorDtype(const KernelModule& km, const Step& st);
 
 /// Launch forms of a loop-nest step (nestgen.cpp): 0 the step's own kernel
 /// (its LDS slabs, 256 threads per workgroup); 1 the same kernel without

@@ -82,6 +82,11 @@ const char* kindName(StepKind k) {
         case StepKind::Nest: return "loop-nest";
         case StepKind::NormRope: return "qk-norm-rope";
         case StepKind::Attention: return "attention";
+        case StepKind::QuantizeRows: return "quantize-rows";
+        case StepKind::MatmulI8: return "matmul-i8";
+        case StepKind::StoreKv4: return "store-kv4";
+        case StepKind::LoadKv4: return "load-kv4";
+        case StepKind::AttentionKv4: return "attention-kv4";
         case StepKind::Fail: return "empty";
     }
     return "?";
@@ -273,7 +278,7 @@ double peakOpsPerSec(const KernelModule& km, const Plan& plan) {
     for (const Step& st : plan.steps) {
         if ((st.kind == StepKind::Gemm && st.a != kInvalidId && km.buffers[st.a].dtype == Dtype::F16) ||
             st.kind == StepKind::ScoreSoftmax ||
-            (st.kind == StepKind::Attention && km.buffers[st.oper.op[kOpQ].buffer].dtype != Dtype::F32)) {
+            st.kind == StepKind::AttentionKv4 || (st.kind == StepKind::Attention && operatorDtype(km, st) != Dtype::F32)) {
             return 2.5e15;
         }
     }
@@ -437,6 +442,16 @@ std::string launchCoverage(const KernelModule& km, const Step& st, int64_t eleme
             workgroups = instances;
             perGroup = 1;
             form = "query heads, by the lengths in the buffers";
+            break;
+        case StepKind::QuantizeRows:
+        case StepKind::MatmulI8:
+        case StepKind::StoreKv4:
+        case StepKind::LoadKv4:
+        case StepKind::AttentionKv4:
+            instances = operatorRows(st);
+            workgroups = instances;
+            perGroup = 1;
+            form = "rows, by the sizes of the buffers";
             break;
         case StepKind::Fail:
             covered = false;
@@ -637,6 +652,10 @@ int HipLoadedKernel::autotune(const DeviceBinding* binds, int n, const double* s
                     int32_t i;
                     std::memcpy(&i, raw.data() + e * 4, 4);
                     v[static_cast<size_t>(e)] = i;
+                } else if (kb.dtype == Dtype::I8) {
+                    v[static_cast<size_t>(e)] = static_cast<int8_t>(raw[static_cast<size_t>(e)]);
+                } else if (kb.dtype == Dtype::U8) {
+                    v[static_cast<size_t>(e)] = raw[static_cast<size_t>(e)];
                 } else {
                     _Float16 h;
                     std::memcpy(&h, raw.data() + e * 2, 2);

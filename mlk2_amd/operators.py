@@ -27,6 +27,19 @@ the outputs. The operators and their operands:
     The same with every sequence's keys behind the rows of prefix_k, prefix_v
     (the first ``prefix_len`` of them).
 
+``quantize_rows``
+    Rows of x as 8-bit integers: scale_out[t] = max |x[t]| / 127, codes_out[t]
+    = x[t] / scale_out[t] rounded (half way to even).
+``matmul_i8``
+    out[t, n] = (sum of a[t, k] b[n, k]) a_scale[t] b_scale[n] + bias[n]: rows
+    a and b of 8-bit integers (b a row for each output channel), exact sums.
+``store_kv4``, ``load_kv4``
+    Heads of k and v to the rows ``slots`` of a cache in 4 bits, and back: a
+    scale for each row and head, its largest magnitude over 6, and 4-bit
+    floating-point numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign), two to a byte.
+``attention_kv4``
+    ``attention`` whose keys and values are such a cache's rows.
+
 Types: f16, bf16 or f32, the same for all rows; sums are held in f32 and each
 output is rounded once. Attention's weights are rounded to the type of v before
 they meet it, so that f16 and bf16 run on the matrix cores; their sum is of the
@@ -154,3 +167,168 @@ def shared_prefix_attention_module(tokens: int, *, prefix_rows: int, kv_rows: Op
     if prefix_len:
         op["prefix_len"] = _buffer(km, "prefix_len", "i32", [1])
     return _attention(km, op, tokens, kv_rows, sequences, heads, kv_heads, dim, dtype, causal, scale, lse)
+
+
+def add_quantize_rows(km: KernelModule, operands: dict, *, cols: int, columns: Optional[dict] = None) -> int:
+    """Appends a quantize_rows Call. ``operands`` maps x, codes_out and
+    scale_out to buffer ids."""
+    attrs = dict(cols=cols)
+    attrs.update({f"{k}_at": v for k, v in (columns or {}).items()})
+    return _call(km, "quantize_rows", operands, attrs)
+
+
+def add_matmul_i8(km: KernelModule, operands: dict, *, cols: int, inner: int, columns: Optional[dict] = None) -> int:
+    """Appends a matmul_i8 Call. ``operands`` maps a, a_scale, b, b_scale, bias
+    and out to buffer ids (bias None or absent: without it)."""
+    attrs = dict(cols=cols, inner=inner)
+    attrs.update({f"{k}_at": v for k, v in (columns or {}).items()})
+    return _call(km, "matmul_i8", operands, attrs)
+
+
+def add_store_kv4(km: KernelModule, operands: dict, *, kv_heads: int, dim: int, columns: Optional[dict] = None) -> int:
+    """Appends a store_kv4 Call. ``operands`` maps k, v, slots, q_offsets,
+    k_codes_out, k_scale_out, v_codes_out and v_scale_out to buffer ids (slots
+    and q_offsets None or absent: without them)."""
+    attrs = dict(kv_heads=kv_heads, dim=dim)
+    attrs.update({f"{k}_at": v for k, v in (columns or {}).items()})
+    return _call(km, "store_kv4", operands, attrs)
+
+
+def add_load_kv4(km: KernelModule, operands: dict, *, kv_heads: int, dim: int, columns: Optional[dict] = None) -> int:
+    """Appends a load_kv4 Call. ``operands`` maps k_codes, k_scale, v_codes,
+    v_scale, slots, q_offsets, k_out and v_out to buffer ids."""
+    attrs = dict(kv_heads=kv_heads, dim=dim)
+    attrs.update({f"{k}_at": v for k, v in (columns or {}).items()})
+    return _call(km, "load_kv4", operands, attrs)
+
+
+def add_attention_kv4(km: KernelModule, operands: dict, *, heads: int, kv_heads: int, dim: int, causal: bool = True,
+                      scale: Optional[float] = None, columns: Optional[dict] = None) -> int:
+    """Appends an attention_kv4 Call. ``operands`` maps q, k_codes, k_scale,
+    v_codes, v_scale, q_offsets, kv_start, kv_len, out and lse to buffer ids."""
+    attrs = dict(heads=heads, kv_heads=kv_heads, dim=dim, causal=int(causal), scale=scale)
+    attrs.update({f"{k}_at": v for k, v in (columns or {}).items()})
+    return _call(km, "attention_kv4", operands, attrs)
+
+
+def quantize_rows_module(rows: int, cols: int, *, dtype: str = "bf16") -> KernelModule:
+    """Buffers: x [rows, cols]; outputs codes [rows, cols] i8, scale [rows]."""
+    km = KernelModule(name="quantize_rows")
+    op = {"x": _buffer(km, "x", dtype, [rows, cols])}
+    op["codes_out"] = _buffer(km, "codes", "i8", [rows, cols], output=True)
+    op["scale_out"] = _buffer(km, "scale", "f32", [rows], output=True)
+    add_quantize_rows(km, op, cols=cols)
+    return km
+
+
+def _weights(km: KernelModule, cols: int, inner: int, bias: bool) -> dict:
+    op = {"b": _buffer(km, "b", "i8", [cols, inner]), "b_scale": _buffer(km, "b_scale", "f32", [cols])}
+    if bias:
+        op["bias"] = _buffer(km, "bias", "f32", [cols])
+    return op
+
+
+def matmul_i8_module(rows: int, cols: int, inner: int, *, dtype: str = "bf16", bias: bool = False) -> KernelModule:
+    """Buffers: a [rows, inner] i8, a_scale [rows], b [cols, inner] i8, b_scale
+    [cols], bias [cols] (with ``bias``); output out [rows, cols]."""
+    km = KernelModule(name="matmul_i8")
+    op = {"a": _buffer(km, "a", "i8", [rows, inner]), "a_scale": _buffer(km, "a_scale", "f32", [rows])}
+    op.update(_weights(km, cols, inner, bias))
+    op["out"] = _buffer(km, "out", dtype, [rows, cols], output=True)
+    add_matmul_i8(km, op, cols=cols, inner=inner)
+    return km
+
+
+def linear_i8_module(rows: int, cols: int, inner: int, *, dtype: str = "bf16", bias: bool = False) -> KernelModule:
+    """quantize_rows, then matmul_i8 of its rows. Buffers: x [rows, inner], b
+    [cols, inner] i8, b_scale [cols], bias [cols] (with ``bias``); outputs codes
+    [rows, inner] i8, scale [rows], out [rows, cols]."""
+    km = KernelModule(name="linear_i8")
+    x = _buffer(km, "x", dtype, [rows, inner])
+    op = _weights(km, cols, inner, bias)
+    op["a"] = _buffer(km, "codes", "i8", [rows, inner], output=True)
+    op["a_scale"] = _buffer(km, "scale", "f32", [rows], output=True)
+    op["out"] = _buffer(km, "out", dtype, [rows, cols], output=True)
+    add_quantize_rows(km, {"x": x, "codes_out": op["a"], "scale_out": op["a_scale"]}, cols=inner)
+    add_matmul_i8(km, op, cols=cols, inner=inner)
+    return km
+
+
+def _cache_kv4(km: KernelModule, rows: int, kv_heads: int, dim: int, output: bool) -> dict:
+    op = {}
+    for part in "kv":
+        op[f"{part}_codes"] = _buffer(km, f"{part}_codes", "u8", [rows, kv_heads, dim // 2], output)
+        op[f"{part}_scale"] = _buffer(km, f"{part}_scale", "f32", [rows, kv_heads], output)
+    return op
+
+
+def _tokens(km: KernelModule, tokens: int, cache_rows: Optional[int], sequences: Optional[int]) -> dict:
+    op = {}
+    if cache_rows is not None:
+        op["slots"] = _buffer(km, "slots", "i32", [tokens])
+    if sequences is not None:
+        op["q_offsets"] = _buffer(km, "q_offsets", "i32", [sequences + 1])
+    return op
+
+
+def store_kv4_module(tokens: int, *, kv_heads: int, dim: int, dtype: str = "bf16", cache_rows: Optional[int] = None,
+                     sequences: Optional[int] = None) -> KernelModule:
+    """Buffers: k and v [tokens, kv_heads, dim], slots [tokens] (with
+    ``cache_rows``), q_offsets [sequences + 1] (with ``sequences``); outputs
+    k_codes [cache_rows or tokens, kv_heads, dim / 2] u8, k_scale [.., kv_heads],
+    v_codes, v_scale."""
+    km = KernelModule(name="store_kv4")
+    op = {p: _buffer(km, p, dtype, [tokens, kv_heads, dim]) for p in "kv"}
+    op.update(_tokens(km, tokens, cache_rows, sequences))
+    cache = _cache_kv4(km, tokens if cache_rows is None else cache_rows, kv_heads, dim, True)
+    op.update({f"{name}_out": b for name, b in cache.items()})
+    add_store_kv4(km, op, kv_heads=kv_heads, dim=dim)
+    return km
+
+
+def load_kv4_module(tokens: int, *, kv_heads: int, dim: int, dtype: str = "bf16", cache_rows: Optional[int] = None,
+                    sequences: Optional[int] = None) -> KernelModule:
+    """Buffers: k_codes, k_scale, v_codes and v_scale as ``store_kv4_module``
+    has them, slots, q_offsets; outputs k and v [tokens, kv_heads, dim]."""
+    km = KernelModule(name="load_kv4")
+    op = _cache_kv4(km, tokens if cache_rows is None else cache_rows, kv_heads, dim, False)
+    op.update(_tokens(km, tokens, cache_rows, sequences))
+    op.update({f"{p}_out": _buffer(km, p, dtype, [tokens, kv_heads, dim], output=True) for p in "kv"})
+    add_load_kv4(km, op, kv_heads=kv_heads, dim=dim)
+    return km
+
+
+def store_load_kv4_module(tokens: int, *, cache_rows: int, kv_heads: int, dim: int, dtype: str = "bf16",
+                          read_dtype: Optional[str] = None) -> KernelModule:
+    """store_kv4, then load_kv4 of the same rows. Buffers: k, v, slots; outputs
+    k_codes, k_scale, v_codes, v_scale, and k_read and v_read [tokens, kv_heads,
+    dim] of ``read_dtype`` (``dtype``)."""
+    km = store_kv4_module(tokens, kv_heads=kv_heads, dim=dim, dtype=dtype, cache_rows=cache_rows)
+    km.name = "store_load_kv4"
+    stored = km.nodes[-1].operands
+    op = {name[:-4]: b for name, b in stored.items() if name.endswith("_out")}
+    op["slots"] = stored["slots"]
+    op.update({f"{p}_out": _buffer(km, f"{p}_read", read_dtype or dtype, [tokens, kv_heads, dim], output=True) for p in "kv"})
+    add_load_kv4(km, op, kv_heads=kv_heads, dim=dim)
+    return km
+
+
+def attention_kv4_module(tokens: int, *, kv_rows: Optional[int] = None, sequences: int, heads: int, kv_heads: int, dim: int,
+                         dtype: str = "bf16", causal: bool = True, scale: Optional[float] = None,
+                         lse: bool = False) -> KernelModule:
+    """Buffers: q [tokens, heads, dim], k_codes [kv_rows or tokens, kv_heads, dim
+    / 2] u8, k_scale [.., kv_heads], v_codes, v_scale, q_offsets [sequences + 1],
+    kv_start and kv_len [sequences] (with ``kv_rows``); outputs out like q, lse
+    [tokens, heads] (with ``lse``)."""
+    km = KernelModule(name="attention_kv4")
+    op = {"q": _buffer(km, "q", dtype, [tokens, heads, dim])}
+    op.update(_cache_kv4(km, tokens if kv_rows is None else kv_rows, kv_heads, dim, False))
+    op["q_offsets"] = _buffer(km, "q_offsets", "i32", [sequences + 1])
+    if kv_rows is not None:
+        op["kv_start"] = _buffer(km, "kv_start", "i32", [sequences])
+        op["kv_len"] = _buffer(km, "kv_len", "i32", [sequences])
+    op["out"] = _buffer(km, "out", dtype, [tokens, heads, dim], output=True)
+    if lse:
+        op["lse"] = _buffer(km, "lse", "f32", [tokens, heads], output=True)
+    add_attention_kv4(km, op, heads=heads, kv_heads=kv_heads, dim=dim, causal=causal, scale=scale)
+    return km
