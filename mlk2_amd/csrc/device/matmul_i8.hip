@@ -1,4 +1,10 @@
-// Products of rows in 8-bit integers, with a scale for each row and column.
+// Products of rows in 8-bit integers, out = (a b^T) a_scale b_scale + bias: exact
+// sums in 32 bits, turned to f32 and scaled as they are stored.
+//
+// v_mfma_i32_16x16x64_i8 takes 16 bytes a lane of either operand, 64 bytes of k
+// of 16 rows, and both operands have their k along their rows, so that a wave's
+// 16-byte pieces are its fragments as they stand. Operand b is the instruction's
+// first: a lane then holds four neighbouring columns of one row of out.
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -7,22 +13,396 @@
 #include <string>
 
 #include "runtime_abi.h"
+#include "xcd.h"
 
 namespace {
 
-/// A thread an output, with any sizes, strides and alignment.
+using i32x4 = int __attribute__((ext_vector_type(4)));
+
+constexpr int kStep = 64;     // bytes of k that an instruction takes
+constexpr int kStages = 4;    // steps in LDS
+
+__device__ __align__(16) const uint32_t kZero16[4] = {0u, 0u, 0u, 0u};
+
+__device__ __forceinline__ i32x4 mfma(i32x4 b, i32x4 a, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, c, 0, 0, 0); }
+
+/// 16 bytes at `from`, of any alignment, of which `left` are there; the others
+/// are zeros.
+__device__ __forceinline__ i32x4 piece(const int8_t* from, int64_t left) {
+    i32x4 v = {};
+    if (left >= 16) {
+        __builtin_memcpy(&v, from, 16);
+    } else if (left > 0) {
+        for (int i = 0; i < left; ++i) v[i >> 2] |= static_cast<int>(static_cast<uint8_t>(from[i])) << (i & 3) * 8;
+    }
+    return v;
+}
+
 template <typename T>
-__global__ __launch_bounds__(256) void matmulI8Any(mlkd_matmul_i8 p) {
+__device__ __forceinline__ T scaled(int sum, float sa, float sb, float bias, bool has) {
+    float v = static_cast<float>(sum) * sa * sb;
+    if (has) v += bias;
+    return static_cast<T>(v);
+}
+
+/// Columns n .. n + 3 of row m from their sums. `wide`: four outputs at their
+/// own alignment at once.
+template <typename T>
+__device__ __forceinline__ void store4(const mlkd_matmul_i8& p, int64_t m, int64_t n, i32x4 sum, float sa, bool wide) {
+    using V = T __attribute__((ext_vector_type(4)));
+    T* out = static_cast<T*>(p.out) + m * p.ldo + n;
+    const bool has = p.bias != nullptr;
+    if (wide && n + 4 <= p.n) {
+        V v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = scaled<T>(sum[e], sa, p.b_scale[n + e], has ? p.bias[n + e] : 0.0f, has);
+        *reinterpret_cast<V*>(out) = v;
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        if (n + e < p.n) out[e] = scaled<T>(sum[e], sa, p.b_scale[n + e], has ? p.bias[n + e] : 0.0f, has);
+    }
+}
+
+// ------------------------------------------------------------- few rows ----
+/// Up to 16 MB rows of a: eight waves take the 256-byte pieces of k in turn, 16
+/// NB rows of b straight from memory, and their sums are added in LDS. A launch
+/// reads b once and nothing waits but on those reads.
+template <typename T, int MB, int NB>
+__global__ __launch_bounds__(512) void matmulI8Few(mlkd_matmul_i8 p, int wide) {
+    constexpr int U = 4;   // steps of a piece
+    __shared__ i32x4 sums[8][MB * NB][64];
+    const int ln = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int l16 = ln & 15, g = ln >> 4;
+    const int64_t blocks = (p.n + 16 * NB - 1) / (16 * NB);
+    for (int64_t block = xcdShare(blockIdx.x, gridDim.x); block < blocks; block += gridDim.x) {
+        const int64_t n0 = block * (16 * NB);
+        const int8_t *a[MB], *b[NB];
+#pragma unroll
+        for (int i = 0; i < MB; ++i) a[i] = p.a + min(int64_t{i * 16 + l16}, p.m - 1) * p.lda + g * 16;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) b[i] = p.b + min(n0 + i * 16 + l16, p.n - 1) * p.ldb + g * 16;
+        i32x4 acc[MB][NB] = {};
+        for (int64_t k = wave * (U * kStep); k < p.k; k += 8 * U * kStep) {
+            i32x4 av[U][MB], bv[U][NB];
+            if (k + U * kStep <= p.k) {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) __builtin_memcpy(&bv[u][i], b[i] + k + u * kStep, 16);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                    for (int i = 0; i < MB; ++i) __builtin_memcpy(&av[u][i], a[i] + k + u * kStep, 16);
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int64_t left = p.k - k - u * kStep - g * 16;
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) bv[u][i] = piece(b[i] + k + u * kStep, left);
+#pragma unroll
+                    for (int i = 0; i < MB; ++i) av[u][i] = piece(a[i] + k + u * kStep, left);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int i = 0; i < MB; ++i) {
+#pragma unroll
+                    for (int j = 0; j < NB; ++j) acc[i][j] = mfma(bv[u][j], av[u][i], acc[i][j]);
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MB; ++i) {
+#pragma unroll
+            for (int j = 0; j < NB; ++j) sums[wave][i * NB + j][ln] = acc[i][j];
+        }
+        __syncthreads();
+        for (int t = wave; t < MB * NB; t += 8) {
+            i32x4 sum = sums[0][t][ln];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) sum += sums[w][t][ln];
+            const int64_t m = t / NB * 16 + l16, n = n0 + t % NB * 16 + 4 * g;
+            if (m < p.m && n < p.n) store4<T>(p, m, n, sum, p.a_scale[m], wide != 0);
+        }
+        __syncthreads();
+    }
+}
+
+// ---------------------------------------------------------------- tiles ----
+struct TileArgs {
+    mlkd_matmul_i8 p;
+    int tilesM, tilesN, splits, wide;
+    int* work;   // [splits][m][n] sums of the ranges of k, or NULL
+};
+
+/// A tile of WM x WN waves of MT x NT products of 16 x 16 each, over steps of 64
+/// bytes of k through a ring of four in LDS.
+///
+/// ALIGNED (rows of a and b in whole 16-byte pieces at 16 bytes): the rows go
+/// straight to LDS, three steps ahead. Otherwise through registers, asked for
+/// three steps ahead and written to LDS a step later. Rows past the last repeat
+/// it, pieces past k are zeros.
+///
+/// LDS holds 64-byte rows, piece c of row r at c ^ (r / 4 % 4): a fragment's
+/// read takes one piece of 16 rows at a time, which then lie in all banks. In
+/// each step the products go in two halves: while the first runs, the second's
+/// rows of a are read; while the second runs, the next step's fragments are read
+/// and the loads of the step three ahead are asked for, in a fixed order, a memory
+/// instruction behind every other product or so.
+template <typename T, int WM, int WN, int MT, int NT, bool ALIGNED>
+__global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) {
+    constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
+    constexpr int kStage = (BM + BN) * kStep, LOADS = (BM + BN) / 16 / NW, HM = MT / 2;
+    static_assert(LOADS * NW * 16 == BM + BN && HM * 2 == MT, "whole loads and halves");
+    extern __shared__ __align__(16) char lds[];
+    const mlkd_matmul_i8& p = args.p;
+    const int ln = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+    const int l16 = ln & 15, g = ln >> 4, wm = wave / WN, wn = wave % WN;
+    // Tiles by XCD, those of one in bands of four tile rows.
+    const int id = xcdShare(blockIdx.x, gridDim.x), split = id % args.splits, tile = id / args.splits;
+    const int band = tile / (4 * args.tilesN), rest = tile - band * 4 * args.tilesN, high = min(4, args.tilesM - band * 4);
+    const int64_t row0 = static_cast<int64_t>(band * 4 + rest % high) * BM, col0 = static_cast<int64_t>(rest / high) * BN;
+    const int all = static_cast<int>((p.k + kStep - 1) / kStep);
+    const int first = static_cast<int>(static_cast<int64_t>(all) * split / args.splits);
+    const int steps = static_cast<int>(static_cast<int64_t>(all) * (split + 1) / args.splits) - first;
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
+
+    // This wave's loads of a step: 16 rows of 64 bytes each, of a's rows then b's.
+    const int8_t* from[LOADS];
+    int at[LOADS];   // of the lane's piece: its first byte of k in a step
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j) {
+        const int row = (wave * LOADS + j) * 16 + (ln >> 2), c = (ln & 3) ^ ((row >> 2) & 3);
+        const bool inA = row < BM;
+        const int64_t r = inA ? min(row0 + row, p.m - 1) : min(col0 + row - BM, p.n - 1);
+        at[j] = c * 16;
+        from[j] = (inA ? p.a + r * p.lda : p.b + r * p.ldb) + static_cast<int64_t>(first) * kStep + c * 16;
+    }
+    const int64_t left0 = p.k - static_cast<int64_t>(first) * kStep;   // bytes of k from this range's first on
+    const bool partial = p.k % kStep != 0 && first + steps == all;
+    i32x4 held[LOADS];
+    // Load j of step t (past the last: the last again) into slot `slot`, or into
+    // registers.
+    auto issue = [&](int t, int slot, int j) {
+        const int s = min(t, steps - 1);
+        const int8_t* src = from[j] + static_cast<int64_t>(s) * kStep;
+        if constexpr (ALIGNED) {
+            if (partial && s == steps - 1 && left0 - static_cast<int64_t>(s) * kStep <= at[j]) src = reinterpret_cast<const int8_t*>(kZero16);
+            const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds0 + slot * kStage + (wave * LOADS + j) * 1024);
+            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0) : "memory");
+        } else if (partial && s == steps - 1) {
+            held[j] = piece(src, left0 - static_cast<int64_t>(s) * kStep - at[j]);
+        } else {
+            __builtin_memcpy(&held[j], src, 16);
+        }
+    };
+    auto put = [&](int slot) {
+        if constexpr (!ALIGNED) {
+#pragma unroll
+            for (int j = 0; j < LOADS; ++j) *reinterpret_cast<i32x4*>(lds + slot * kStage + (wave * LOADS + j) * 1024 + ln * 16) = held[j];
+        }
+    };
+    i32x4 acc[MT][NT] = {};
+    const uint32_t turn = (g ^ (l16 >> 2)) << 4;
+    const uint32_t atA = lds0 + (wm * MT * 16 + l16) * kStep + turn, atB = lds0 + (BM + wn * NT * 16 + l16) * kStep + turn;
+    const uint32_t atA2 = atA + 2 * kStage, atB2 = atB + 2 * kStage;   // an instruction's offset holds 16 bits
+    auto readA = [&](int slot, int i) {
+        return *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>((slot < 2 ? atA : atA2) + static_cast<uint32_t>((slot & 1) * kStage + i * 16 * kStep));
+    };
+    auto readB = [&](int slot, int i) {
+        return *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>((slot < 2 ? atB : atB2) + static_cast<uint32_t>((slot & 1) * kStage + i * 16 * kStep));
+    };
+    // Waits for all of this wave's loads but those of `later` steps.
+    auto landed = [&](auto later) {
+        if constexpr (ALIGNED) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(later() * LOADS) : "memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        asm volatile("s_barrier" ::: "memory");
+    };
+#pragma unroll
+    for (int t = 0; t < kStages - 1; ++t) {
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) issue(t, t, j);
+        if (t < kStages - 2) put(t);
+    }
+    landed([] { return kStages - 2; });
+    i32x4 aLo[HM], aHi[HM], bX[NT], bY[NT];
+#pragma unroll
+    for (int i = 0; i < HM; ++i) aLo[i] = readA(0, i);
+#pragma unroll
+    for (int i = 0; i < NT; ++i) bX[i] = readB(0, i);
+    // Step s in slot q.
+    auto step = [&](int s, const int q, i32x4 (&bCur)[NT], i32x4 (&bNext)[NT]) {
+        constexpr int N = HM * NT;
+        const int next = (q + 1) & 3;
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            const int i = x / NT, j = (i & 1) != 0 ? NT - 1 - x % NT : x % NT;
+            acc[i][j] = mfma(bCur[j], aLo[i], acc[i][j]);
+#pragma unroll
+            for (int r = 0; r < HM; ++r) {
+                if (r * N / (2 * HM) == x) aHi[r] = readA(q, HM + r);
+            }
+            if constexpr (ALIGNED) __builtin_amdgcn_sched_barrier(0);
+        }
+        put((q + 2) & 3);   // the loads of step s + 2, asked for a step ago
+        // Step s + 1 is in LDS; every wave is past step s - 1, whose slot is free.
+        landed([] { return 1; });
+        __builtin_amdgcn_sched_barrier(0);
+        constexpr int READS = NT + HM;   // B 0, A 0, the other Bs, the other As
+#pragma unroll
+        for (int x = 0; x < N; ++x) {
+            const int i = x / NT, j = (i & 1) != 0 ? NT - 1 - x % NT : x % NT;
+            acc[HM + i][j] = mfma(bCur[j], aHi[i], acc[HM + i][j]);
+#pragma unroll
+            for (int r = 0; r < READS; ++r) {
+                if (r * N / READS != x) continue;
+                if (r == 0) bNext[0] = readB(next, 0);
+                else if (r == 1) aLo[0] = readA(next, 0);
+                else if (r <= NT) bNext[r - 1] = readB(next, r - 1);
+                else aLo[r - NT] = readA(next, r - NT);
+            }
+#pragma unroll
+            for (int l = 0; l < LOADS; ++l) {
+                if ((2 * l + 1) * N / (2 * LOADS) == x) issue(s + kStages - 1, (q + 3) & 3, l);
+            }
+            if constexpr (ALIGNED) __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    int s = 0;
+    for (; s + 4 <= steps; s += 4) {
+        step(s, 0, bX, bY);
+        step(s + 1, 1, bY, bX);
+        step(s + 2, 2, bX, bY);
+        step(s + 3, 3, bY, bX);
+    }
+    if (s < steps) step(s, 0, bX, bY);
+    if (s + 1 < steps) step(s + 1, 1, bY, bX);
+    if (s + 2 < steps) step(s + 2, 2, bX, bY);
+    // No load may still be writing LDS when the workgroup ends.
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int64_t m = row0 + (wm * MT + i) * 16 + l16;
+        if (m >= p.m) continue;
+        const float sa = p.a_scale[m];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int64_t n = col0 + (wn * NT + j) * 16 + 4 * g;
+            if (n >= p.n) continue;
+            if (args.splits == 1) {
+                store4<T>(p, m, n, acc[i][j], sa, args.wide != 0);
+            } else {
+                int* to = args.work + (split * p.m + m) * p.n + n;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    if (n + e < p.n) to[e] = acc[i][j][e];
+                }
+            }
+        }
+    }
+}
+
+/// The ranges' sums added, scaled and stored.
+template <typename T>
+__global__ __launch_bounds__(256) void matmulI8Join(TileArgs args) {
+    const mlkd_matmul_i8& p = args.p;
     const int64_t total = p.m * p.n;
     for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t t = i / p.n, c = i % p.n;
-        const int8_t *a = p.a + t * p.lda, *b = p.b + c * p.ldb;
         int sum = 0;
-        for (int64_t k = 0; k < p.k; ++k) sum += static_cast<int>(a[k]) * b[k];
-        float v = static_cast<float>(sum) * p.a_scale[t] * p.b_scale[c];
-        if (p.bias != nullptr) v += p.bias[c];
-        static_cast<T*>(p.out)[t * p.ldo + c] = static_cast<T>(v);
+        for (int s = 0; s < args.splits; ++s) sum += args.work[s * total + i];
+        const int64_t m = i / p.n, n = i - m * p.n;
+        static_cast<T*>(p.out)[m * p.ldo + n] = scaled<T>(sum, p.a_scale[m], p.b_scale[n], p.bias != nullptr ? p.bias[n] : 0.0f, p.bias != nullptr);
     }
+}
+
+// --------------------------------------------------------------- launch ----
+enum Form { kFew, kTile64, kTile128, kTile256 };
+
+struct Plan {
+    Form form{kFew};
+    bool aligned{false}, wide{false};
+    int mb{1}, nb{1};      // kFew: 16 rows of a, of b, a workgroup
+    int64_t tilesM{0}, tilesN{0};
+    int splits{1};
+};
+
+int outBytes(const mlkd_matmul_i8* p) { return p->dtype == MLKD_F32 ? 4 : 2; }
+
+Plan planOf(const mlkd_matmul_i8* p) {
+    Plan n;
+    const int size = outBytes(p);
+    n.wide = p->ldo % 4 == 0 && reinterpret_cast<uintptr_t>(p->out) % (4 * size) == 0;
+    n.aligned = p->k % 16 == 0 && p->lda % 16 == 0 && p->ldb % 16 == 0 && reinterpret_cast<uintptr_t>(p->a) % 16 == 0 &&
+                reinterpret_cast<uintptr_t>(p->b) % 16 == 0;
+    if (p->m <= 64) {
+        n.mb = p->m <= 16 ? 1 : p->m <= 32 ? 2 : 4;
+        n.nb = n.mb == 4 && p->n >= 32 * 200 ? 2 : 1;
+        return n;
+    }
+    auto tiles = [&](int64_t of) {
+        n.tilesM = (p->m + of - 1) / of;
+        n.tilesN = (p->n + of - 1) / of;
+        return n.tilesM * n.tilesN;
+    };
+    n.form = n.aligned && tiles(256) >= 192 ? kTile256 : tiles(128) >= 192 ? kTile128 : kTile64;
+    const int64_t count = tiles(n.form == kTile256 ? 256 : n.form == kTile128 ? 128 : 64);
+    // Ranges of k of 1024 bytes and more where the tiles leave units idle.
+    n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / count, p->k / 1024, 32})));
+    return n;
+}
+
+Plan planFor(const mlkd_matmul_i8* p) {
+    Plan n = planOf(p);
+    if (n.splits > 1 && (p->work == nullptr || p->work_bytes < mlkd_matmul_i8_work_bytes(p))) n.splits = 1;
+    return n;
+}
+
+template <typename T, int MB>
+void launchFew(const mlkd_matmul_i8* p, const Plan& n, hipStream_t st) {
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>((p->n + 16 * n.nb - 1) / (16 * n.nb), int64_t{1} << 20));
+    auto* kernel = n.nb == 2 ? matmulI8Few<T, MB, 2> : matmulI8Few<T, MB, 1>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(512), 0, st, *p, n.wide ? 1 : 0);
+}
+
+template <typename T, int WM, int WN, int MT, int NT, bool ALIGNED>
+int launchTiles(const TileArgs& a, hipStream_t st) {
+    constexpr int bytes = (WM * MT + WN * NT) * 16 * kStep * kStages;
+    auto* kernel = matmulI8Tiles<T, WM, WN, MT, NT, ALIGNED>;
+    // Once per process; a function-local static initializes thread-safely.
+    static const bool allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                    bytes) == hipSuccess;
+    if (!allowed) return MLKD_RT_LAUNCH;
+    const int64_t grid = static_cast<int64_t>(a.tilesM) * a.tilesN * a.splits;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), bytes, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
+}
+
+template <typename T, bool ALIGNED>
+int launchForm(const TileArgs& a, Form form, hipStream_t st) {
+    if constexpr (ALIGNED) {
+        if (form == kTile256) return launchTiles<T, 2, 4, 8, 4, true>(a, st);
+    }
+    return form == kTile128 ? launchTiles<T, 2, 2, 4, 4, ALIGNED>(a, st) : launchTiles<T, 2, 2, 2, 2, ALIGNED>(a, st);
+}
+
+template <typename T>
+int launch(const mlkd_matmul_i8* p, hipStream_t st) {
+    const Plan n = planFor(p);
+    if (n.form == kFew) {
+        n.mb == 1 ? launchFew<T, 1>(p, n, st) : n.mb == 2 ? launchFew<T, 2>(p, n, st) : launchFew<T, 4>(p, n, st);
+        return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
+    }
+    TileArgs a{*p, static_cast<int>(n.tilesM), static_cast<int>(n.tilesN), n.splits, n.wide ? 1 : 0, static_cast<int*>(p->work)};
+    const int rc = n.aligned ? launchForm<T, true>(a, n.form, st) : launchForm<T, false>(a, n.form, st);
+    if (rc != 0 || n.splits == 1) return rc;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((p->m * p->n + 255) / 256, int64_t{1} << 16)));
+    hipLaunchKernelGGL(matmulI8Join<T>, grid, dim3(256), 0, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
 }
 
 const char* typeName(int dtype) { return dtype == MLKD_F32 ? "float" : dtype == MLKD_F16 ? "_Float16" : "__bf16"; }
@@ -31,20 +411,29 @@ const char* typeName(int dtype) { return dtype == MLKD_F32 ? "float" : dtype == 
 
 extern "C" {
 
-int64_t mlkd_matmul_i8_work_bytes(const mlkd_matmul_i8*) { return 0; }
+int64_t mlkd_matmul_i8_work_bytes(const mlkd_matmul_i8* p) {
+    const int splits = planOf(p).splits;
+    return splits > 1 ? splits * p->m * p->n * static_cast<int64_t>(sizeof(int)) : 0;
+}
 
 const char* mlkd_matmul_i8_kernel_names(const mlkd_matmul_i8* p) {
     static thread_local std::string name;
-    name = std::string("matmulI8Any<") + typeName(p->dtype) + ">";
+    const std::string type = typeName(p->dtype);
+    const Plan n = planFor(p);
+    if (n.form == kFew) {
+        name = "matmulI8Few<" + type + ", " + std::to_string(n.mb) + ", " + std::to_string(n.nb) + ">";
+        return name.c_str();
+    }
+    name = "matmulI8Tiles<" + type + (n.form == kTile256 ? ", 2, 4, 8, 4, " : n.form == kTile128 ? ", 2, 2, 4, 4, " : ", 2, 2, 2, 2, ") +
+           (n.aligned ? "true>" : "false>");
+    if (n.splits > 1) name += "+matmulI8Join<" + type + ">";
     return name.c_str();
 }
 
 int mlkd_launch_matmul_i8(const mlkd_matmul_i8* p, void* stream) {
     if (p->m == 0) return 0;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((p->m * p->n + 255) / 256, int64_t{1} << 20)));
-    auto* kernel = p->dtype == MLKD_F32 ? matmulI8Any<float> : p->dtype == MLKD_F16 ? matmulI8Any<_Float16> : matmulI8Any<__bf16>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), *p);
-    return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    return p->dtype == MLKD_F32 ? launch<float>(p, st) : p->dtype == MLKD_F16 ? launch<_Float16>(p, st) : launch<__bf16>(p, st);
 }
 
 }  // extern "C"

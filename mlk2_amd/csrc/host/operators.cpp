@@ -23,6 +23,7 @@ constexpr const char* kSlotNames[kOperandSlots] = {
 
 constexpr int64_t kMaxRows = INT32_MAX;   // rows are named by i32 buffers
 constexpr int kMaxDim = 256, kMaxHeads = 4096;
+constexpr int64_t kMaxProduct = int64_t{1} << 30;   // rows and columns of a product in 8 bits: their tiles' threads are counted in 32
 constexpr int64_t kMaxInner = (1 << 17) - 1;   // of a product in 8 bits: 2^14 a term, sums below 2^31
 
 int operandCode(Dtype d) {
@@ -335,7 +336,7 @@ bool quantizeRows(Reader& r, OperatorStep& o) {
 /// out [m, n] of a [m, inner] and b [n, inner].
 bool matmulI8(Reader& r, OperatorStep& o) {
     int64_t cols = 0, inner = 0;
-    if (!r.names({kOpA, kOpAScale, kOpB, kOpBScale, kOpBias, kOpOut}, {"cols", "inner"}) || !r.whole("cols", 0, 1, INT32_MAX, cols) ||
+    if (!r.names({kOpA, kOpAScale, kOpB, kOpBScale, kOpBias, kOpOut}, {"cols", "inner"}) || !r.whole("cols", 0, 1, kMaxProduct, cols) ||
         !r.whole("inner", 0, 1, kMaxInner, inner)) {
         return false;
     }
@@ -347,6 +348,7 @@ bool matmulI8(Reader& r, OperatorStep& o) {
     if (!r.heads(kOpOut, 1, cols, r.dtype(kOpOut), o.op[kOpOut])) return false;
     if (o.op[kOpB].rows != cols) return r.fail("'b' must have " + std::to_string(cols) + " rows");
     const int64_t rows = o.op[kOpA].rows;
+    if (rows > kMaxProduct) return r.fail("'a' has more than 2^30 rows");
     if (o.op[kOpOut].rows != rows) return r.fail("'a' and 'out' must have the same rows");
     if (!r.dense(kOpAScale, Dtype::F32, rows, "f32", o.op[kOpAScale]) || !r.dense(kOpBScale, Dtype::F32, cols, "f32", o.op[kOpBScale])) {
         return false;
