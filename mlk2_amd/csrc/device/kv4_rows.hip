@@ -16,7 +16,7 @@ using mlk::Scale;
 /// Tokens that there are: those below the end of the last sequence.
 __device__ __forceinline__ int64_t tokensOf(const mlkd_kv4_rows& p) {
     if (p.q_offsets == nullptr) return p.tokens;
-    return min(p.tokens, static_cast<int64_t>(p.q_offsets[p.sequences]));
+    return max(int64_t{0}, min(p.tokens, static_cast<int64_t>(p.q_offsets[p.sequences])));
 }
 
 /// A wave a head of k or v, with any dim, strides and alignment, two elements a
@@ -72,22 +72,94 @@ __global__ __launch_bounds__(256) void kv4RowsAny(mlkd_kv4_rows p) {
     }
 }
 
+/// Eight elements a lane, LANES lanes a head of up to 8 LANES elements, of any
+/// alignment: the heads of a token's k, then those of its v, side by side. A
+/// head is read once and written once. Bound by memory.
+template <typename T, int LANES, bool STORE>
+__global__ __launch_bounds__(256) void kv4Rows(mlkd_kv4_rows p) {
+    const int lane = threadIdx.x % LANES, c = lane * 8, bytes = p.dim / 2;
+    const uint32_t heads = p.kv_heads, all = static_cast<uint32_t>(tokensOf(p)) * 2 * heads;
+    // A wave's lanes take as many turns, as their exchange asks.
+    for (uint32_t n0 = (blockIdx.x * 256 + threadIdx.x / 64 * 64) / LANES; n0 < all; n0 += gridDim.x * 256 / LANES) {
+        const uint32_t n = min(n0 + threadIdx.x % 64 / LANES, all - 1), part = n / heads, h = n - part * heads, t = part >> 1;
+        const bool value = (part & 1) != 0;
+        const int64_t row = p.slots != nullptr ? p.slots[t] : static_cast<int64_t>(t);
+        const bool held = row >= 0 && row < p.cache_rows && c < p.dim;
+        T* x = static_cast<T*>(value ? p.v : p.k) + t * (value ? p.v_stride : p.k_stride) + static_cast<int64_t>(h) * p.dim + c;
+        uint8_t* codes = (value ? p.v_codes : p.k_codes) + row * (value ? p.v_codes_stride : p.k_codes_stride) + static_cast<int64_t>(h) * bytes + c / 2;
+        float* scale = (value ? p.v_scale : p.k_scale) + row * p.kv_heads + h;
+        if constexpr (STORE) {
+            float v[8] = {};
+            if (held) {
+                T raw[8];
+                __builtin_memcpy(raw, x, sizeof(raw));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = static_cast<float>(raw[e]);
+            }
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = max(top, mlk::magnitude(v[e]));
+#pragma unroll
+            for (int d = LANES / 2; d > 0; d >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d, 64)));
+            const Scale s = mlk::scaleOf(top, 6.0f);
+            uint32_t word = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) word |= mlk::codeFp4(v[e], s) << 4 * e;
+            if (top >= 0x7f800000u) word = 0;
+            if (held) {
+                __builtin_memcpy(codes, &word, 4);
+                if (lane == 0) *scale = s.stored;
+            }
+        } else if (held) {
+            const float s = *scale;
+            uint32_t word;
+            __builtin_memcpy(&word, codes, 4);
+            const mlk::F32x2 v[4] = {mlk::numbersOf<0>(word), mlk::numbersOf<1>(word), mlk::numbersOf<2>(word), mlk::numbersOf<3>(word)};
+            T out[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[e] = static_cast<T>(v[e / 2][e % 2] * s);
+            __builtin_memcpy(x, out, sizeof(out));
+        }
+    }
+}
+
+/// Whole lanes' elements, and heads that 32 bits count with a grid's more.
+bool rowsApply(const mlkd_kv4_rows* p) { return p->dim % 8 == 0 && p->tokens * p->kv_heads < (int64_t{1} << 30); }
+
+int lanesOf(const mlkd_kv4_rows* p) { return p->dim <= 32 ? 4 : p->dim <= 64 ? 8 : p->dim <= 128 ? 16 : 32; }
+
+template <typename T, bool STORE>
+void launchRows(const mlkd_kv4_rows* p, hipStream_t st) {
+    const int lanes = lanesOf(p);
+    const int64_t heads = p->tokens * p->kv_heads * 2, each = 256 / lanes;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((heads + each - 1) / each, int64_t{1} << 16)));
+    auto* kernel = lanes == 4 ? kv4Rows<T, 4, STORE> : lanes == 8 ? kv4Rows<T, 8, STORE> : lanes == 16 ? kv4Rows<T, 16, STORE> : kv4Rows<T, 32, STORE>;
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, *p);
+}
+
 const char* typeName(int dtype) { return dtype == MLKD_F32 ? "float" : dtype == MLKD_F16 ? "_Float16" : "__bf16"; }
 
 template <bool STORE>
 const char* kernelName(const mlkd_kv4_rows* p) {
     static thread_local std::string name;
-    name = std::string("kv4RowsAny<") + typeName(p->dtype) + (STORE ? ", true>" : ", false>");
+    name = rowsApply(p) ? std::string("kv4Rows<") + typeName(p->dtype) + ", " + std::to_string(lanesOf(p))
+                        : std::string("kv4RowsAny<") + typeName(p->dtype);
+    name += STORE ? ", true>" : ", false>";
     return name.c_str();
 }
 
 template <bool STORE>
 int launch(const mlkd_kv4_rows* p, void* stream) {
     if (p->tokens == 0) return 0;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (rowsApply(p)) {
+        p->dtype == MLKD_F32 ? launchRows<float, STORE>(p, st) : p->dtype == MLKD_F16 ? launchRows<_Float16, STORE>(p, st) : launchRows<__bf16, STORE>(p, st);
+        return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
+    }
     const int64_t heads = p->tokens * p->kv_heads * 2;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((heads + 3) / 4, int64_t{1} << 20)));
     auto* kernel = p->dtype == MLKD_F32 ? kv4RowsAny<float, STORE> : p->dtype == MLKD_F16 ? kv4RowsAny<_Float16, STORE> : kv4RowsAny<__bf16, STORE>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), *p);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, *p);
     return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
 }
 

@@ -45,8 +45,8 @@ __device__ __forceinline__ T scaled(int sum, float sa, float sb, float bias, boo
     return static_cast<T>(v);
 }
 
-/// Columns n .. n + 3 of row m from their sums. `wide`: four outputs at their
-/// own alignment at once.
+/// Columns n .. n + 3 of row m from their sums, n a multiple of 4. `wide`: rows
+/// of whole 16-byte pieces at 16 bytes.
 template <typename T>
 __device__ __forceinline__ void store4(const mlkd_matmul_i8& p, int64_t m, int64_t n, i32x4 sum, float sa, bool wide) {
     using V = T __attribute__((ext_vector_type(4)));
@@ -137,7 +137,8 @@ __global__ __launch_bounds__(512) void matmulI8Few(mlkd_matmul_i8 p, int wide) {
 struct TileArgs {
     mlkd_matmul_i8 p;
     int tilesM, tilesN, splits, wide;
-    int* work;   // [splits][m][n] sums of the ranges of k, or NULL
+    int* work;     // [splits][m][ldw] sums of the ranges of k, or NULL
+    int64_t ldw;   // n in whole fours
 };
 
 /// A tile of WM x WN waves of MT x NT products of 16 x 16 each, over steps of 64
@@ -283,40 +284,104 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
     if (s < steps) step(s, 0, bX, bY);
     if (s + 1 < steps) step(s + 1, 1, bY, bX);
     if (s + 2 < steps) step(s + 2, 2, bX, bY);
-    // No load may still be writing LDS when the workgroup ends.
+    // No load may still be writing LDS, and no wave be reading it, when its rows
+    // of results take its place.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    // By whole rows through LDS, each wave its own, 16 bytes a lane (four columns
+    // of 16 rows at a time, as the sums are held, took 15 us for 4096^2 f16 where
+    // this takes 9).
+    const int64_t m0 = row0 + wm * MT * 16, n0 = col0 + wn * NT * 16;
+    auto store = [&](auto zero, bool wide, auto value, auto rowAt) {
+        using O = decltype(zero);
+        using V4 = O __attribute__((ext_vector_type(4)));
+        constexpr int SIZE = sizeof(O), E = 16 / SIZE, PITCH = NT * 16 * SIZE, PIECES = PITCH / 16, PER = 64 / PIECES;
+        constexpr int CHUNK = MT * 16 * PITCH * NW <= kStage * kStages ? MT : MT / 2;   // 16 rows each
+        static_assert(CHUNK * 16 * PITCH * NW <= kStage * kStages && MT % CHUNK == 0, "the rows fit LDS");
+        char* const mine = lds + wave * (CHUNK * 16 * PITCH);
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        const int64_t m = row0 + (wm * MT + i) * 16 + l16;
-        if (m >= p.m) continue;
-        const float sa = p.a_scale[m];
+        for (int i0 = 0; i0 < MT; i0 += CHUNK) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int64_t n = col0 + (wn * NT + j) * 16 + 4 * g;
-            if (n >= p.n) continue;
-            if (args.splits == 1) {
-                store4<T>(p, m, n, acc[i][j], sa, args.wide != 0);
-            } else {
-                int* to = args.work + (split * p.m + m) * p.n + n;
+            for (int j = 0; j < NT; ++j) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    if (n + e < p.n) to[e] = acc[i][j][e];
+                for (int i = 0; i < CHUNK; ++i) {
+                    const int byte = (j * 16 + 4 * g) * SIZE;
+                    const V4 v = value(i0 + i, j, acc[i0 + i][j]);
+                    *reinterpret_cast<V4*>(mine + (i * 16 + l16) * PITCH + (((byte >> 4) ^ (l16 & (PIECES - 1))) << 4) + (byte & 15)) = v;
                 }
             }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+            for (int r = 0; r < CHUNK * 16 / PER; ++r) {
+                const int row = r * PER + ln / PIECES, c = ln % PIECES;
+                using V = O __attribute__((ext_vector_type(E)));
+                const V v = *reinterpret_cast<const V*>(mine + row * PITCH + ((c ^ (row & 15 & (PIECES - 1))) << 4));
+                const int64_t m = m0 + i0 * 16 + row, n = n0 + c * E;
+                if (m >= p.m) continue;
+                O* to = rowAt(m) + n;
+                if (wide && n + E <= p.n) {
+                    *reinterpret_cast<V*>(to) = v;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        if (n + e < p.n) to[e] = v[e];
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
+    };
+    if (args.splits > 1) {
+        store(0, true, [&](int, int, i32x4 sum) { return sum; }, [&](int64_t m) { return args.work + (split * p.m + m) * args.ldw; });
+        return;
+    }
+    using f32x4 = float __attribute__((ext_vector_type(4)));
+    float sa[MT];
+    f32x4 sb[NT], bias[NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) sa[i] = p.a_scale[min(m0 + i * 16 + l16, p.m - 1)];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int64_t n = min(n0 + j * 16 + 4 * g + e, p.n - 1);
+            sb[j][e] = p.b_scale[n];
+            bias[j][e] = p.bias != nullptr ? p.bias[n] : 0.0f;
+        }
+    }
+    store(static_cast<T>(0.0f), args.wide != 0, [&](int i, int j, i32x4 sum) {
+        T __attribute__((ext_vector_type(4))) v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = scaled<T>(sum[e], sa[i], sb[j][e], bias[j][e], p.bias != nullptr);
+        return v;
+    }, [&](int64_t m) { return static_cast<T*>(p.out) + m * p.ldo; });
+}
+
+/// Rows of k bytes copied to rows of whole steps at 16 bytes, with zeros behind
+/// them: a's, then b's. A thread a piece of 16 bytes.
+__global__ __launch_bounds__(256) void matmulI8Pack(mlkd_matmul_i8 p, int8_t* to, int64_t pitch) {
+    const int64_t pieces = pitch / 16, total = (p.m + p.n) * pieces;
+    for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t r = i / pieces, c = (i - r * pieces) * 16;
+        const int8_t* row = r < p.m ? p.a + r * p.lda : p.b + (r - p.m) * p.ldb;
+        *reinterpret_cast<i32x4*>(to + i * 16) = piece(row + c, p.k - c);
     }
 }
 
-/// The ranges' sums added, scaled and stored.
+/// The ranges' sums added, scaled and stored, four columns a thread.
 template <typename T>
 __global__ __launch_bounds__(256) void matmulI8Join(TileArgs args) {
     const mlkd_matmul_i8& p = args.p;
-    const int64_t total = p.m * p.n;
+    const int64_t quads = args.ldw / 4, total = p.m * quads;
     for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
-        int sum = 0;
-        for (int s = 0; s < args.splits; ++s) sum += args.work[s * total + i];
-        const int64_t m = i / p.n, n = i - m * p.n;
-        static_cast<T*>(p.out)[m * p.ldo + n] = scaled<T>(sum, p.a_scale[m], p.b_scale[n], p.bias != nullptr ? p.bias[n] : 0.0f, p.bias != nullptr);
+        i32x4 sum = {};
+        for (int s = 0; s < args.splits; ++s) sum += reinterpret_cast<const i32x4*>(args.work)[s * total + i];
+        const int64_t m = i / quads;
+        store4<T>(p, m, (i - m * quads) * 4, sum, p.a_scale[m], args.wide != 0);
     }
 }
 
@@ -325,7 +390,7 @@ enum Form { kFew, kTile64, kTile128, kTile256 };
 
 struct Plan {
     Form form{kFew};
-    bool aligned{false}, wide{false};
+    bool aligned{false}, wide{false}, pack{false};
     int mb{1}, nb{1};      // kFew: 16 rows of a, of b, a workgroup
     int64_t tilesM{0}, tilesN{0};
     int splits{1};
@@ -333,10 +398,18 @@ struct Plan {
 
 int outBytes(const mlkd_matmul_i8* p) { return p->dtype == MLKD_F32 ? 4 : 2; }
 
-Plan planOf(const mlkd_matmul_i8* p) {
+int64_t pitchOf(const mlkd_matmul_i8* p) { return (p->k + kStep - 1) / kStep * kStep; }
+/// The workspace: the copied rows, then the ranges' sums.
+int64_t packBytes(const mlkd_matmul_i8* p, const Plan& n) { return n.pack ? (p->m + p->n) * pitchOf(p) : 0; }
+int64_t sumBytes(const mlkd_matmul_i8* p, const Plan& n) {
+    return n.splits > 1 ? n.splits * p->m * ((p->n + 3) / 4 * 4) * static_cast<int64_t>(sizeof(int)) : 0;
+}
+
+/// `room`: with the workspace that it asks for.
+Plan planOf(const mlkd_matmul_i8* p, bool room) {
     Plan n;
     const int size = outBytes(p);
-    n.wide = p->ldo % 4 == 0 && reinterpret_cast<uintptr_t>(p->out) % (4 * size) == 0;
+    n.wide = p->ldo * size % 16 == 0 && reinterpret_cast<uintptr_t>(p->out) % 16 == 0;
     n.aligned = p->k % 16 == 0 && p->lda % 16 == 0 && p->ldb % 16 == 0 && reinterpret_cast<uintptr_t>(p->a) % 16 == 0 &&
                 reinterpret_cast<uintptr_t>(p->b) % 16 == 0;
     if (p->m <= 64) {
@@ -344,6 +417,10 @@ Plan planOf(const mlkd_matmul_i8* p) {
         n.nb = n.mb == 4 && p->n >= 32 * 200 ? 2 : 1;
         return n;
     }
+    // Rows off 16 bytes are copied first: reads of them take three times as long
+    // (333 x 1000 x 1501: 23 us, aligned 7), each tile's anew.
+    n.pack = !n.aligned && room;
+    n.aligned = n.aligned || n.pack;
     auto tiles = [&](int64_t of) {
         n.tilesM = (p->m + of - 1) / of;
         n.tilesN = (p->n + of - 1) / of;
@@ -352,14 +429,14 @@ Plan planOf(const mlkd_matmul_i8* p) {
     n.form = n.aligned && tiles(256) >= 192 ? kTile256 : tiles(128) >= 192 ? kTile128 : kTile64;
     const int64_t count = tiles(n.form == kTile256 ? 256 : n.form == kTile128 ? 128 : 64);
     // Ranges of k of 1024 bytes and more where the tiles leave units idle.
-    n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / count, p->k / 1024, 32})));
+    if (room) n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / count, p->k / 1024, 32})));
     return n;
 }
 
+/// The plan a launch has the workspace for.
 Plan planFor(const mlkd_matmul_i8* p) {
-    Plan n = planOf(p);
-    if (n.splits > 1 && (p->work == nullptr || p->work_bytes < mlkd_matmul_i8_work_bytes(p))) n.splits = 1;
-    return n;
+    const int64_t need = mlkd_matmul_i8_work_bytes(p);
+    return planOf(p, need == 0 || (p->work != nullptr && p->work_bytes >= need));
 }
 
 template <typename T, int MB>
@@ -385,7 +462,7 @@ int launchTiles(const TileArgs& a, hipStream_t st) {
 template <typename T, bool ALIGNED>
 int launchForm(const TileArgs& a, Form form, hipStream_t st) {
     if constexpr (ALIGNED) {
-        if (form == kTile256) return launchTiles<T, 2, 4, 8, 4, true>(a, st);
+        if (form == kTile256) return launchTiles<T, 4, 2, 4, 8, true>(a, st);
     }
     return form == kTile128 ? launchTiles<T, 2, 2, 4, 4, ALIGNED>(a, st) : launchTiles<T, 2, 2, 2, 2, ALIGNED>(a, st);
 }
@@ -397,10 +474,20 @@ int launch(const mlkd_matmul_i8* p, hipStream_t st) {
         n.mb == 1 ? launchFew<T, 1>(p, n, st) : n.mb == 2 ? launchFew<T, 2>(p, n, st) : launchFew<T, 4>(p, n, st);
         return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
     }
-    TileArgs a{*p, static_cast<int>(n.tilesM), static_cast<int>(n.tilesN), n.splits, n.wide ? 1 : 0, static_cast<int*>(p->work)};
+    TileArgs a{*p, static_cast<int>(n.tilesM), static_cast<int>(n.tilesN), n.splits, n.wide ? 1 : 0, nullptr, (p->n + 3) / 4 * 4};
+    if (n.splits > 1) a.work = reinterpret_cast<int*>(static_cast<char*>(p->work) + packBytes(p, n));
+    if (n.pack) {
+        int8_t* to = static_cast<int8_t*>(p->work);
+        const int64_t pitch = pitchOf(p), pieces = (p->m + p->n) * pitch / 16;
+        hipLaunchKernelGGL(matmulI8Pack, dim3(static_cast<unsigned>(std::min<int64_t>((pieces + 255) / 256, int64_t{1} << 16))), dim3(256), 0, st, *p, to, pitch);
+        if (hipGetLastError() != hipSuccess) return MLKD_RT_LAUNCH;
+        a.p.a = to;
+        a.p.b = to + p->m * pitch;
+        a.p.lda = a.p.ldb = a.p.k = pitch;
+    }
     const int rc = n.aligned ? launchForm<T, true>(a, n.form, st) : launchForm<T, false>(a, n.form, st);
     if (rc != 0 || n.splits == 1) return rc;
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((p->m * p->n + 255) / 256, int64_t{1} << 16)));
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((p->m * a.ldw / 4 + 255) / 256, int64_t{1} << 16)));
     hipLaunchKernelGGL(matmulI8Join<T>, grid, dim3(256), 0, st, a);
     return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
 }
@@ -412,8 +499,8 @@ const char* typeName(int dtype) { return dtype == MLKD_F32 ? "float" : dtype == 
 extern "C" {
 
 int64_t mlkd_matmul_i8_work_bytes(const mlkd_matmul_i8* p) {
-    const int splits = planOf(p).splits;
-    return splits > 1 ? splits * p->m * p->n * static_cast<int64_t>(sizeof(int)) : 0;
+    const Plan n = planOf(p, true);
+    return packBytes(p, n) + sumBytes(p, n);
 }
 
 const char* mlkd_matmul_i8_kernel_names(const mlkd_matmul_i8* p) {
@@ -424,7 +511,7 @@ const char* mlkd_matmul_i8_kernel_names(const mlkd_matmul_i8* p) {
         name = "matmulI8Few<" + type + ", " + std::to_string(n.mb) + ", " + std::to_string(n.nb) + ">";
         return name.c_str();
     }
-    name = "matmulI8Tiles<" + type + (n.form == kTile256 ? ", 2, 4, 8, 4, " : n.form == kTile128 ? ", 2, 2, 4, 4, " : ", 2, 2, 2, 2, ") +
+    name = std::string(n.pack ? "matmulI8Pack+" : "") + "matmulI8Tiles<" + type + (n.form == kTile256 ? ", 4, 2, 4, 8, " : n.form == kTile128 ? ", 2, 2, 4, 4, " : ", 2, 2, 2, 2, ") +
            (n.aligned ? "true>" : "false>");
     if (n.splits > 1) name += "+matmulI8Join<" + type + ">";
     return name.c_str();

@@ -207,7 +207,7 @@ def store_case(hip, t, g, d, dtype, cache=None, valid=None, x=None):
         old[f"{part}_codes"] = host[f"{part}_codes"] = rng.integers(0, 256, (rows, g, d // 2))
         old[f"{part}_scale"] = host[f"{part}_scale"] = np.full((rows, g), KEEP)
     got = run(hip, km, host)
-    n = t if valid is None else valid
+    n = t if valid is None else max(0, min(t, valid))
     for i, part in enumerate("kv"):
         codes, scale = store_kv4(x[i])
         want_codes, want_scale = old[f"{part}_codes"].copy(), old[f"{part}_scale"].copy()
@@ -244,7 +244,8 @@ def test_store_sizes(hip, dtype, t, g, d):
     store_case(hip, t, g, d, dtype, cache=t + 9)
 
 
-@pytest.mark.parametrize("kw", [dict(), dict(valid=17), dict(valid=0), dict(valid=9, cache=31), dict(valid=20, cache=20)])
+@pytest.mark.parametrize("kw", [dict(), dict(valid=17), dict(valid=0), dict(valid=9, cache=31), dict(valid=20, cache=20),
+                                dict(valid=-5), dict(valid=99, cache=30), dict(valid=-2 ** 31)])
 @pytest.mark.parametrize("d", [64, 36])
 def test_store_options(hip, kw, d):
     store_case(hip, 20, 2, d, "f16", **kw)
