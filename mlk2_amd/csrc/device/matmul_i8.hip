@@ -30,11 +30,46 @@ __device__ __forceinline__ i32x4 mfma(i32x4 b, i32x4 a, i32x4 c) { return __buil
 /// are zeros.
 __device__ __forceinline__ i32x4 piece(const int8_t* from, int64_t left) {
     i32x4 v = {};
-    if (left >= 16) {
-        __builtin_memcpy(&v, from, 16);
-    } else if (left > 0) {
-        for (int i = 0; i < left; ++i) v[i >> 2] |= static_cast<int>(static_cast<uint8_t>(from[i])) << (i & 3) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (left >= 4 * i + 4) {
+            int word;
+            __builtin_memcpy(&word, from + 4 * i, 4);
+            v[i] = word;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; ++e) {
+                if (left > 4 * i + e) v[i] |= static_cast<int>(static_cast<uint8_t>(from[4 * i + e])) << e * 8;
+            }
+        }
     }
+    return v;
+}
+
+/// 16 bytes of any alignment by whole words: reads off 4 bytes take three to five
+/// times as long (64 x 8000 x 4095: 55 us, 4092: 22). The five words around them, or
+/// the bytes as they are where a word reaches out of the operand, [lo, hi).
+struct Window {
+    i32x4 words;
+    int last;
+};
+__device__ __forceinline__ bool whole(const int8_t* from, const int8_t* lo, const int8_t* hi) {
+    const int8_t* base = from - (reinterpret_cast<uintptr_t>(from) & 3);
+    return base >= lo && base + 20 <= hi;
+}
+__device__ __forceinline__ Window ask(const int8_t* from, const int8_t* lo, const int8_t* hi) {
+    const bool in = whole(from, lo, hi);
+    const int8_t* base = in ? from - (reinterpret_cast<uintptr_t>(from) & 3) : from;
+    Window w;
+    __builtin_memcpy(&w.words, base, 16);
+    __builtin_memcpy(&w.last, base + (in ? 16 : 12), 4);
+    return w;
+}
+__device__ __forceinline__ i32x4 take(const Window& w, const int8_t* from, const int8_t* lo, const int8_t* hi) {
+    const int shift = whole(from, lo, hi) ? static_cast<int>(reinterpret_cast<uintptr_t>(from) & 3) : 0;
+    i32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __builtin_amdgcn_alignbyte(i < 3 ? w.words[i + 1] : w.last, w.words[i], shift);
     return v;
 }
 
@@ -66,27 +101,30 @@ __device__ __forceinline__ void store4(const mlkd_matmul_i8& p, int64_t m, int64
 }
 
 // ------------------------------------------------------------- few rows ----
-/// Up to 16 MB rows of a: eight waves take the 256-byte pieces of k in turn, 16
+/// Blocks of 16 MB rows of a: eight waves take the 256-byte pieces of k in turn, 16
 /// NB rows of b straight from memory, and their sums are added in LDS. A launch
 /// reads b once and nothing waits but on those reads.
-template <typename T, int MB, int NB>
+/// ALIGNED: rows at 4 bytes.
+template <typename T, int MB, int NB, bool ALIGNED>
 __global__ __launch_bounds__(512) void matmulI8Few(mlkd_matmul_i8 p, int wide) {
     constexpr int U = 4;   // steps of a piece
+    const int8_t *endA = p.a + (p.m - 1) * p.lda + p.k, *endB = p.b + (p.n - 1) * p.ldb + p.k;
     __shared__ i32x4 sums[8][MB * NB][64];
     const int ln = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
     const int l16 = ln & 15, g = ln >> 4;
     const int64_t blocks = (p.n + 16 * NB - 1) / (16 * NB);
     for (int64_t block = xcdShare(blockIdx.x, gridDim.x); block < blocks; block += gridDim.x) {
         const int64_t n0 = block * (16 * NB);
+        const int64_t rows = blockIdx.y * int64_t{16 * MB};
         const int8_t *a[MB], *b[NB];
 #pragma unroll
-        for (int i = 0; i < MB; ++i) a[i] = p.a + min(int64_t{i * 16 + l16}, p.m - 1) * p.lda + g * 16;
+        for (int i = 0; i < MB; ++i) a[i] = p.a + min(rows + i * 16 + l16, p.m - 1) * p.lda + g * 16;
 #pragma unroll
         for (int i = 0; i < NB; ++i) b[i] = p.b + min(n0 + i * 16 + l16, p.n - 1) * p.ldb + g * 16;
         i32x4 acc[MB][NB] = {};
         for (int64_t k = wave * (U * kStep); k < p.k; k += 8 * U * kStep) {
             i32x4 av[U][MB], bv[U][NB];
-            if (k + U * kStep <= p.k) {
+            if (k + U * kStep <= p.k && ALIGNED) {
 #pragma unroll
                 for (int u = 0; u < U; ++u) {
 #pragma unroll
@@ -96,6 +134,25 @@ __global__ __launch_bounds__(512) void matmulI8Few(mlkd_matmul_i8 p, int wide) {
                 for (int u = 0; u < U; ++u) {
 #pragma unroll
                     for (int i = 0; i < MB; ++i) __builtin_memcpy(&av[u][i], a[i] + k + u * kStep, 16);
+                }
+            } else if (k + U * kStep <= p.k) {
+                Window aw[U][MB], bw[U][NB];
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) bw[u][i] = ask(b[i] + k + u * kStep, p.b, endB);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                    for (int i = 0; i < MB; ++i) aw[u][i] = ask(a[i] + k + u * kStep, p.a, endA);
+                }
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+#pragma unroll
+                    for (int i = 0; i < NB; ++i) bv[u][i] = take(bw[u][i], b[i] + k + u * kStep, p.b, endB);
+#pragma unroll
+                    for (int i = 0; i < MB; ++i) av[u][i] = take(aw[u][i], a[i] + k + u * kStep, p.a, endA);
                 }
             } else {
 #pragma unroll
@@ -126,7 +183,7 @@ __global__ __launch_bounds__(512) void matmulI8Few(mlkd_matmul_i8 p, int wide) {
             i32x4 sum = sums[0][t][ln];
 #pragma unroll
             for (int w = 1; w < 8; ++w) sum += sums[w][t][ln];
-            const int64_t m = t / NB * 16 + l16, n = n0 + t % NB * 16 + 4 * g;
+            const int64_t m = rows + t / NB * 16 + l16, n = n0 + t % NB * 16 + 4 * g;
             if (m < p.m && n < p.n) store4<T>(p, m, n, sum, p.a_scale[m], wide != 0);
         }
         __syncthreads();
@@ -144,10 +201,8 @@ struct TileArgs {
 /// A tile of WM x WN waves of MT x NT products of 16 x 16 each, over steps of 64
 /// bytes of k through a ring of four in LDS.
 ///
-/// ALIGNED (rows of a and b in whole 16-byte pieces at 16 bytes): the rows go
-/// straight to LDS, three steps ahead. Otherwise through registers, asked for
-/// three steps ahead and written to LDS a step later. Rows past the last repeat
-/// it, pieces past k are zeros.
+/// Rows of a and b, whole 16-byte pieces at 16 bytes, go straight to LDS, three
+/// steps ahead. Rows past the last repeat it, pieces past k are zeros.
 ///
 /// LDS holds 64-byte rows, piece c of row r at c ^ (r / 4 % 4): a fragment's
 /// read takes one piece of 16 rows at a time, which then lie in all banks. In
@@ -155,7 +210,7 @@ struct TileArgs {
 /// rows of a are read; while the second runs, the next step's fragments are read
 /// and the loads of the step three ahead are asked for, in a fixed order, a memory
 /// instruction behind every other product or so.
-template <typename T, int WM, int WN, int MT, int NT, bool ALIGNED>
+template <typename T, int WM, int WN, int MT, int NT>
 __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) {
     constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
     constexpr int kStage = (BM + BN) * kStep, LOADS = (BM + BN) / 16 / NW, HM = MT / 2;
@@ -174,38 +229,31 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(lds));
 
     // This wave's loads of a step: 16 rows of 64 bytes each, of a's rows then b's.
-    const int8_t* from[LOADS];
-    int at[LOADS];   // of the lane's piece: its first byte of k in a step
+    // A lane's piece lies `off` past its tile's first row.
+    const int8_t* const tileA = p.a + row0 * p.lda + static_cast<int64_t>(first) * kStep;
+    const int8_t* const tileB = p.b + col0 * p.ldb + static_cast<int64_t>(first) * kStep;
+    uint32_t off[LOADS];
+    const int at = ((ln & 3) ^ (ln >> 4)) * 16;   // the piece's first byte of k in a step
 #pragma unroll
     for (int j = 0; j < LOADS; ++j) {
-        const int row = (wave * LOADS + j) * 16 + (ln >> 2), c = (ln & 3) ^ ((row >> 2) & 3);
-        const bool inA = row < BM;
-        const int64_t r = inA ? min(row0 + row, p.m - 1) : min(col0 + row - BM, p.n - 1);
-        at[j] = c * 16;
-        from[j] = (inA ? p.a + r * p.lda : p.b + r * p.ldb) + static_cast<int64_t>(first) * kStep + c * 16;
+        const int row = (wave * LOADS + j) * 16 + (ln >> 2);
+        const int64_t r = row < BM ? min(row0 + row, p.m - 1) - row0 : min(col0 + row - BM, p.n - 1) - col0;
+        off[j] = static_cast<uint32_t>(r * (row < BM ? p.lda : p.ldb)) + at;
     }
-    const int64_t left0 = p.k - static_cast<int64_t>(first) * kStep;   // bytes of k from this range's first on
-    const bool partial = p.k % kStep != 0 && first + steps == all;
-    i32x4 held[LOADS];
-    // Load j of step t (past the last: the last again) into slot `slot`, or into
-    // registers.
-    auto issue = [&](int t, int slot, int j) {
-        const int s = min(t, steps - 1);
-        const int8_t* src = from[j] + static_cast<int64_t>(s) * kStep;
-        if constexpr (ALIGNED) {
-            if (partial && s == steps - 1 && left0 - static_cast<int64_t>(s) * kStep <= at[j]) src = reinterpret_cast<const int8_t*>(kZero16);
-            const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds0 + slot * kStage + (wave * LOADS + j) * 1024);
-            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(m0) : "memory");
-        } else if (partial && s == steps - 1) {
-            held[j] = piece(src, left0 - static_cast<int64_t>(s) * kStep - at[j]);
+    const int tail = static_cast<int>(p.k % kStep);   // bytes of the last step, or 0: all
+    const bool partial = tail != 0 && first + steps == all;
+    constexpr auto yes = [] { return true; };
+    constexpr auto no = [] { return false; };
+    // Load j of step t (past the last: the last again) into slot `slot`. `ends`:
+    // that step may be the last.
+    auto issue = [&](int t, int slot, int j, auto ends) __attribute__((always_inline)) {
+        const int8_t* src = ((wave * LOADS + j) * 16 < BM ? tileA : tileB) + static_cast<int64_t>(ends() ? min(t, steps - 1) : t) * kStep;
+        const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds0 + slot * kStage + (wave * LOADS + j) * 1024);
+        if (ends() && partial && t >= steps - 1) {
+            const int8_t* from = at < tail ? src + off[j] : reinterpret_cast<const int8_t*>(kZero16);
+            asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(from), "s"(m0) : "memory");
         } else {
-            __builtin_memcpy(&held[j], src, 16);
-        }
-    };
-    auto put = [&](int slot) {
-        if constexpr (!ALIGNED) {
-#pragma unroll
-            for (int j = 0; j < LOADS; ++j) *reinterpret_cast<i32x4*>(lds + slot * kStage + (wave * LOADS + j) * 1024 + ln * 16) = held[j];
+            asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off[j]), "s"(src), "s"(m0) : "memory");
         }
     };
     i32x4 acc[MT][NT] = {};
@@ -220,15 +268,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
     };
     // Waits for all of this wave's loads but those of `later` steps.
     auto landed = [&](auto later) {
-        if constexpr (ALIGNED) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(later() * LOADS) : "memory");
-        else asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(later() * LOADS) : "memory");
         asm volatile("s_barrier" ::: "memory");
     };
 #pragma unroll
     for (int t = 0; t < kStages - 1; ++t) {
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) issue(t, t, j);
-        if (t < kStages - 2) put(t);
+        for (int j = 0; j < LOADS; ++j) issue(t, t, j, yes);
     }
     landed([] { return kStages - 2; });
     i32x4 aLo[HM], aHi[HM], bX[NT], bY[NT];
@@ -237,7 +283,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
 #pragma unroll
     for (int i = 0; i < NT; ++i) bX[i] = readB(0, i);
     // Step s in slot q.
-    auto step = [&](int s, const int q, i32x4 (&bCur)[NT], i32x4 (&bNext)[NT]) {
+    auto step = [&](int s, const int q, i32x4 (&bCur)[NT], i32x4 (&bNext)[NT], auto ends) __attribute__((always_inline)) {
         constexpr int N = HM * NT;
         const int next = (q + 1) & 3;
 #pragma unroll
@@ -248,9 +294,8 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
             for (int r = 0; r < HM; ++r) {
                 if (r * N / (2 * HM) == x) aHi[r] = readA(q, HM + r);
             }
-            if constexpr (ALIGNED) __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        put((q + 2) & 3);   // the loads of step s + 2, asked for a step ago
         // Step s + 1 is in LDS; every wave is past step s - 1, whose slot is free.
         landed([] { return 1; });
         __builtin_amdgcn_sched_barrier(0);
@@ -269,21 +314,24 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
             }
 #pragma unroll
             for (int l = 0; l < LOADS; ++l) {
-                if ((2 * l + 1) * N / (2 * LOADS) == x) issue(s + kStages - 1, (q + 3) & 3, l);
+                if ((2 * l + 1) * N / (2 * LOADS) == x) issue(s + kStages - 1, (q + 3) & 3, l, ends);
             }
-            if constexpr (ALIGNED) __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     int s = 0;
-    for (; s + 4 <= steps; s += 4) {
-        step(s, 0, bX, bY);
-        step(s + 1, 1, bY, bX);
-        step(s + 2, 2, bX, bY);
-        step(s + 3, 3, bY, bX);
-    }
-    if (s < steps) step(s, 0, bX, bY);
-    if (s + 1 < steps) step(s + 1, 1, bY, bX);
-    if (s + 2 < steps) step(s + 2, 2, bX, bY);
+    auto four = [&](auto ends) __attribute__((always_inline)) {
+        step(s, 0, bX, bY, ends);
+        step(s + 1, 1, bY, bX, ends);
+        step(s + 2, 2, bX, bY, ends);
+        step(s + 3, 3, bY, bX, ends);
+        s += 4;
+    };
+    while (s + 3 + kStages - 1 < steps - 1) four(no);
+    while (s + 4 <= steps) four(yes);
+    if (s < steps) step(s, 0, bX, bY, yes);
+    if (s + 1 < steps) step(s + 1, 1, bY, bX, yes);
+    if (s + 2 < steps) step(s + 2, 2, bX, bY, yes);
     // No load may still be writing LDS, and no wave be reading it, when its rows
     // of results take its place.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -292,7 +340,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
     // of 16 rows at a time, as the sums are held, took 15 us for 4096^2 f16 where
     // this takes 9).
     const int64_t m0 = row0 + wm * MT * 16, n0 = col0 + wn * NT * 16;
-    auto store = [&](auto zero, bool wide, auto value, auto rowAt) {
+    auto store = [&](auto zero, bool wide, auto value, auto rowAt) __attribute__((always_inline)) {
         using O = decltype(zero);
         using V4 = O __attribute__((ext_vector_type(4)));
         constexpr int SIZE = sizeof(O), E = 16 / SIZE, PITCH = NT * 16 * SIZE, PIECES = PITCH / 16, PER = 64 / PIECES;
@@ -339,36 +387,30 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
         store(0, true, [&](int, int, i32x4 sum) { return sum; }, [&](int64_t m) { return args.work + (split * p.m + m) * args.ldw; });
         return;
     }
-    using f32x4 = float __attribute__((ext_vector_type(4)));
     float sa[MT];
-    f32x4 sb[NT], bias[NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) sa[i] = p.a_scale[min(m0 + i * 16 + l16, p.m - 1)];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int64_t n = min(n0 + j * 16 + 4 * g + e, p.n - 1);
-            sb[j][e] = p.b_scale[n];
-            bias[j][e] = p.bias != nullptr ? p.bias[n] : 0.0f;
-        }
-    }
     store(static_cast<T>(0.0f), args.wide != 0, [&](int i, int j, i32x4 sum) {
         T __attribute__((ext_vector_type(4))) v;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = scaled<T>(sum[e], sa[i], sb[j][e], bias[j][e], p.bias != nullptr);
+        for (int e = 0; e < 4; ++e) {
+            const int64_t n = min(n0 + j * 16 + 4 * g + e, p.n - 1);
+            v[e] = scaled<T>(sum[e], sa[i], p.b_scale[n], p.bias != nullptr ? p.bias[n] : 0.0f, p.bias != nullptr);
+        }
         return v;
     }, [&](int64_t m) { return static_cast<T*>(p.out) + m * p.ldo; });
 }
 
-/// Rows of k bytes copied to rows of whole steps at 16 bytes, with zeros behind
-/// them: a's, then b's. A thread a piece of 16 bytes.
+/// Rows of k bytes copied to rows of `pitch` bytes at 16, zeros behind them: a's,
+/// then b's. A thread a piece of 16 bytes.
 __global__ __launch_bounds__(256) void matmulI8Pack(mlkd_matmul_i8 p, int8_t* to, int64_t pitch) {
+    const int8_t *endA = p.a + (p.m - 1) * p.lda + p.k, *endB = p.b + (p.n - 1) * p.ldb + p.k;
     const int64_t pieces = pitch / 16, total = (p.m + p.n) * pieces;
     for (int64_t i = blockIdx.x * int64_t{256} + threadIdx.x; i < total; i += static_cast<int64_t>(gridDim.x) * 256) {
         const int64_t r = i / pieces, c = (i - r * pieces) * 16;
-        const int8_t* row = r < p.m ? p.a + r * p.lda : p.b + (r - p.m) * p.ldb;
-        *reinterpret_cast<i32x4*>(to + i * 16) = piece(row + c, p.k - c);
+        const bool inA = r < p.m;
+        const int8_t *from = (inA ? p.a + r * p.lda : p.b + (r - p.m) * p.ldb) + c, *lo = inA ? p.a : p.b, *hi = inA ? endA : endB;
+        *reinterpret_cast<i32x4*>(to + i * 16) = p.k - c >= 16 ? take(ask(from, lo, hi), from, lo, hi) : piece(from, p.k - c);
     }
 }
 
@@ -398,7 +440,14 @@ struct Plan {
 
 int outBytes(const mlkd_matmul_i8* p) { return p->dtype == MLKD_F32 ? 4 : 2; }
 
+/// Rows of whole pieces of so many bytes.
+bool rowsAt(const mlkd_matmul_i8* p, int bytes) {
+    return p->lda % bytes == 0 && p->ldb % bytes == 0 && reinterpret_cast<uintptr_t>(p->a) % bytes == 0 &&
+           reinterpret_cast<uintptr_t>(p->b) % bytes == 0;
+}
+
 int64_t pitchOf(const mlkd_matmul_i8* p) { return (p->k + kStep - 1) / kStep * kStep; }
+
 /// The workspace: the copied rows, then the ranges' sums.
 int64_t packBytes(const mlkd_matmul_i8* p, const Plan& n) { return n.pack ? (p->m + p->n) * pitchOf(p) : 0; }
 int64_t sumBytes(const mlkd_matmul_i8* p, const Plan& n) {
@@ -410,23 +459,22 @@ Plan planOf(const mlkd_matmul_i8* p, bool room) {
     Plan n;
     const int size = outBytes(p);
     n.wide = p->ldo * size % 16 == 0 && reinterpret_cast<uintptr_t>(p->out) % 16 == 0;
-    n.aligned = p->k % 16 == 0 && p->lda % 16 == 0 && p->ldb % 16 == 0 && reinterpret_cast<uintptr_t>(p->a) % 16 == 0 &&
-                reinterpret_cast<uintptr_t>(p->b) % 16 == 0;
-    if (p->m <= 64) {
+    // A tile's rows lie 2^32 bytes apart at most.
+    n.aligned = p->k % 16 == 0 && rowsAt(p, 16) && std::max(p->lda, p->ldb) < (int64_t{1} << 23);
+    // The tiles take rows at 16 bytes: others are copied to such first.
+    n.pack = !n.aligned && p->m > 64 && room;
+    if (p->m <= 64 || !(n.aligned || n.pack)) {
         n.mb = p->m <= 16 ? 1 : p->m <= 32 ? 2 : 4;
+        n.aligned = rowsAt(p, 4);
         n.nb = n.mb == 4 && p->n >= 32 * 200 ? 2 : 1;
         return n;
     }
-    // Rows off 16 bytes are copied first: reads of them take three times as long
-    // (333 x 1000 x 1501: 23 us, aligned 7), each tile's anew.
-    n.pack = !n.aligned && room;
-    n.aligned = n.aligned || n.pack;
     auto tiles = [&](int64_t of) {
         n.tilesM = (p->m + of - 1) / of;
         n.tilesN = (p->n + of - 1) / of;
         return n.tilesM * n.tilesN;
     };
-    n.form = n.aligned && tiles(256) >= 192 ? kTile256 : tiles(128) >= 192 ? kTile128 : kTile64;
+    n.form = tiles(256) >= 192 ? kTile256 : tiles(128) >= 192 ? kTile128 : kTile64;
     const int64_t count = tiles(n.form == kTile256 ? 256 : n.form == kTile128 ? 128 : 64);
     // Ranges of k of 1024 bytes and more where the tiles leave units idle.
     if (room) n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / count, p->k / 1024, 32})));
@@ -442,14 +490,23 @@ Plan planFor(const mlkd_matmul_i8* p) {
 template <typename T, int MB>
 void launchFew(const mlkd_matmul_i8* p, const Plan& n, hipStream_t st) {
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>((p->n + 16 * n.nb - 1) / (16 * n.nb), int64_t{1} << 20));
-    auto* kernel = n.nb == 2 ? matmulI8Few<T, MB, 2> : matmulI8Few<T, MB, 1>;
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(512), 0, st, *p, n.wide ? 1 : 0);
+    auto* kernel = n.aligned ? (n.nb == 2 ? matmulI8Few<T, MB, 2, true> : matmulI8Few<T, MB, 1, true>)
+                             : (n.nb == 2 ? matmulI8Few<T, MB, 2, false> : matmulI8Few<T, MB, 1, false>);
+    constexpr int64_t kRows = (int64_t{16} * MB) << 15;   // a launch's: blocks of them along y
+    for (int64_t r = 0; r < p->m; r += kRows) {
+        mlkd_matmul_i8 part = *p;
+        part.a += r * p->lda;
+        part.a_scale += r;
+        part.out = static_cast<T*>(p->out) + r * p->ldo;
+        part.m = std::min(kRows, p->m - r);
+        hipLaunchKernelGGL(kernel, dim3(grid, static_cast<unsigned>((part.m + 16 * MB - 1) / (16 * MB))), dim3(512), 0, st, part, n.wide ? 1 : 0);
+    }
 }
 
-template <typename T, int WM, int WN, int MT, int NT, bool ALIGNED>
+template <typename T, int WM, int WN, int MT, int NT>
 int launchTiles(const TileArgs& a, hipStream_t st) {
     constexpr int bytes = (WM * MT + WN * NT) * 16 * kStep * kStages;
-    auto* kernel = matmulI8Tiles<T, WM, WN, MT, NT, ALIGNED>;
+    auto* kernel = matmulI8Tiles<T, WM, WN, MT, NT>;
     // Once per process; a function-local static initializes thread-safely.
     static const bool allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                     bytes) == hipSuccess;
@@ -457,14 +514,6 @@ int launchTiles(const TileArgs& a, hipStream_t st) {
     const int64_t grid = static_cast<int64_t>(a.tilesM) * a.tilesN * a.splits;
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(WM * WN * 64), bytes, st, a);
     return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
-}
-
-template <typename T, bool ALIGNED>
-int launchForm(const TileArgs& a, Form form, hipStream_t st) {
-    if constexpr (ALIGNED) {
-        if (form == kTile256) return launchTiles<T, 4, 2, 4, 8, true>(a, st);
-    }
-    return form == kTile128 ? launchTiles<T, 2, 2, 4, 4, ALIGNED>(a, st) : launchTiles<T, 2, 2, 2, 2, ALIGNED>(a, st);
 }
 
 template <typename T>
@@ -485,7 +534,9 @@ int launch(const mlkd_matmul_i8* p, hipStream_t st) {
         a.p.b = to + p->m * pitch;
         a.p.lda = a.p.ldb = a.p.k = pitch;
     }
-    const int rc = n.aligned ? launchForm<T, true>(a, n.form, st) : launchForm<T, false>(a, n.form, st);
+    const int rc = n.form == kTile256   ? launchTiles<T, 4, 2, 4, 8>(a, st)
+                   : n.form == kTile128 ? launchTiles<T, 2, 2, 4, 4>(a, st)
+                                        : launchTiles<T, 2, 2, 2, 2>(a, st);
     if (rc != 0 || n.splits == 1) return rc;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((p->m * a.ldw / 4 + 255) / 256, int64_t{1} << 16)));
     hipLaunchKernelGGL(matmulI8Join<T>, grid, dim3(256), 0, st, a);
@@ -508,11 +559,11 @@ const char* mlkd_matmul_i8_kernel_names(const mlkd_matmul_i8* p) {
     const std::string type = typeName(p->dtype);
     const Plan n = planFor(p);
     if (n.form == kFew) {
-        name = "matmulI8Few<" + type + ", " + std::to_string(n.mb) + ", " + std::to_string(n.nb) + ">";
+        name = "matmulI8Few<" + type + ", " + std::to_string(n.mb) + ", " + std::to_string(n.nb) + (n.aligned ? ", true>" : ", false>");
         return name.c_str();
     }
-    name = std::string(n.pack ? "matmulI8Pack+" : "") + "matmulI8Tiles<" + type + (n.form == kTile256 ? ", 4, 2, 4, 8, " : n.form == kTile128 ? ", 2, 2, 4, 4, " : ", 2, 2, 2, 2, ") +
-           (n.aligned ? "true>" : "false>");
+    name = std::string(n.pack ? "matmulI8Pack+" : "") + "matmulI8Tiles<" + type +
+           (n.form == kTile256 ? ", 4, 2, 4, 8>" : n.form == kTile128 ? ", 2, 2, 4, 4>" : ", 2, 2, 2, 2>");
     if (n.splits > 1) name += "+matmulI8Join<" + type + ">";
     return name.c_str();
 }
