@@ -6,7 +6,8 @@
 #include <algorithm>
 #include <string>
 
-#include "attention_span.h"
+#include "attention_kv4_tiles.h"
+#include "attention_rows.h"
 #include "bits.h"
 #include "runtime_abi.h"
 
@@ -14,35 +15,6 @@ namespace {
 
 using mlk::SeqSpan;
 using mlk::spanOf;
-
-constexpr float kLn2 = 0.6931471805599453f;
-
-__device__ __forceinline__ float waveMax(float v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d, 64));
-    return v;
-}
-
-__device__ __forceinline__ float waveSum(float v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) v += __shfl_xor(v, d, 64);
-    return v;
-}
-
-__device__ __forceinline__ float lane(float v, int i) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i));
-}
-
-/// The sequence that holds query row t, or -1.
-__device__ __forceinline__ int sequenceOf(const mlkd_attention& p, int64_t t) {
-    int lo = 0, hi = p.sequences;
-    while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (p.q_offsets[mid] <= t) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo > 0 && t < p.q_offsets[lo] ? lo - 1 : -1;
-}
 
 /// A query row in one wave, with any even dim, strides and alignment: a lane per
 /// key for the scores, then a lane per output column.
@@ -111,26 +83,140 @@ __global__ __launch_bounds__(256) void attentionKv4Rows(mlkd_attention_kv4 args)
     }
 }
 
+/// How a launch runs: on the matrix cores or row by row, waves to a row block,
+/// key ranges.
+struct Plan {
+    bool tiles{false};
+    int waves{1}, splits{1};
+    int parts() const { return splits > 1 ? splits : 0; }
+};
+
+/// The matrix-core kernels take rows of whole 16-byte pieces, and codes of whole
+/// eights of heads that are multiples of 16.
+bool tilesApply(const mlkd_attention* p) {
+    const int size = p->dtype == MLKD_F32 ? 4 : 2;
+    // As attention's: a block reads the lengths 64 at a time, rows and keys are
+    // counted in 32 bits.
+    return p->dim % 16 == 0 && p->sequences <= 4096 && p->q_rows * (p->heads / p->kv_heads) < (int64_t{1} << 30) &&
+           p->kv_rows <= (int64_t{1} << 30) && aligned(p->q, p->q_stride, 16, size) && aligned(p->out, p->out_stride, 16, size) &&
+           aligned(p->k, p->k_stride, 16, 1) && aligned(p->v, p->v_stride, 16, 1);
+}
+
+int dimOf(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
+
+/// Row blocks of a launch: at most so many for any lengths.
+int64_t rowBlocks(const mlkd_attention* p) {
+    const int64_t rows = p->q_rows * (p->heads / p->kv_heads);
+    return rows / 32 + std::min<int64_t>(p->sequences, rows);
+}
+
+Plan planOf(const mlkd_attention* p) {
+    Plan n;
+    n.tiles = tilesApply(p);
+    if (!n.tiles) return n;
+    const int64_t group = p->heads / p->kv_heads, each = (p->q_rows + p->sequences - 1) / p->sequences * group;   // rows of a sequence, on average
+    const int64_t count = p->sequences * ((each + 31) / 32) * p->kv_heads, keys = std::max<int64_t>(1, p->kv_rows / p->sequences);
+    n.waves = count >= 2048 ? 1 : 4;
+    if (n.waves == 4) n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({1024 / count, keys / 256, 64})));
+    return n;
+}
+
+/// The plan a launch has the workspace for.
+Plan planFor(const mlkd_attention_kv4* p) {
+    Plan n = planOf(&p->a);
+    if (n.parts() > 0 && (p->a.work == nullptr || p->a.work_bytes < mlkd_attention_kv4_work_bytes(p))) n.splits = 1;
+    return n;
+}
+
+template <typename T, int DT, int NW>
+int launchTiles(mlk::Kv4Args a, hipStream_t st) {
+    constexpr int bytes = mlk::Kv4Tiles<T, DT, NW>::kLds;
+    auto* kernel = mlk::attentionKv4Tiles<T, DT, NW>;
+    // Once per process; a function-local static initializes thread-safely.
+    static const bool allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                    bytes) == hipSuccess;
+    if (!allowed) return MLKD_RT_LAUNCH;
+    const int64_t grid = (static_cast<int64_t>(a.units) + 7) / 8 * 8 * a.t.p.kv_heads;
+    if (grid * NW * 64 >= (int64_t{1} << 32)) return -1;
+    hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(grid)), dim3(NW * 64), bytes, st, a);
+    return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
+}
+
+template <typename T, int DT>
+int launchWaves(const mlk::Kv4Args& a, int waves, hipStream_t st) {
+    return waves == 1 ? launchTiles<T, DT, 1>(a, st) : launchTiles<T, DT, 4>(a, st);
+}
+
+template <typename T>
+int launchPlan(const mlkd_attention_kv4* p, const Plan& n, hipStream_t st) {
+    mlk::Kv4Args a{};
+    a.t.p = p->a;
+    a.k_scale = p->k_scale;
+    a.v_scale = p->v_scale;
+    a.t.splits = n.splits;
+    a.t.parts = n.parts();
+    if (a.t.parts > 0) {
+        a.t.acc = static_cast<float*>(p->a.work);
+        a.t.ml = reinterpret_cast<float2*>(a.t.acc + a.t.parts * p->a.q_rows * p->a.heads * p->a.dim);
+    }
+    a.t.by_group = dividerOf(p->a.heads / p->a.kv_heads);
+    a.t.by_kv_heads = dividerOf(p->a.kv_heads);
+    a.t.by_splits = dividerOf(n.splits);
+    a.t.by_heads = dividerOf(p->a.heads);
+    const int64_t units = rowBlocks(&p->a) * n.splits;
+    if (units >= (int64_t{1} << 30)) return -1;
+    a.units = static_cast<int>(units);
+    int rc = 0;
+    switch (dimOf(p->a.dim)) {
+        case 64: rc = launchWaves<T, 64>(a, n.waves, st); break;
+        case 96: rc = launchWaves<T, 96>(a, n.waves, st); break;
+        case 128: rc = launchWaves<T, 128>(a, n.waves, st); break;
+        default: rc = launchWaves<T, 256>(a, n.waves, st); break;
+    }
+    if (rc != 0 || a.t.parts == 0) return rc;
+    const int64_t rows = p->a.q_rows * p->a.heads;
+    auto* join = p->a.dim <= 64 ? attentionJoin<T, 16> : p->a.dim <= 128 ? attentionJoin<T, 32> : attentionJoin<T, 64>;
+    hipLaunchKernelGGL(join, dim3(static_cast<unsigned>(std::min<int64_t>((rows + 3) / 4, int64_t{1} << 20))), dim3(256), 0, st, a.t);
+    return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
+}
+
 const char* typeName(int dtype) { return dtype == MLKD_F32 ? "float" : dtype == MLKD_F16 ? "_Float16" : "__bf16"; }
 
 }  // namespace
 
 extern "C" {
 
-int64_t mlkd_attention_kv4_work_bytes(const mlkd_attention_kv4*) { return 0; }
+int64_t mlkd_attention_kv4_work_bytes(const mlkd_attention_kv4* p) {
+    return planOf(&p->a).parts() * p->a.q_rows * p->a.heads * (p->a.dim * static_cast<int64_t>(sizeof(float)) + static_cast<int64_t>(sizeof(float2)));
+}
 
 const char* mlkd_attention_kv4_kernel_names(const mlkd_attention_kv4* p) {
     static thread_local std::string name;
-    name = std::string("attentionKv4Rows<") + typeName(p->a.dtype) + ">";
+    const std::string type = typeName(p->a.dtype);
+    const Plan n = planFor(p);
+    if (!n.tiles) {
+        name = "attentionKv4Rows<" + type + ">";
+        return name.c_str();
+    }
+    const int dt = dimOf(p->a.dim);
+    name = "attentionKv4Tiles<" + type + ", " + std::to_string(dt) + ", " + std::to_string(n.waves) + ">";
+    if (n.parts() > 0) name += "+attentionJoin<" + type + ", " + std::to_string(p->a.dim <= 64 ? 16 : p->a.dim <= 128 ? 32 : 64) + ">";
     return name.c_str();
 }
 
 int mlkd_launch_attention_kv4(const mlkd_attention_kv4* p, void* stream) {
     const int64_t rows = p->a.q_rows * p->a.heads;
     if (rows == 0) return 0;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (const Plan n = planFor(p); n.tiles) {
+        const int rc = p->a.dtype == MLKD_F32   ? launchPlan<float>(p, n, st)
+                       : p->a.dtype == MLKD_F16 ? launchPlan<_Float16>(p, n, st)
+                                                : launchPlan<__bf16>(p, n, st);
+        if (rc >= 0) return rc;   // else a grid past the limit
+    }
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((rows + 3) / 4, int64_t{1} << 20)));
     auto* kernel = p->a.dtype == MLKD_F32 ? attentionKv4Rows<float> : p->a.dtype == MLKD_F16 ? attentionKv4Rows<_Float16> : attentionKv4Rows<__bf16>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, static_cast<hipStream_t>(stream), *p);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, *p);
     return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
 }
 
