@@ -102,7 +102,9 @@ bool tilesApply(const mlkd_attention* p) {
            aligned(p->k, p->k_stride, 16, 1) && aligned(p->v, p->v_stride, 16, 1);
 }
 
-int dimOf(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
+/// Columns of a kernel that takes a head's codes in whole pieces: of 16 bytes for
+/// 64 and 128, of 8 for 96 and 256.
+int dimOf(int dim) { return dim % 32 == 0 && dim <= 64 ? 64 : dim <= 96 ? 96 : dim == 128 ? 128 : 256; }
 
 /// Row blocks of a launch: at most so many for any lengths.
 int64_t rowBlocks(const mlkd_attention* p) {

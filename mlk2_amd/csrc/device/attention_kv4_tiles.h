@@ -48,6 +48,7 @@ struct Kv4Tiles {
     static constexpr int kPartsW = std::is_same_v<T, float> ? 3 : std::is_same_v<T, _Float16> ? 2 : 1;   // of a weight
     static constexpr int KS = DT / 16, DB = DT / 32;                        // steps of q k^T; 32-column blocks of out
     static constexpr int kWords = DT / 16;                                  // of a lane: half a key's codes
+    static constexpr int kPiece = DT == 64 || DT == 128 ? 16 : 8;           // bytes of a load of codes; a head is whole ones
     static constexpr int kPitch = DT == 64 ? 48 : DT <= 128 ? 80 : 144;     // bytes from value row to row in LDS: 16 rows' words in different banks
     static constexpr int kTile = 32 * kPitch + 256;                         // a wave's values and scales
     static constexpr int kRow = DT * 4;                                     // bytes of a row of results
@@ -142,22 +143,15 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT)) void attentionKv4Tiles(Kv
         float scale;   // a key's: of k in the lower half wave, of v in the upper
     };
     const int halfAt = hl * (DT / 4), bytes = p.dim / 2;
+    // Pieces of the half row behind the head's end repeat its last: their queries
+    // are zeros, their columns not stored.
     auto codes = [&](int (&to)[WORDS], const char* row) {
-        if (DT != 96 && bytes == DT / 2) {   // whole pieces
+        using Words = int __attribute__((ext_vector_type(S::kPiece / 4)));
 #pragma unroll
-            for (int i = 0; i < WORDS; i += 4) {
-                const i32x4 v = *reinterpret_cast<const i32x4*>(row + 4 * i);
+        for (int i = 0; i < WORDS; i += S::kPiece / 4) {
+            const Words v = *reinterpret_cast<const Words*>(row + min(halfAt + 4 * i, bytes - S::kPiece));
 #pragma unroll
-                for (int e = 0; e < 4; ++e) to[i + e < WORDS ? i + e : 0] = v[e];
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < WORDS; i += 2) {
-                i32x2 v = {};
-                if (halfAt + 4 * i < bytes) v = *reinterpret_cast<const i32x2*>(row + 4 * i);
-                to[i] = v[0];
-                to[i + 1] = v[1];
-            }
+            for (int e = 0; e < S::kPiece / 4; ++e) to[i + e] = v[e];
         }
     };
     const char *const k0 = static_cast<const char*>(p.k) + s.k0 * p.k_stride + static_cast<int64_t>(g) * bytes,
@@ -166,8 +160,8 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT)) void attentionKv4Tiles(Kv
     auto load = [&](int it, Tile& to) {
         const int64_t j0 = static_cast<int64_t>(it) * 32;
         const int j = min(l32, limHi - 1 - it * 32);   // keys behind the last repeat it
-        codes(to.k, k0 + j0 * p.k_stride + static_cast<uint32_t>(j) * static_cast<uint32_t>(p.k_stride) + halfAt);
-        codes(to.v, v0 + j0 * p.v_stride + static_cast<uint32_t>(j) * static_cast<uint32_t>(p.v_stride) + halfAt);
+        codes(to.k, k0 + j0 * p.k_stride + static_cast<uint32_t>(j) * static_cast<uint32_t>(p.k_stride));
+        codes(to.v, v0 + j0 * p.v_stride + static_cast<uint32_t>(j) * static_cast<uint32_t>(p.v_stride));
         to.scale = scales[(j0 + j) * p.kv_heads];
     };
 
@@ -189,7 +183,7 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT)) void attentionKv4Tiles(Kv
 #pragma unroll
             for (int n = 0; n < S::kPartsQ; ++n) x = mfma(k, q[n][i], x);
         }
-        if (then < end) load(then, tile);
+        load(min(then, end - 1), tile);   // always: a wait for one tile's loads counts the next one's
         f32x4 ks[4], vs[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -255,7 +249,7 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT)) void attentionKv4Tiles(Kv
     if constexpr (DT <= 128) {   // two tiles in registers
         Tile one, two;
         if (first < end) load(first, one);
-        if (first + NW < end) load(first + NW, two);
+        if (first < end) load(min(first + NW, end - 1), two);
         for (int it = first; it < end; it += 2 * NW) {
             process(it, one, it + 2 * NW);
             if (it + NW >= end) break;
