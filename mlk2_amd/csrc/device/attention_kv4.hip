@@ -83,33 +83,31 @@ __global__ __launch_bounds__(256) void attentionKv4Rows(mlkd_attention_kv4 args)
     }
 }
 
-/// How a launch runs: on the matrix cores or row by row, waves to a row block,
-/// key ranges.
+/// How a launch runs: on the matrix cores or row by row, rows of a block, waves to
+/// one, units of a head that the keys are dealt out to in so many ranges at most (0:
+/// one range to a row block).
 struct Plan {
     bool tiles{false};
-    int waves{1}, splits{1};
-    int parts() const { return splits > 1 ? splits : 0; }
+    int rows{16}, waves{4}, parts{0};
+    int64_t units{0};
 };
 
-/// The matrix-core kernels take rows of whole 16-byte pieces, and codes of whole
-/// eights of heads that are multiples of 16.
+/// The matrix-core kernels take rows of whole 16-byte pieces, and heads of
+/// 32 and more elements in whole sixteens.
 bool tilesApply(const mlkd_attention* p) {
     const int size = p->dtype == MLKD_F32 ? 4 : 2;
     // As attention's: a block reads the lengths 64 at a time, rows and keys are
     // counted in 32 bits.
-    return p->dim % 16 == 0 && p->sequences <= 4096 && p->q_rows * (p->heads / p->kv_heads) < (int64_t{1} << 30) &&
+    return p->dim % 16 == 0 && p->dim >= 32 && p->sequences <= 4096 && p->q_rows * (p->heads / p->kv_heads) < (int64_t{1} << 30) &&
            p->kv_rows <= (int64_t{1} << 30) && aligned(p->q, p->q_stride, 16, size) && aligned(p->out, p->out_stride, 16, size) &&
            aligned(p->k, p->k_stride, 16, 1) && aligned(p->v, p->v_stride, 16, 1);
 }
 
-/// Columns of a kernel that takes a head's codes in whole pieces: of 16 bytes for
-/// 64 and 128, of 8 for 96 and 256.
-int dimOf(int dim) { return dim % 32 == 0 && dim <= 64 ? 64 : dim <= 96 ? 96 : dim == 128 ? 128 : 256; }
-
+int dimOf(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }
 /// Row blocks of a launch: at most so many for any lengths.
-int64_t rowBlocks(const mlkd_attention* p) {
+int64_t rowBlocks(const mlkd_attention* p, int of) {
     const int64_t rows = p->q_rows * (p->heads / p->kv_heads);
-    return rows / 32 + std::min<int64_t>(p->sequences, rows);
+    return rows / of + std::min<int64_t>(p->sequences, rows);
 }
 
 Plan planOf(const mlkd_attention* p) {
@@ -117,23 +115,35 @@ Plan planOf(const mlkd_attention* p) {
     n.tiles = tilesApply(p);
     if (!n.tiles) return n;
     const int64_t group = p->heads / p->kv_heads, each = (p->q_rows + p->sequences - 1) / p->sequences * group;   // rows of a sequence, on average
-    const int64_t count = p->sequences * ((each + 31) / 32) * p->kv_heads, keys = std::max<int64_t>(1, p->kv_rows / p->sequences);
-    n.waves = count >= 2048 ? 1 : 4;
-    if (n.waves == 4) n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({1024 / count, keys / 256, 64})));
+    const int64_t keys = p->kv_rows / p->sequences;   // likewise
+    n.rows = each <= 16 ? 16 : 32;
+    const int64_t blocks = p->sequences * ((each + n.rows - 1) / n.rows), most = rowBlocks(p, n.rows);
+    n.waves = n.rows == 32 && blocks * p->kv_heads >= 4096 ? 1 : 4;
+    n.units = most;
+    // Where the blocks leave units of the chip idle, three of four waves of 16 rows
+    // or two of 32: dealt out by the keys.
+    const int64_t room = (n.rows == 16 ? 768 : 512) / p->kv_heads;
+    if (p->sequences <= 64 && blocks * 4 <= room * 3 && keys >= 512) {
+        n.units = std::max(room, most + 1);
+        n.parts = static_cast<int>(std::min<int64_t>(64, std::max<int64_t>(16, 4 * n.units / p->sequences)));
+    }
     return n;
 }
 
 /// The plan a launch has the workspace for.
 Plan planFor(const mlkd_attention_kv4* p) {
     Plan n = planOf(&p->a);
-    if (n.parts() > 0 && (p->a.work == nullptr || p->a.work_bytes < mlkd_attention_kv4_work_bytes(p))) n.splits = 1;
+    if (n.parts > 0 && (p->a.work == nullptr || p->a.work_bytes < mlkd_attention_kv4_work_bytes(p))) {
+        n.parts = 0;
+        n.units = rowBlocks(&p->a, n.rows);
+    }
     return n;
 }
 
-template <typename T, int DT, int NW>
-int launchTiles(mlk::Kv4Args a, hipStream_t st) {
-    constexpr int bytes = mlk::Kv4Tiles<T, DT, NW>::kLds;
-    auto* kernel = mlk::attentionKv4Tiles<T, DT, NW>;
+template <typename T, int DT, int ROWS, int NW>
+int launchTiles(const mlk::Kv4Args& a, hipStream_t st) {
+    constexpr int bytes = mlk::Kv4Tiles<T, DT, ROWS, NW>::kLds;
+    auto* kernel = mlk::attentionKv4Tiles<T, DT, ROWS, NW>;
     // Once per process; a function-local static initializes thread-safely.
     static const bool allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                     bytes) == hipSuccess;
@@ -145,8 +155,10 @@ int launchTiles(mlk::Kv4Args a, hipStream_t st) {
 }
 
 template <typename T, int DT>
-int launchWaves(const mlk::Kv4Args& a, int waves, hipStream_t st) {
-    return waves == 1 ? launchTiles<T, DT, 1>(a, st) : launchTiles<T, DT, 4>(a, st);
+int launchForm(const mlk::Kv4Args& a, const Plan& n, hipStream_t st) {
+    if (n.rows == 16) return launchTiles<T, DT, 16, 4>(a, st);
+    if (n.waves == 4) return launchTiles<T, DT, 32, 4>(a, st);
+    return launchTiles<T, DT, 32, 1>(a, st);
 }
 
 template <typename T>
@@ -155,25 +167,22 @@ int launchPlan(const mlkd_attention_kv4* p, const Plan& n, hipStream_t st) {
     a.t.p = p->a;
     a.k_scale = p->k_scale;
     a.v_scale = p->v_scale;
-    a.t.splits = n.splits;
-    a.t.parts = n.parts();
+    a.t.parts = n.parts;
+    if (n.units >= (int64_t{1} << 30)) return -1;
+    a.units = static_cast<int>(n.units);
     if (a.t.parts > 0) {
         a.t.acc = static_cast<float*>(p->a.work);
         a.t.ml = reinterpret_cast<float2*>(a.t.acc + a.t.parts * p->a.q_rows * p->a.heads * p->a.dim);
     }
     a.t.by_group = dividerOf(p->a.heads / p->a.kv_heads);
     a.t.by_kv_heads = dividerOf(p->a.kv_heads);
-    a.t.by_splits = dividerOf(n.splits);
     a.t.by_heads = dividerOf(p->a.heads);
-    const int64_t units = rowBlocks(&p->a) * n.splits;
-    if (units >= (int64_t{1} << 30)) return -1;
-    a.units = static_cast<int>(units);
     int rc = 0;
     switch (dimOf(p->a.dim)) {
-        case 64: rc = launchWaves<T, 64>(a, n.waves, st); break;
-        case 96: rc = launchWaves<T, 96>(a, n.waves, st); break;
-        case 128: rc = launchWaves<T, 128>(a, n.waves, st); break;
-        default: rc = launchWaves<T, 256>(a, n.waves, st); break;
+        case 64: rc = launchForm<T, 64>(a, n, st); break;
+        case 96: rc = launchForm<T, 96>(a, n, st); break;
+        case 128: rc = launchForm<T, 128>(a, n, st); break;
+        default: rc = launchForm<T, 256>(a, n, st); break;
     }
     if (rc != 0 || a.t.parts == 0) return rc;
     const int64_t rows = p->a.q_rows * p->a.heads;
@@ -189,7 +198,7 @@ const char* typeName(int dtype) { return dtype == MLKD_F32 ? "float" : dtype == 
 extern "C" {
 
 int64_t mlkd_attention_kv4_work_bytes(const mlkd_attention_kv4* p) {
-    return planOf(&p->a).parts() * p->a.q_rows * p->a.heads * (p->a.dim * static_cast<int64_t>(sizeof(float)) + static_cast<int64_t>(sizeof(float2)));
+    return planOf(&p->a).parts * p->a.q_rows * p->a.heads * (p->a.dim * static_cast<int64_t>(sizeof(float)) + static_cast<int64_t>(sizeof(float2)));
 }
 
 const char* mlkd_attention_kv4_kernel_names(const mlkd_attention_kv4* p) {
@@ -201,8 +210,8 @@ const char* mlkd_attention_kv4_kernel_names(const mlkd_attention_kv4* p) {
         return name.c_str();
     }
     const int dt = dimOf(p->a.dim);
-    name = "attentionKv4Tiles<" + type + ", " + std::to_string(dt) + ", " + std::to_string(n.waves) + ">";
-    if (n.parts() > 0) name += "+attentionJoin<" + type + ", " + std::to_string(p->a.dim <= 64 ? 16 : p->a.dim <= 128 ? 32 : 64) + ">";
+    name = "attentionKv4Tiles<" + type + ", " + std::to_string(dt) + ", " + std::to_string(n.rows) + ", " + std::to_string(n.waves) + ">";
+    if (n.parts > 0) name += "+attentionJoin<" + type + ", " + std::to_string(p->a.dim <= 64 ? 16 : p->a.dim <= 128 ? 32 : 64) + ">";
     return name.c_str();
 }
 

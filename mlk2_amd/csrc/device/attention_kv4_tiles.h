@@ -20,7 +20,7 @@ using f16x2 = _Float16 __attribute__((ext_vector_type(2)));
 struct Kv4Args {
     TileArgs t;                      // p's k and v: the codes, strides in bytes
     const float *k_scale, *v_scale;  // [kv_rows, kv_heads]
-    int units;                       // row blocks times key ranges
+    int units;                       // row blocks, or with parts their key ranges, of one head at most
 };
 
 /// The numbers of a word's eight codes, exact in either type.
@@ -39,244 +39,425 @@ __device__ __forceinline__ Piece<_Float16> numbers<_Float16>(int word) {
     return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-/// NW waves with the same 32 rows, the tiles in turn; their sums are joined at
-/// the end.
-template <typename T, int DT, int NW>
+template <int N>
+using F32 = float __attribute__((ext_vector_type(N)));
+
+/// c += a b: 32 x 32 by 16, or 16 x 16 by 32.
+template <int EDGE>
+__device__ __forceinline__ F32<EDGE * EDGE / 64> product(Piece<__bf16> a, Piece<__bf16> b, F32<EDGE * EDGE / 64> c) {
+    if constexpr (EDGE == 32) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+template <int EDGE>
+__device__ __forceinline__ F32<EDGE * EDGE / 64> product(Piece<_Float16> a, Piece<_Float16> b, F32<EDGE * EDGE / 64> c) {
+    if constexpr (EDGE == 32) return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+/// The value of lane l ^ 16.
+__device__ __forceinline__ float otherSixteen(float v) {
+    const int i = __builtin_bit_cast(int, v);
+    const auto r = __builtin_amdgcn_permlane16_swap(i, i, false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 16) != 0 ? r[0] : r[1]);
+}
+
+/// The largest, and the sum, over the lanes of one query: those EDGE apart.
+template <int EDGE>
+__device__ __forceinline__ float largestOf(float v) {
+    if constexpr (EDGE == 16) v = fmaxf(v, otherSixteen(v));
+    return fmaxf(v, otherHalf(v));
+}
+template <int EDGE>
+__device__ __forceinline__ float sumOf(float v) {
+    if constexpr (EDGE == 16) v += otherSixteen(v);
+    return v + otherHalf(v);
+}
+
+/// NW waves with the same ROWS query rows, tiles of 32 keys in turn; their sums are
+/// joined at the end.
+template <typename T, int DT, int ROWS, int NW>
 struct Kv4Tiles {
     using Q = std::conditional_t<std::is_same_v<T, float>, __bf16, T>;      // the scores' operands
     static constexpr int kPartsQ = std::is_same_v<T, float> ? 3 : 1;        // of a query: 24 bits in 8 each
     static constexpr int kPartsW = std::is_same_v<T, float> ? 3 : std::is_same_v<T, _Float16> ? 2 : 1;   // of a weight
-    static constexpr int KS = DT / 16, DB = DT / 32;                        // steps of q k^T; 32-column blocks of out
-    static constexpr int kWords = DT / 16;                                  // of a lane: half a key's codes
-    static constexpr int kPiece = DT == 64 || DT == 128 ? 16 : 8;           // bytes of a load of codes; a head is whole ones
-    static constexpr int kPitch = DT == 64 ? 48 : DT <= 128 ? 80 : 144;     // bytes from value row to row in LDS: 16 rows' words in different banks
-    static constexpr int kTile = 32 * kPitch + 256;                         // a wave's values and scales
+    static constexpr int kEdge = ROWS < 32 ? 16 : 32, kLanes = 64 / kEdge;  // of a product; lanes of a query (or a key)
+    static constexpr int QB = ROWS / kEdge, KB = 32 / kEdge;                // blocks of queries, of a tile's keys
+    static constexpr int KS = DT / 8 / kLanes;                              // steps of q k^T, eight elements a lane
+    static constexpr int NS = kEdge * kEdge / 64 * KB;                      // scores of a lane, per block of queries
+    static constexpr int NO = kEdge * kEdge / 64, DB = DT / kEdge;          // sums of a lane and block of out; its blocks
+    static constexpr int kPieces = DT <= 64 ? 2 : DT <= 128 ? 4 : 8;        // 16-byte pieces of a row in LDS
+    static constexpr int kPitch = 16 * kPieces;
+    static constexpr int kHalf = 32 * kPitch, kStage = 2 * kHalf + 256;     // a tile's keys (or values); with the scales
+    static constexpr int kLoads = kHalf / 1024;                             // of 64 pieces, for keys and again for values
+    static constexpr int kPerTile = 2 * kLoads + 1;
+    static constexpr int kStages = ROWS == 16 ? 3 : 4;                      // three times four waves of 16 rows fit a compute unit
+    static constexpr int kRing = kStage * kStages;
     static constexpr int kRow = DT * 4;                                     // bytes of a row of results
-    static constexpr int kJoin = 32 * kRow + 256;
-    static constexpr int kLds = NW * (kTile > kJoin ? kTile : kJoin);
+    static constexpr int kJoin = ROWS * (kRow + 8);
+    static constexpr int kLds = NW * (kRing > kJoin ? kRing : kJoin);
+    static_assert(kPerTile * (kStages - 1) <= 63, "the loads waited on by number fit the counter");
+
+    /// Turn of row j's pieces, so that the rows that are read at a time lie in
+    /// different banks: 16 from one on, or fours of them eight or sixteen apart.
+    static __device__ __forceinline__ int swizzle(int j) {
+        return kPieces == 2 ? j >> 3 & 1 : kPieces == 4 ? (j >> 2 & 3) ^ (j >> 4 & 1) : (j >> 1 & 7) ^ (j >> 4 & 1) << 1;
+    }
+
+    /// 16 (or 4) bytes a lane to LDS at `m0` + 16 (4) * lane. A load to LDS takes M0
+    /// one wait state after a scalar write of it at the earliest (s_nop 0).
+    static __device__ __forceinline__ void dma16(const void* base, uint32_t off, uint32_t m0) {
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory");
+    }
+    static __device__ __forceinline__ void dma4(const void* from, uint32_t m0) {
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(from), "s"(__builtin_amdgcn_readfirstlane(m0)) : "memory");
+    }
+    /// Waits until at most `ahead` tiles of this wave's loads are in flight, and no
+    /// read of LDS.
+    static __device__ __forceinline__ void wait(int ahead) {
+        if (kStages > 3 && ahead >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * kPerTile) : "memory");
+        else if (ahead >= 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kPerTile) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    }
 };
+
+/// What a workgroup takes: a row block of a sequence, and which of so many ranges of
+/// its keys.
+struct Kv4Unit {
+    SeqSpan s;
+    int r0, split, splits;
+};
+
+/// Unit `unit` of `units`, which are dealt out by the keys there are: a sequence's
+/// row blocks are split into as many ranges, `parts` at most, as make all of them
+/// about equally long, so that all units of a launch run at once and end together
+/// (32 single tokens over 1024 to 8192 keys: BALANCED). For 64 sequences at most, a
+/// lane each, and more units than there are row blocks.
+template <int ROWS>
+__device__ __forceinline__ bool dealtUnit(const mlkd_attention& p, int group, int unit, int units, int parts, Kv4Unit& u) {
+    const int ln = threadIdx.x & 63;
+    SeqSpan of{};
+    if (ln < p.sequences) of = spanOf(p, ln);
+    const int blocks = (of.nq * group + ROWS - 1) / ROWS, tiles = blocks > 0 ? (of.nk + 31) / 32 : 0;
+    const int free = units - __builtin_amdgcn_readlane(sumUpTo(blocks), 63);   // units beside a block's first
+    float all = static_cast<float>(blocks) * static_cast<float>(tiles);
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) all += __shfl_xor(all, d, 64);
+    // The shortest range that the units suffice for, to a sixteenth of where it lies:
+    // no shorter than all tiles over all units, and all over the free ones (a little
+    // more than exactly) has room for the blocks' last, shorter ranges. One tile for
+    // each wave at least, two where the ranges' number is no limit.
+    const int shortest = max(8, (largest(tiles) + parts - 1) / parts);
+    auto rangesOf = [&](int range) { return max(1, (tiles + range - 1) / range); };
+    int range = max(shortest, static_cast<int>(fminf(all / static_cast<float>(free) * 1.001f, 1e9f)) + 1);
+    int below = max(shortest, static_cast<int>(fminf(all / static_cast<float>(units), 1e9f)));
+    for (int n = 0; n < 4 && below < range; ++n) {
+        const int middle = (below + range) / 2;
+        if (__builtin_amdgcn_readlane(sumUpTo(blocks * rangesOf(middle)), 63) <= units) range = middle;
+        else below = middle + 1;
+    }
+    const int ranges = rangesOf(range);
+    const int sum = sumUpTo(blocks * ranges);
+    const uint64_t past = __ballot(sum > unit);
+    if (past == 0) return false;
+    const int b = __builtin_ctzll(past), at = unit - __builtin_amdgcn_readlane(sum - blocks * ranges, b);
+    u.splits = __builtin_amdgcn_readlane(ranges, b);
+    const int block = at / u.splits;
+    u.split = at - block * u.splits;
+    u.r0 = (__builtin_amdgcn_readlane(blocks, b) - 1 - block) * ROWS;
+    u.s = SeqSpan{laneOf(of.q0, b), laneOf(of.k0, b), __builtin_amdgcn_readlane(of.nq, b), __builtin_amdgcn_readlane(of.nk, b)};
+    return true;
+}
 
 /// Waves of a SIMD that the registers have to hold.
 template <typename T>
-constexpr int kv4Waves(int dt) {
-    return std::is_same_v<T, float> || dt > 128 ? 1 : 2;
+constexpr int kv4Waves(int dt, int rows) {
+    return rows == 16 ? (std::is_same_v<T, float> || dt > 128 ? 2 : 3) : std::is_same_v<T, float> || dt > 128 ? 1 : 2;
 }
 
-/// One row block of one key/value head. With S^T = K Q^T in 32 x 32 blocks a lane
-/// holds 16 keys' scores of one query (the other 16 in lane ^ 32), so the softmax
-/// is register work but for one exchange of maxima. The products run on the codes
-/// as numbers, which either 16-bit type holds exactly: a key's scale goes to its
-/// scores, a value's to its weights. Half a key row's codes are a lane's operand
-/// as they lie in memory, eight to a word. Values take one trip through LDS: a
-/// transposing read of 4-bit elements hands a lane one column of the 16 keys whose
-/// weights it holds, in their order.
+/// One row block of one key/value head. With S^T = K Q^T a lane holds some keys'
+/// scores of one query, so the softmax is register work but for one exchange of
+/// maxima. The products run on the codes as numbers, which either 16-bit type holds
+/// exactly: a key's scale goes to its scores, a value's to its weights. Codes come
+/// straight to LDS, three tiles ahead; a word of a key's row is eight elements of
+/// the product's operand as it lies. Values are read transposed, 4 bits at a time:
+/// a lane gets a column's numbers of the keys whose weights it holds, in their
+/// order.
 ///
 /// What is rounded: a weight times its value's scale to bf16 (f16 rows: to two
 /// bf16 parts, 16 bits, f32 rows three), half a step of itself; f32 queries are
 /// three bf16 parts, exactly. Scores, weights, their sum and out's sums are f32.
 /// The maximum that the weights are relative to follows the running one only when
 /// that has grown by 2^8.
-template <typename T, int DT, int NW>
-__global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT)) void attentionKv4Tiles(Kv4Args args) {
-    using S = Kv4Tiles<T, DT, NW>;
+template <typename T, int DT, int ROWS, int NW>
+__global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT, ROWS)) void attentionKv4Tiles(Kv4Args args) {
+    using S = Kv4Tiles<T, DT, ROWS, NW>;
     using Q = typename S::Q;
-    constexpr int KS = S::KS, DB = S::DB, WORDS = S::kWords;
+    constexpr int EDGE = S::kEdge, QB = S::QB, KB = S::KB, KS = S::KS, NS = S::NS, NO = S::NO, DB = S::DB;
     extern __shared__ __align__(16) char ldsTiles[];
     const TileArgs& a = args.t;
     const mlkd_attention& p = a.p;
     const int wave = NW == 1 ? 0 : __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-    const int ln = threadIdx.x & 63, l32 = ln & 31, hl = ln >> 5;
+    const int ln = threadIdx.x & 63, col = ln % EDGE, part = ln / EDGE;
     // The heads of a unit go to one XCD one after the other: neighbouring heads'
     // codes share lines of 128 bytes.
     const int id = static_cast<int>(blockIdx.x), turn = id / 8, upper = turn / a.by_kv_heads, g = turn - upper * p.kv_heads;
     const int unit = upper * 8 + id % 8;
     if (unit >= args.units) return;
-    const int rest = unit / a.by_splits, split = unit - rest * a.splits, group = p.heads / p.kv_heads;
-    SeqSpan s{};
-    int r0 = 0;
-    if (!rowBlock<32>(p, group, rest, s, r0)) return;
-    s = SeqSpan{uniform(s.q0), uniform(s.k0), static_cast<int32_t>(uniform(s.nq)), static_cast<int32_t>(uniform(s.nk))};
-    r0 = __builtin_amdgcn_readfirstlane(r0);
+    const int group = p.heads / p.kv_heads;
+    Kv4Unit u{};
+    u.splits = 1;
+    if (!(a.parts > 0 ? dealtUnit<ROWS>(p, group, unit, args.units, a.parts, u) : rowBlock<ROWS>(p, group, unit, u.s, u.r0))) return;
+    const SeqSpan s{uniform(u.s.q0), uniform(u.s.k0), static_cast<int32_t>(uniform(u.s.nq)), static_cast<int32_t>(uniform(u.s.nk))};
+    const int r0 = __builtin_amdgcn_readfirstlane(u.r0), split = __builtin_amdgcn_readfirstlane(u.split), splits = __builtin_amdgcn_readfirstlane(u.splits);
     const int rows = s.nq * group;
     // Keys that a row sees: those below its limit.
     auto limit = [&](int r) {
         return p.causal != 0 ? min(max(min(r, rows - 1) / a.by_group + s.nk - s.nq + 1, 0), s.nk) : s.nk;
     };
-    const int limLo = __builtin_amdgcn_readfirstlane(limit(r0)), limHi = __builtin_amdgcn_readfirstlane(limit(r0 + 31)), lim = limit(r0 + l32);
-    const int tiles = (limHi + 31) / 32, each = tiles / a.by_splits, more = tiles - each * a.splits;
-    const int first = __builtin_amdgcn_readfirstlane(each * split + min(split, more)) + wave;
-    const int end = __builtin_amdgcn_readfirstlane(each * split + min(split, more) + each + (split < more ? 1 : 0));
+    const int limLo = __builtin_amdgcn_readfirstlane(limit(r0)), limHi = __builtin_amdgcn_readfirstlane(limit(r0 + ROWS - 1));
+    int lim[QB];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) lim[b] = limit(r0 + b * EDGE + col) - 4 * part;
+    const int tiles = (limHi + 31) / 32, each = __builtin_amdgcn_readfirstlane(tiles / splits), more = tiles - each * splits;
+    const int first = each * split + min(split, more) + wave;
+    const int end = each * split + min(split, more) + each + (split < more ? 1 : 0);
     const int token0 = __builtin_amdgcn_readfirstlane(r0 / a.by_group);
     auto tokenOf = [&](int r) { return r / a.by_group - token0; };
     auto headOf = [&](int r, int t) { return r - (t + token0) * group + g * group; };
 
-    // Queries: step i takes elements hl DT / 2 + 8 i .. + 7, as half a key row lies.
-    Piece<Q> q[S::kPartsQ][KS];
-    {
-        const int r = min(r0 + l32, rows - 1), t = tokenOf(r);
+    // Where sixteen elements of a head lie in LDS, from which on (-1: nowhere). A
+    // head of half a piece more than whole ones has its last 16 bytes as a piece,
+    // the first eight of them a second time.
+    const int bytes = p.dim / 2, lastPiece = (bytes - 1) / 16;
+    const bool half = bytes % 16 != 0;
+    auto elementsAt = [&](int unit16) {
+        const int n = half && unit16 >= 2 * lastPiece ? (unit16 == 2 * lastPiece + 1 ? 2 * lastPiece : -1) : unit16;
+        return n >= 0 && n * 16 < p.dim ? n * 16 : -1;
+    };
+
+    // This wave's loads of a tile: row and piece of each, by lane.
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(ldsTiles)) + wave * S::kRing;
+    const char *const k0 = static_cast<const char*>(p.k) + s.k0 * p.k_stride + static_cast<int64_t>(g) * bytes,
+               *const v0 = static_cast<const char*>(p.v) + s.k0 * p.v_stride + static_cast<int64_t>(g) * bytes;
+    // Rows of a tile lie less than 2^24 bytes apart, keys of 31 of them and scales too.
+    const uint32_t ks = static_cast<uint32_t>(p.k_stride), vs = static_cast<uint32_t>(p.v_stride), heads4 = p.kv_heads * 4;
+    const char* const scales = reinterpret_cast<const char*>((ln < 32 ? args.k_scale : args.v_scale) + s.k0 * p.kv_heads + g);
+    uint32_t place = lds0;   // of the next tile to ask for
+    auto load = [&](int it) __attribute__((always_inline)) {
+        const int64_t j0 = static_cast<int64_t>(it) * 32;
+        const int last = limHi - 1 - it * 32;   // keys behind the last repeat it
+        const char *const kt = reinterpret_cast<const char*>(uniform(reinterpret_cast<int64_t>(k0 + j0 * p.k_stride))),
+                   *const vt = reinterpret_cast<const char*>(uniform(reinterpret_cast<int64_t>(v0 + j0 * p.v_stride)));
+#pragma unroll
+        for (int i = 0; i < S::kLoads; ++i) {
+            const int row = (i * 64 + ln) / S::kPieces, piece = ln % S::kPieces ^ S::swizzle(row);
+            const uint32_t at = piece == lastPiece ? bytes - 16 : piece * 16, j = min(row, last);
+            if (piece <= lastPiece) {
+                S::dma16(kt, __umul24(j, ks) + at, place + i * 1024);
+                S::dma16(vt, __umul24(j, vs) + at, place + S::kHalf + i * 1024);
+            }
+        }
+        S::dma4(scales + j0 * heads4 + __umul24(min(ln & 31, last), heads4), place + 2 * S::kHalf);
+        place = place == lds0 + (S::kStages - 1) * S::kStage ? lds0 : place + S::kStage;
+    };
+#pragma unroll
+    for (int n = 0; n < S::kStages - 1; ++n) {
+        if (first + n * NW < end) load(first + n * NW);
+    }
+
+    // Queries: step i takes the eight elements whose codes a lane's i-th word holds.
+    Piece<Q> q[S::kPartsQ][QB][KS];
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        const int r = min(r0 + b * EDGE + col, rows - 1), t = tokenOf(r);
         const T* row = static_cast<const T*>(p.q) + (s.q0 + token0 + t) * p.q_stride + static_cast<int64_t>(headOf(r, t)) * p.dim;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-            const int d = hl * (DT / 2) + 8 * i;
+            const int place = part * KS + i, d = elementsAt(place / 2);
             using V8 = T __attribute__((ext_vector_type(8)));
             V8 v = {};
-            if (d < p.dim) v = *reinterpret_cast<const V8*>(row + d);
+            if (d >= 0) v = *reinterpret_cast<const V8*>(row + d + place % 2 * 8);
             if constexpr (S::kPartsQ == 1) {
-                q[0][i] = v;
+                q[0][b][i] = v;
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) {
                     float left = v[e];
 #pragma unroll
                     for (int n = 0; n < S::kPartsQ; ++n) {
-                        q[n][i][e] = static_cast<Q>(left);
-                        left -= static_cast<float>(q[n][i][e]);
+                        q[n][b][i][e] = static_cast<Q>(left);
+                        left -= static_cast<float>(q[n][b][i][e]);
                     }
                 }
             }
         }
     }
+    // They are taken here: the compiler knows nothing of the loads to LDS and would
+    // wait for these, and so for all, in every tile.
+#pragma unroll
+    for (int n = 0; n < S::kPartsQ; ++n) {
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+#pragma unroll
+            for (int i = 0; i < KS; ++i) {
+                i32x4 bits = __builtin_bit_cast(i32x4, q[n][b][i]);
+                asm volatile("" : "+v"(bits));
+                q[n][b][i] = __builtin_bit_cast(Piece<Q>, bits);
+            }
+        }
+    }
     const float c = static_cast<float>(p.scale * 1.4426950408889634);
 
-    struct Tile {
-        int k[WORDS], v[WORDS];
-        float scale;   // a key's: of k in the lower half wave, of v in the upper
-    };
-    const int halfAt = hl * (DT / 4), bytes = p.dim / 2;
-    // Pieces of the half row behind the head's end repeat its last: their queries
-    // are zeros, their columns not stored.
-    auto codes = [&](int (&to)[WORDS], const char* row) {
-        using Words = int __attribute__((ext_vector_type(S::kPiece / 4)));
+    // A lane's words of key block kb: those of row kb EDGE + col from `part` on.
+    constexpr int WB = KS * 4;   // bytes of them
+    auto words = [&](const char* tile, int kb, int (&w)[KS]) __attribute__((always_inline)) {
+        const int row = kb * EDGE + col, turned = S::swizzle(row) << 4;
+        constexpr int READ = WB % 16 == 0 ? 16 : WB % 8 == 0 ? 8 : 4;
+        using Words = int __attribute__((ext_vector_type(READ / 4)));
 #pragma unroll
-        for (int i = 0; i < WORDS; i += S::kPiece / 4) {
-            const Words v = *reinterpret_cast<const Words*>(row + min(halfAt + 4 * i, bytes - S::kPiece));
+        for (int i = 0; i < KS; i += READ / 4) {
+            const int byte = part * WB + i * 4;
+            const auto v = *reinterpret_cast<const Words*>(tile + row * S::kPitch + (byte ^ turned));
+            if constexpr (READ == 4) {
+                w[i] = v[0];
+            } else {
 #pragma unroll
-            for (int e = 0; e < S::kPiece / 4; ++e) to[i + e] = v[e];
+                for (int e = 0; e < READ / 4; ++e) w[i + e] = v[e];
+            }
         }
     };
-    const char *const k0 = static_cast<const char*>(p.k) + s.k0 * p.k_stride + static_cast<int64_t>(g) * bytes,
-               *const v0 = static_cast<const char*>(p.v) + s.k0 * p.v_stride + static_cast<int64_t>(g) * bytes;
-    const float* const scales = (hl == 0 ? args.k_scale : args.v_scale) + s.k0 * p.kv_heads + g;
-    auto load = [&](int it, Tile& to) {
-        const int64_t j0 = static_cast<int64_t>(it) * 32;
-        const int j = min(l32, limHi - 1 - it * 32);   // keys behind the last repeat it
-        codes(to.k, k0 + j0 * p.k_stride + static_cast<uint32_t>(j) * static_cast<uint32_t>(p.k_stride));
-        codes(to.v, v0 + j0 * p.v_stride + static_cast<uint32_t>(j) * static_cast<uint32_t>(p.v_stride));
-        to.scale = scales[(j0 + j) * p.kv_heads];
-    };
+    // The row whose eight bytes this lane hands the transposing read, and where.
+    const int j16 = ln & 15;
+    const int vrow = EDGE == 32 ? 8 * (j16 >> 2) + 4 * part + (j16 & 3) : 16 * ((j16 >> 2) & 1) + 4 * part + (j16 & 3);
+    const uint32_t vat = vrow * S::kPitch + (S::swizzle(vrow) << 4) + (EDGE == 32 ? (ln >> 4) & 1 : j16 >> 3) * 8;
 
-    char* const mine = ldsTiles + wave * S::kTile;
-    float* const tileScales = reinterpret_cast<float*>(mine + 32 * S::kPitch);
-    // The row whose bytes this lane hands the transposing read, and its columns.
-    const char* const column = mine + (8 * ((ln & 15) >> 2) + 4 * hl + (ln & 3)) * S::kPitch + ((ln >> 4) & 1) * 8;
-    f32x16 o[DB] = {};
-    float m = kLowest, l = 0.0f;   // what the weights of this lane's query are relative to; of this lane's keys, their sum
-    // Tile `it`; its registers take tile `then`'s codes once they are used.
-    auto process = [&](int it, Tile& tile, int then) __attribute__((always_inline)) {
+    F32<NO> o[QB][DB] = {};
+    float m[QB], l[QB];   // what the weights of this lane's queries are relative to; of this lane's keys, their sum
 #pragma unroll
-        for (int i = 0; i < WORDS; i += 2) *reinterpret_cast<i32x2*>(mine + l32 * S::kPitch + halfAt + 4 * i) = i32x2{tile.v[i], tile.v[i + 1]};
-        tileScales[ln] = hl == 0 ? tile.scale * c : tile.scale;
-        f32x16 x = {};
+    for (int b = 0; b < QB; ++b) {
+        m[b] = kLowest;
+        l[b] = 0.0f;
+    }
+    constexpr int kApart = EDGE == 32 ? 8 : 16;   // between the fours of keys that a lane holds
+    int taken = 0;   // the tile's place
+    for (int it = first; it < end; it += NW) {
+        const char* const tile = ldsTiles + wave * S::kRing + taken;
+        taken = taken == (S::kStages - 1) * S::kStage ? 0 : taken + S::kStage;
+        S::wait(it + 2 * NW < end ? 2 : it + NW < end ? 1 : 0);
+        // Into the place of the tile before, whose values are in their sums.
+        if (it + (S::kStages - 1) * NW < end) load(it + (S::kStages - 1) * NW);
+        F32<NO> x[QB][KB] = {};
 #pragma unroll
-        for (int i = 0; i < KS; ++i) {
-            const Piece<Q> k = numbers<Q>(tile.k[i]);
+        for (int kb = 0; kb < KB; ++kb) {
+            int w[KS];
+            words(tile, kb, w);
 #pragma unroll
-            for (int n = 0; n < S::kPartsQ; ++n) x = mfma(k, q[n][i], x);
+            for (int i = 0; i < KS; ++i) {
+                const Piece<Q> k = numbers<Q>(w[i]);
+#pragma unroll
+                for (int b = 0; b < QB; ++b) {
+#pragma unroll
+                    for (int n = 0; n < S::kPartsQ; ++n) x[b][kb] = product<EDGE>(k, q[n][b][i], x[b][kb]);
+                }
+            }
         }
-        load(min(then, end - 1), tile);   // always: a wait for one tile's loads counts the next one's
-        f32x4 ks[4], vs[4];
+        f32x4 kScale[NS / 4], vScale[NS / 4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            ks[e] = *reinterpret_cast<const f32x4*>(tileScales + 8 * e + 4 * hl);
-            vs[e] = *reinterpret_cast<const f32x4*>(tileScales + 32 + 8 * e + 4 * hl);
+        for (int e = 0; e < NS / 4; ++e) {
+            const float* const at = reinterpret_cast<const float*>(tile + 2 * S::kHalf) + kApart * e + 4 * part;
+            kScale[e] = *reinterpret_cast<const f32x4*>(at) * c;
+            vScale[e] = *reinterpret_cast<const f32x4*>(at + 32);
         }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[e] *= ks[e / 4][e % 4];
-        const int seen = lim - it * 32 - 4 * hl;   // keys of this lane's, counted as the scores are
         const bool edge = limLo < it * 32 + 32;
-        if (edge) {
+        Piece<__bf16> w[QB][S::kPartsW][NS / 8];
 #pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = 8 * (e / 4) + e % 4 < seen ? x[e] : -INFINITY;
-            asm volatile("" : "+v"(x));   // a branch
-        }
-        float top = x[0];
+        for (int b = 0; b < QB; ++b) {
+            const int seen = lim[b] - it * 32;   // keys of this lane's, counted as the scores are
+            float y[NS];
 #pragma unroll
-        for (int e = 1; e < 16; ++e) top = fmaxf(top, x[e]);
-        top = fmaxf(top, otherHalf(top));
-        while (__any(top > m + 8.0f)) {   // once at most
-            const float base = fmaxf(m, top), keep = __builtin_amdgcn_exp2f(m - base);
-            m = base;
-            l *= keep;
+            for (int e = 0; e < NS; ++e) y[e] = x[b][e / NO][e % NO] * kScale[e / 4][e % 4];
+            if (edge) {
 #pragma unroll
-            for (int i = 0; i < DB; ++i) {
+                for (int e = 0; e < NS; ++e) {
+                    y[e] = kApart * (e / 4) + e % 4 < seen ? y[e] : -INFINITY;
+                    asm volatile("" : "+v"(y[e]));   // a branch
+                }
+            }
+            float top = y[0];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) o[i][e] *= keep;
+            for (int e = 1; e < NS; ++e) top = fmaxf(top, y[e]);
+            top = largestOf<EDGE>(top);
+            if (__any(top > m[b] + 8.0f)) {
+                const float base = fmaxf(m[b], top), keep = __builtin_amdgcn_exp2f(m[b] - base);
+                m[b] = base;
+                l[b] *= keep;
+#pragma unroll
+                for (int i = 0; i < DB; ++i) {
+#pragma unroll
+                    for (int e = 0; e < NO; ++e) o[b][i][e] *= keep;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < NS; ++e) {
+                y[e] = __builtin_amdgcn_exp2f(y[e] - m[b]);
+                l[b] += y[e];
+                y[e] *= vScale[e / 4][e % 4];
+            }
+            if (edge) {   // a hidden value's scale may be anything
+#pragma unroll
+                for (int e = 0; e < NS; ++e) {
+                    y[e] = kApart * (e / 4) + e % 4 < seen ? y[e] : 0.0f;
+                    asm volatile("" : "+v"(y[e]));
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < NS; ++e) {
+                float left = y[e];
+#pragma unroll
+                for (int n = 0; n < S::kPartsW; ++n) {
+                    w[b][n][e / 8][e % 8] = static_cast<__bf16>(left);
+                    left -= static_cast<float>(w[b][n][e / 8][e % 8]);
+                }
             }
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            x[e] = __builtin_amdgcn_exp2f(x[e] - m);
-            l += x[e];
-            x[e] *= vs[e / 4][e % 4];
-        }
-        if (edge) {   // a hidden value's scale may be anything
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x[e] = 8 * (e / 4) + e % 4 < seen ? x[e] : 0.0f;
-            asm volatile("" : "+v"(x));
-        }
-        Piece<__bf16> w[S::kPartsW][2];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            float left = x[e];
-#pragma unroll
-            for (int n = 0; n < S::kPartsW; ++n) {
-                w[n][e / 8][e % 8] = static_cast<__bf16>(left);
-                left -= static_cast<float>(w[n][e / 8][e % 8]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < DB; ++i) {
+        for (int i = 0; i < DT / 32; ++i) {
             using Lds = __attribute__((address_space(3))) i32x2;
-            const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32((Lds*)(column + i * 16));
+            const i32x2 v = __builtin_amdgcn_ds_read_tr4_b64_v2i32((Lds*)(tile + S::kHalf + (vat ^ (i << 4))));
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const Piece<__bf16> vv = numbers<__bf16>(v[half]);
+            for (int n = 0; n < 2; ++n) {
+                // Of 32 columns a read's halves are those of the first and the second
+                // eight keys, of 16 those of two blocks of columns.
+                const Piece<__bf16> vv = numbers<__bf16>(v[n]);
+                const int block = EDGE == 32 ? i : 2 * i + n, keys = EDGE == 32 ? n : 0;
 #pragma unroll
-                for (int n = 0; n < S::kPartsW; ++n) o[i] = mfma(vv, w[n][half], o[i]);
+                for (int b = 0; b < QB; ++b) {
+#pragma unroll
+                    for (int k = 0; k < S::kPartsW; ++k) o[b][block] = product<EDGE>(vv, w[b][k][keys], o[b][block]);
+                }
             }
         }
-    };
-    if constexpr (DT <= 128) {   // two tiles in registers
-        Tile one, two;
-        if (first < end) load(first, one);
-        if (first < end) load(min(first + NW, end - 1), two);
-        for (int it = first; it < end; it += 2 * NW) {
-            process(it, one, it + 2 * NW);
-            if (it + NW >= end) break;
-            process(it + NW, two, it + 3 * NW);
-        }
-    } else {
-        Tile one;
-        if (first < end) load(first, one);
-        for (int it = first; it < end; it += NW) process(it, one, it + NW);
     }
 
     // The waves' sums by rows through LDS, 16 bytes a lane, joined on the way out.
-    l += otherHalf(l);
     if constexpr (NW > 1) __syncthreads();   // all are done with their tiles
     char* const sums = ldsTiles;
-    float2* const tops = reinterpret_cast<float2*>(ldsTiles + NW * 32 * S::kRow);
-    if (r0 + l32 < rows) {
-        char* const at = sums + (wave * 32 + l32) * S::kRow;
+    float2* const tops = reinterpret_cast<float2*>(ldsTiles + NW * ROWS * S::kRow);
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        l[b] = sumOf<EDGE>(l[b]);
+        const int row = b * EDGE + col;
+        if (r0 + row >= rows) continue;
+        char* const at = sums + (wave * ROWS + row) * S::kRow;
 #pragma unroll
         for (int i = 0; i < DB; ++i) {
 #pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int piece = i * 8 + 2 * (e / 4) + hl;
-                *reinterpret_cast<f32x4*>(at + ((piece ^ (l32 & 7)) << 4)) = f32x4{o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]};
+            for (int e = 0; e < NO; e += 4) {
+                const int piece = (i * EDGE + (EDGE == 32 ? 8 * (e / 4) : 0)) / 4 + part;
+                *reinterpret_cast<f32x4*>(at + ((piece ^ (row & 7)) << 4)) = f32x4{o[b][i][e], o[b][i][e + 1], o[b][i][e + 2], o[b][i][e + 3]};
             }
         }
-        if (hl == 0) tops[wave * 32 + l32] = make_float2(m, l);
+        if (part == 0) tops[wave * ROWS + row] = make_float2(m[b], l[b]);
     }
     if constexpr (NW > 1) {
         __syncthreads();
@@ -286,13 +467,13 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT)) void attentionKv4Tiles(Kv
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
     constexpr int LPR = DT <= 64 ? 16 : DT <= 128 ? 32 : 64, SIDE = 64 / LPR;   // lanes of a row, rows side by side
-    const int piece = ln % LPR;
-    for (int row = wave * SIDE + ln / LPR; row < min(32, rows - r0); row += NW * SIDE) {
+    const int piece = ln % LPR, d0 = piece * 4 < DT ? elementsAt(piece / 4) : -1, d = d0 + piece % 4 * 4;
+    for (int row = wave * SIDE + ln / LPR; row < min(ROWS, rows - r0); row += NW * SIDE) {
         float2 ml[NW];
         float top = kLowest, sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < NW; ++w) {
-            ml[w] = tops[w * 32 + row];
+            ml[w] = tops[w * ROWS + row];
             top = fmaxf(top, ml[w].x);
         }
         f32x4 v = {};
@@ -300,23 +481,26 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT)) void attentionKv4Tiles(Kv
         for (int w = 0; w < NW; ++w) {
             const float keep = NW == 1 ? 1.0f : __builtin_amdgcn_exp2f(ml[w].x - top);
             sum += ml[w].y * keep;
-            if (piece * 4 < DT) v += *reinterpret_cast<const f32x4*>(sums + (w * 32 + row) * S::kRow + ((piece ^ (row & 7)) << 4)) * keep;
+            if (d0 >= 0) v += *reinterpret_cast<const f32x4*>(sums + (w * ROWS + row) * S::kRow + ((piece ^ (row & 7)) << 4)) * keep;
         }
         const int t = tokenOf(r0 + row), h = headOf(r0 + row, t);
         const int64_t at = (s.q0 + token0 + t) * p.heads + h;
+        if (a.parts > 0 && split == 0) {   // ranges that this row does not have
+            for (int n = splits + piece; n < a.parts; n += LPR) a.ml[static_cast<int64_t>(n) * p.q_rows * p.heads + at] = make_float2(kLowest, 0.0f);
+        }
         if (piece == 0) {
             if (a.parts > 0) a.ml[static_cast<int64_t>(split) * p.q_rows * p.heads + at] = make_float2(top, sum);
             else if (p.lse != nullptr) p.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
         }
-        if (piece * 4 >= p.dim) continue;
+        if (d0 < 0) continue;
         if (a.parts > 0) {
-            *reinterpret_cast<f32x4*>(a.acc + (static_cast<int64_t>(split) * p.q_rows * p.heads + at) * p.dim + piece * 4) = v;
+            *reinterpret_cast<f32x4*>(a.acc + (static_cast<int64_t>(split) * p.q_rows * p.heads + at) * p.dim + d) = v;
         } else {
             const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
             Vec4<T> out;
 #pragma unroll
             for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(v[e] * inv);
-            *reinterpret_cast<Vec4<T>*>(static_cast<T*>(p.out) + (s.q0 + token0 + t) * p.out_stride + static_cast<int64_t>(h) * p.dim + piece * 4) = out;
+            *reinterpret_cast<Vec4<T>*>(static_cast<T*>(p.out) + (s.q0 + token0 + t) * p.out_stride + static_cast<int64_t>(h) * p.dim + d) = out;
         }
     }
 }
