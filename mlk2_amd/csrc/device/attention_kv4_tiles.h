@@ -90,10 +90,10 @@ struct Kv4Tiles {
     static constexpr int kHalf = 32 * kPitch, kStage = 2 * kHalf + 256;     // a tile's keys (or values); with the scales
     static constexpr int kLoads = kHalf / 1024;                             // of 64 pieces, for keys and again for values
     static constexpr int kPerTile = 2 * kLoads + 1;
-    static constexpr int kStages = ROWS == 16 ? 3 : 4;                      // three times four waves of 16 rows fit a compute unit
+    static constexpr int kStages = 3;                                       // three times four waves fit a compute unit
     static constexpr int kRing = kStage * kStages;
     static constexpr int kRow = DT * 4;                                     // bytes of a row of results
-    static constexpr int kJoin = ROWS * (kRow + 8);
+    static constexpr int kJoin = 16 * (kRow + 8);                           // sixteen rows at a time
     static constexpr int kLds = NW * (kRing > kJoin ? kRing : kJoin);
     static_assert(kPerTile * (kStages - 1) <= 63, "the loads waited on by number fit the counter");
 
@@ -114,8 +114,8 @@ struct Kv4Tiles {
     /// Waits until at most `ahead` tiles of this wave's loads are in flight, and no
     /// read of LDS.
     static __device__ __forceinline__ void wait(int ahead) {
-        if (kStages > 3 && ahead >= 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(2 * kPerTile) : "memory");
-        else if (ahead >= 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kPerTile) : "memory");
+        static_assert(kStages == 3, "");
+        if (ahead >= 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kPerTile) : "memory");
         else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     }
 };
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT, ROWS)) void attentionKv4Ti
     for (int it = first; it < end; it += NW) {
         const char* const tile = ldsTiles + wave * S::kRing + taken;
         taken = taken == (S::kStages - 1) * S::kStage ? 0 : taken + S::kStage;
-        S::wait(it + 2 * NW < end ? 2 : it + NW < end ? 1 : 0);
+        S::wait(it + NW < end ? 1 : 0);
         // Into the place of the tile before, whose values are in their sums.
         if (it + (S::kStages - 1) * NW < end) load(it + (S::kStages - 1) * NW);
         F32<NO> x[QB][KB] = {};
@@ -439,68 +439,77 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT, ROWS)) void attentionKv4Ti
         }
     }
 
-    // The waves' sums by rows through LDS, 16 bytes a lane, joined on the way out.
-    if constexpr (NW > 1) __syncthreads();   // all are done with their tiles
+    // The waves' sums by rows through LDS, 16 rows at a time and 16 bytes a lane,
+    // joined on the way out.
     char* const sums = ldsTiles;
-    float2* const tops = reinterpret_cast<float2*>(ldsTiles + NW * ROWS * S::kRow);
-#pragma unroll
-    for (int b = 0; b < QB; ++b) {
-        l[b] = sumOf<EDGE>(l[b]);
-        const int row = b * EDGE + col;
-        if (r0 + row >= rows) continue;
-        char* const at = sums + (wave * ROWS + row) * S::kRow;
-#pragma unroll
-        for (int i = 0; i < DB; ++i) {
-#pragma unroll
-            for (int e = 0; e < NO; e += 4) {
-                const int piece = (i * EDGE + (EDGE == 32 ? 8 * (e / 4) : 0)) / 4 + part;
-                *reinterpret_cast<f32x4*>(at + ((piece ^ (row & 7)) << 4)) = f32x4{o[b][i][e], o[b][i][e + 1], o[b][i][e + 2], o[b][i][e + 3]};
-            }
-        }
-        if (part == 0) tops[wave * ROWS + row] = make_float2(m[b], l[b]);
-    }
-    if constexpr (NW > 1) {
-        __syncthreads();
-    } else {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-    }
+    float2* const tops = reinterpret_cast<float2*>(ldsTiles + NW * 16 * S::kRow);
     constexpr int LPR = DT <= 64 ? 16 : DT <= 128 ? 32 : 64, SIDE = 64 / LPR;   // lanes of a row, rows side by side
     const int piece = ln % LPR, d0 = piece * 4 < DT ? elementsAt(piece / 4) : -1, d = d0 + piece % 4 * 4;
-    for (int row = wave * SIDE + ln / LPR; row < min(ROWS, rows - r0); row += NW * SIDE) {
-        float2 ml[NW];
-        float top = kLowest, sum = 0.0f;
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            ml[w] = tops[w * ROWS + row];
-            top = fmaxf(top, ml[w].x);
-        }
-        f32x4 v = {};
-#pragma unroll
-        for (int w = 0; w < NW; ++w) {
-            const float keep = NW == 1 ? 1.0f : __builtin_amdgcn_exp2f(ml[w].x - top);
-            sum += ml[w].y * keep;
-            if (d0 >= 0) v += *reinterpret_cast<const f32x4*>(sums + (w * ROWS + row) * S::kRow + ((piece ^ (row & 7)) << 4)) * keep;
-        }
-        const int t = tokenOf(r0 + row), h = headOf(r0 + row, t);
-        const int64_t at = (s.q0 + token0 + t) * p.heads + h;
-        if (a.parts > 0 && split == 0) {   // ranges that this row does not have
-            for (int n = splits + piece; n < a.parts; n += LPR) a.ml[static_cast<int64_t>(n) * p.q_rows * p.heads + at] = make_float2(kLowest, 0.0f);
-        }
-        if (piece == 0) {
-            if (a.parts > 0) a.ml[static_cast<int64_t>(split) * p.q_rows * p.heads + at] = make_float2(top, sum);
-            else if (p.lse != nullptr) p.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
-        }
-        if (d0 < 0) continue;
-        if (a.parts > 0) {
-            *reinterpret_cast<f32x4*>(a.acc + (static_cast<int64_t>(split) * p.q_rows * p.heads + at) * p.dim + d) = v;
+    auto meet = [] {
+        if constexpr (NW > 1) {
+            __syncthreads();
         } else {
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            Vec4<T> out;
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        }
+    };
 #pragma unroll
-            for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(v[e] * inv);
-            *reinterpret_cast<Vec4<T>*>(static_cast<T*>(p.out) + (s.q0 + token0 + t) * p.out_stride + static_cast<int64_t>(h) * p.dim + d) = out;
+    for (int b = 0; b < QB; ++b) l[b] = sumOf<EDGE>(l[b]);
+#pragma unroll
+    for (int row0 = 0; row0 < ROWS; row0 += 16) {
+        if (r0 + row0 >= rows) break;
+        meet();   // all are done with what lay there
+        constexpr int kBlocks = EDGE == 16 ? 16 : 32;
+        const int b = row0 / kBlocks;
+        const int row = EDGE == 16 ? col : b * 32 + col - row0;   // of the sixteen
+        if (row >= 0 && row < 16 && r0 + row0 + row < rows) {
+            char* const at = sums + (wave * 16 + row) * S::kRow;
+#pragma unroll
+            for (int i = 0; i < DB; ++i) {
+#pragma unroll
+                for (int e = 0; e < NO; e += 4) {
+                    const int to = (i * EDGE + (EDGE == 32 ? 8 * (e / 4) : 0)) / 4 + part;
+                    *reinterpret_cast<f32x4*>(at + ((to ^ (row & 7)) << 4)) = f32x4{o[b][i][e], o[b][i][e + 1], o[b][i][e + 2], o[b][i][e + 3]};
+                }
+            }
+            if (part == 0) tops[wave * 16 + row] = make_float2(m[b], l[b]);
+        }
+        meet();
+        for (int at16 = wave * SIDE + ln / LPR; at16 < min(16, rows - r0 - row0); at16 += NW * SIDE) {
+            float2 ml[NW];
+            float top = kLowest, sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                ml[w] = tops[w * 16 + at16];
+                top = fmaxf(top, ml[w].x);
+            }
+            f32x4 v = {};
+#pragma unroll
+            for (int w = 0; w < NW; ++w) {
+                const float keep = NW == 1 ? 1.0f : __builtin_amdgcn_exp2f(ml[w].x - top);
+                sum += ml[w].y * keep;
+                if (d0 >= 0) v += *reinterpret_cast<const f32x4*>(sums + (w * 16 + at16) * S::kRow + ((piece ^ (at16 & 7)) << 4)) * keep;
+            }
+            const int r = r0 + row0 + at16, t = tokenOf(r), h = headOf(r, t);
+            const int64_t at = (s.q0 + token0 + t) * p.heads + h;
+            if (a.parts > 0 && split == 0) {   // ranges that this row does not have
+                for (int n = splits + piece; n < a.parts; n += LPR) a.ml[static_cast<int64_t>(n) * p.q_rows * p.heads + at] = make_float2(kLowest, 0.0f);
+            }
+            if (piece == 0) {
+                if (a.parts > 0) a.ml[static_cast<int64_t>(split) * p.q_rows * p.heads + at] = make_float2(top, sum);
+                else if (p.lse != nullptr) p.lse[at] = sum == 0.0f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
+            }
+            if (d0 < 0) continue;
+            if (a.parts > 0) {
+                *reinterpret_cast<f32x4*>(a.acc + (static_cast<int64_t>(split) * p.q_rows * p.heads + at) * p.dim + d) = v;
+            } else {
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                Vec4<T> out;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(v[e] * inv);
+                *reinterpret_cast<Vec4<T>*>(static_cast<T*>(p.out) + (s.q0 + token0 + t) * p.out_stride + static_cast<int64_t>(h) * p.dim + d) = out;
+            }
         }
     }
 }
