@@ -20,7 +20,6 @@ namespace {
 using i32x4 = int __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = 64;     // bytes of k that an instruction takes
-constexpr int kStages = 4;    // steps in LDS
 
 __device__ __align__(16) const uint32_t kZero16[4] = {0u, 0u, 0u, 0u};
 
@@ -199,18 +198,20 @@ struct TileArgs {
 };
 
 /// A tile of WM x WN waves of MT x NT products of 16 x 16 each, over steps of 64
-/// bytes of k through a ring of four in LDS.
+/// bytes of k through a ring of kStages in LDS.
 ///
-/// Rows of a and b, whole 16-byte pieces at 16 bytes, go straight to LDS, three
-/// steps ahead. Rows past the last repeat it, pieces past k are zeros.
+/// Rows of a and b, whole 16-byte pieces at 16 bytes, go straight to LDS, all but
+/// one of the ring's steps ahead. The smaller tiles have longer rings, as they have
+/// to ask for as many bytes to keep memory busy: 64 x 16384 of k = 4096 by 64 x 64
+/// in 17.4 us with a ring of four, 14.4 with eight. Rows past the last repeat it, pieces past k are zeros.
 ///
 /// LDS holds 64-byte rows, piece c of row r at c ^ (r / 4 % 4): a fragment's
 /// read takes one piece of 16 rows at a time, which then lie in all banks. In
 /// each step the products go in two halves: while the first runs, the second's
 /// rows of a are read; while the second runs, the next step's fragments are read
-/// and the loads of the step three ahead are asked for, in a fixed order, a memory
+/// and a later step's loads are asked for, in a fixed order, a memory
 /// instruction behind every other product or so.
-template <typename T, int WM, int WN, int MT, int NT>
+template <typename T, int WM, int WN, int MT, int NT, int kStages>
 __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) {
     constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
     constexpr int kStage = (BM + BN) * kStep, LOADS = (BM + BN) / 16 / NW, HM = MT / 2;
@@ -259,12 +260,13 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
     i32x4 acc[MT][NT] = {};
     const uint32_t turn = (g ^ (l16 >> 2)) << 4;
     const uint32_t atA = lds0 + (wm * MT * 16 + l16) * kStep + turn, atB = lds0 + (BM + wn * NT * 16 + l16) * kStep + turn;
-    const uint32_t atA2 = atA + 2 * kStage, atB2 = atB + 2 * kStage;   // an instruction's offset holds 16 bits
+    constexpr int HS = kStages / 2;
+    const uint32_t atA2 = atA + HS * kStage, atB2 = atB + HS * kStage;   // an instruction's offset holds 16 bits
     auto readA = [&](int slot, int i) {
-        return *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>((slot < 2 ? atA : atA2) + static_cast<uint32_t>((slot & 1) * kStage + i * 16 * kStep));
+        return *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>((slot < HS ? atA : atA2) + static_cast<uint32_t>(slot % HS * kStage + i * 16 * kStep));
     };
     auto readB = [&](int slot, int i) {
-        return *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>((slot < 2 ? atB : atB2) + static_cast<uint32_t>((slot & 1) * kStage + i * 16 * kStep));
+        return *reinterpret_cast<const __attribute__((address_space(3))) i32x4*>((slot < HS ? atB : atB2) + static_cast<uint32_t>(slot % HS * kStage + i * 16 * kStep));
     };
     // Waits for all of this wave's loads but those of `later` steps.
     auto landed = [&](auto later) {
@@ -285,7 +287,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
     // Step s in slot q.
     auto step = [&](int s, const int q, i32x4 (&bCur)[NT], i32x4 (&bNext)[NT], auto ends) __attribute__((always_inline)) {
         constexpr int N = HM * NT;
-        const int next = (q + 1) & 3;
+        const int next = (q + 1) % kStages;
 #pragma unroll
         for (int x = 0; x < N; ++x) {
             const int i = x / NT, j = (i & 1) != 0 ? NT - 1 - x % NT : x % NT;
@@ -297,7 +299,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
             __builtin_amdgcn_sched_barrier(0);
         }
         // Step s + 1 is in LDS; every wave is past step s - 1, whose slot is free.
-        landed([] { return 1; });
+        landed([] { return kStages - 3; });
         __builtin_amdgcn_sched_barrier(0);
         constexpr int READS = NT + HM;   // B 0, A 0, the other Bs, the other As
 #pragma unroll
@@ -314,24 +316,25 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
             }
 #pragma unroll
             for (int l = 0; l < LOADS; ++l) {
-                if ((2 * l + 1) * N / (2 * LOADS) == x) issue(s + kStages - 1, (q + 3) & 3, l, ends);
+                if ((2 * l + 1) * N / (2 * LOADS) == x) issue(s + kStages - 1, (q + kStages - 1) % kStages, l, ends);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
     };
     int s = 0;
-    auto four = [&](auto ends) __attribute__((always_inline)) {
-        step(s, 0, bX, bY, ends);
-        step(s + 1, 1, bY, bX, ends);
-        step(s + 2, 2, bX, bY, ends);
-        step(s + 3, 3, bY, bX, ends);
-        s += 4;
+    // The slots' steps, from s on.
+    auto round = [&](auto ends) __attribute__((always_inline)) {
+#pragma unroll
+        for (int q = 0; q < kStages; q += 2) {
+            if (ends() && s + q >= steps) break;
+            step(s + q, q, bX, bY, ends);
+            if (ends() && s + q + 1 >= steps) break;
+            step(s + q + 1, q + 1, bY, bX, ends);
+        }
+        s += kStages;
     };
-    while (s + 3 + kStages - 1 < steps - 1) four(no);
-    while (s + 4 <= steps) four(yes);
-    if (s < steps) step(s, 0, bX, bY, yes);
-    if (s + 1 < steps) step(s + 1, 1, bY, bX, yes);
-    if (s + 2 < steps) step(s + 2, 2, bX, bY, yes);
+    while (s + 2 * (kStages - 1) < steps - 1) round(no);
+    while (s < steps) round(yes);
     // No load may still be writing LDS, and no wave be reading it, when its rows
     // of results take its place.
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -428,7 +431,14 @@ __global__ __launch_bounds__(256) void matmulI8Join(TileArgs args) {
 }
 
 // --------------------------------------------------------------- launch ----
-enum Form { kFew, kTile64, kTile128, kTile256 };
+enum Form { kFew, kTile64, kTile128x64, kTile128, kTile256 };
+
+/// A tile's rows and columns, and the time of a round of 256 of them, one a unit,
+/// in halves of a microsecond at k = 4096 (measured 10, 13 to 16, 17 to 25, 45 to 60 us).
+struct TileSize {
+    int rows, cols, round;
+};
+constexpr TileSize kTiles[] = {{}, {64, 64, 20}, {128, 64, 30}, {128, 128, 46}, {256, 256, 100}};
 
 struct Plan {
     Form form{kFew};
@@ -461,23 +471,38 @@ Plan planOf(const mlkd_matmul_i8* p, bool room) {
     n.wide = p->ldo * size % 16 == 0 && reinterpret_cast<uintptr_t>(p->out) % 16 == 0;
     // A tile's rows lie 2^32 bytes apart at most.
     n.aligned = p->k % 16 == 0 && rowsAt(p, 16) && std::max(p->lda, p->ldb) < (int64_t{1} << 23);
+    // Few rows go without LDS while reading b is what takes the time: 32 x 8000 of
+    // k = 4096 in 10.1 us there and 11.4 by tiles, 64 x 8000 in 13.9 and 11.5; of
+    // k = 2048 in 8.5 and 7.0, of 1024 in 5.8 and 7.1, but 64 x 12800 of 1024, two
+    // rounds of workgroups, in 10.1 and 5.9; 32 x 2048 of 16384 in 23.3 and 14.0.
+    const bool few = p->m <= 16 || (p->m <= 32 && p->k <= 8192) || (p->m <= 64 && p->k < 2048 && p->n <= 8192) || (p->m <= 64 && !n.aligned);
     // The tiles take rows at 16 bytes: others are copied to such first.
-    n.pack = !n.aligned && p->m > 64 && room;
-    if (p->m <= 64 || !(n.aligned || n.pack)) {
+    n.pack = !n.aligned && !few && room;
+    if (few || !(n.aligned || n.pack)) {
         n.mb = p->m <= 16 ? 1 : p->m <= 32 ? 2 : 4;
         n.aligned = rowsAt(p, 4);
-        n.nb = n.mb == 4 && p->n >= 32 * 200 ? 2 : 1;
+        // 32 of b's rows a workgroup where that still makes 200: 16 x 8000 of k = 4096
+        // in 7.9 us, by 16 in 9.7; 32 x 2048 in 9.6, by 16 in 7.7.
+        n.nb = p->n >= 32 * 200 ? 2 : 1;
         return n;
     }
-    auto tiles = [&](int64_t of) {
-        n.tilesM = (p->m + of - 1) / of;
-        n.tilesN = (p->n + of - 1) / of;
-        return n.tilesM * n.tilesN;
-    };
-    n.form = tiles(256) >= 192 ? kTile256 : tiles(128) >= 192 ? kTile128 : kTile64;
-    const int64_t count = tiles(n.form == kTile256 ? 256 : n.form == kTile128 ? 128 : 64);
-    // Ranges of k of 1024 bytes and more where the tiles leave units idle.
-    if (room) n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / count, p->k / 1024, 32})));
+    // The size whose rounds over 256 units take least: 256 x 4096 of k = 4096 by
+    // 64 x 64 in 10.8 us and 128 x 64 in 12.9; 384 x 4096 in 19.5, 13.1 and, by
+    // 128 x 128, 17.2; 512 x 8192 in 34.9, 30.7 and 25.1; 2560 x 4096 by 128 x 128
+    // in 59.4 and 256 x 256 in 47.3.
+    int64_t best = INT64_MAX;
+    for (Form f : {kTile64, kTile128x64, kTile128, kTile256}) {
+        const int64_t rows = (p->m + kTiles[f].rows - 1) / kTiles[f].rows, cols = (p->n + kTiles[f].cols - 1) / kTiles[f].cols;
+        const int64_t time = (rows * cols + 255) / 256 * kTiles[f].round;
+        if (time >= best) continue;
+        best = time;
+        n.form = f;
+        n.tilesM = rows;
+        n.tilesN = cols;
+    }
+    // Ranges of k of 2048 bytes and more where the tiles leave units idle: 64 x 2048
+    // of k = 16384 in 32.0 us whole, 14.0 in eight; of k = 4096 9.7 either way.
+    if (room) n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / (n.tilesM * n.tilesN), p->k / 2048, 32})));
     return n;
 }
 
@@ -503,10 +528,10 @@ void launchFew(const mlkd_matmul_i8* p, const Plan& n, hipStream_t st) {
     }
 }
 
-template <typename T, int WM, int WN, int MT, int NT>
+template <typename T, int WM, int WN, int MT, int NT, int kStages>
 int launchTiles(const TileArgs& a, hipStream_t st) {
     constexpr int bytes = (WM * MT + WN * NT) * 16 * kStep * kStages;
-    auto* kernel = matmulI8Tiles<T, WM, WN, MT, NT>;
+    auto* kernel = matmulI8Tiles<T, WM, WN, MT, NT, kStages>;
     // Once per process; a function-local static initializes thread-safely.
     static const bool allowed = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
                                                     bytes) == hipSuccess;
@@ -534,9 +559,10 @@ int launch(const mlkd_matmul_i8* p, hipStream_t st) {
         a.p.b = to + p->m * pitch;
         a.p.lda = a.p.ldb = a.p.k = pitch;
     }
-    const int rc = n.form == kTile256   ? launchTiles<T, 4, 2, 4, 8>(a, st)
-                   : n.form == kTile128 ? launchTiles<T, 2, 2, 4, 4>(a, st)
-                                        : launchTiles<T, 2, 2, 2, 2>(a, st);
+    const int rc = n.form == kTile256      ? launchTiles<T, 4, 2, 4, 8, 4>(a, st)
+                   : n.form == kTile128    ? launchTiles<T, 2, 2, 4, 4, 4>(a, st)
+                   : n.form == kTile128x64 ? launchTiles<T, 2, 2, 4, 2, 6>(a, st)
+                                           : launchTiles<T, 2, 2, 2, 2, 8>(a, st);
     if (rc != 0 || n.splits == 1) return rc;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((p->m * a.ldw / 4 + 255) / 256, int64_t{1} << 16)));
     hipLaunchKernelGGL(matmulI8Join<T>, grid, dim3(256), 0, st, a);
@@ -563,7 +589,7 @@ const char* mlkd_matmul_i8_kernel_names(const mlkd_matmul_i8* p) {
         return name.c_str();
     }
     name = std::string(n.pack ? "matmulI8Pack+" : "") + "matmulI8Tiles<" + type +
-           (n.form == kTile256 ? ", 4, 2, 4, 8>" : n.form == kTile128 ? ", 2, 2, 4, 4>" : ", 2, 2, 2, 2>");
+           (n.form == kTile256 ? ", 4, 2, 4, 8, 4>" : n.form == kTile128 ? ", 2, 2, 4, 4, 4>" : n.form == kTile128x64 ? ", 2, 2, 4, 2, 6>" : ", 2, 2, 2, 2, 8>");
     if (n.splits > 1) name += "+matmulI8Join<" + type + ">";
     return name.c_str();
 }

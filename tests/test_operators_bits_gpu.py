@@ -148,6 +148,19 @@ def test_matmul_many_tiles(hip, dtype, m, n, k):
     matmul_case(hip, m, n, k, dtype, bias=True)
 
 
+@pytest.mark.parametrize("m,n,k", [(33, 64, 2048), (64, 130, 2064), (32, 70, 8208), (17, 70, 16384), (40, 8200, 64), (32, 6500, 48), (16, 6400, 80),
+                                   (256, 5120, 80), (250, 5100, 96), (640, 5120, 72), (600, 5100, 144), (2560, 4096, 64), (2500, 4000, 80)])
+def test_matmul_each_tile(hip, m, n, k):
+    matmul_case(hip, m, n, k, "bf16", bias=True)
+
+
+@pytest.mark.parametrize("n", [66, 5120, 9000])
+@pytest.mark.parametrize("m", [66, 250])
+def test_matmul_every_count_of_steps(hip, m, n):
+    for steps in list(range(1, 24)) if n == 66 else (1, 2, 5, 6, 7, 8, 9, 13):
+        matmul_case(hip, m, n, 64 * steps - (16 if steps % 2 else 0), "f32")
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(5, 70, 100), (40, 90, 256), (150, 140, 130), (300, 270, 320)])
 @pytest.mark.parametrize("at,extra", [(dict(a=1, b=3, out=5), 11), (dict(a=16, b=32, out=8), 48), (dict(a=0, b=0, out=0), 16), (dict(a=4, b=8, out=2), 12)])
