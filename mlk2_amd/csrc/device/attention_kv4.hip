@@ -120,10 +120,16 @@ Plan planOf(const mlkd_attention* p) {
     const int64_t blocks = p->sequences * ((each + n.rows - 1) / n.rows), most = rowBlocks(p, n.rows);
     n.waves = n.rows == 32 && blocks * p->kv_heads >= 4096 ? 1 : 4;
     n.units = most;
-    // Where the blocks leave units of the chip idle, three of four waves of 16 rows
-    // or two of 32: dealt out by the keys.
+    // Dealt out by the keys, with a join, over the chip's room: three of four waves
+    // of 16 rows a unit or two of 32. That costs 6 to 10 us (more row blocks, more
+    // parts to join), and a block's keys take 5.5 to 6.5 us a thousand, so it pays
+    // where few blocks have many keys. Heads 32 on 8, dim 128, bf16, all of one
+    // length, whole and dealt: a token over 1024 keys 9.7 and 12.6 us, 2048 15.3 and
+    // 12.7, 8192 46.9 and 14.4; 8 over 2048 15.7 and 14.9; 32 over 4096 35.8 and 41.9;
+    // 32 over 1000 to 8192 59.6 and 50.4; 128 tokens over 1024 14.5 and 25.9, 4096 33.0
+    // and 34.0, 8192 57.1 and 43.2; twice 128 over 8192 59.6 and 67.0.
     const int64_t room = (n.rows == 16 ? 768 : 512) / p->kv_heads;
-    if (p->sequences <= 64 && blocks * 4 <= room * 3 && keys >= 512) {
+    if (p->sequences <= 64 && keys * (room - 2 * blocks) >= 1500 * room) {
         n.units = std::max(room, most + 1);
         n.parts = static_cast<int>(std::min<int64_t>(64, std::max<int64_t>(16, 4 * n.units / p->sequences)));
     }
