@@ -200,10 +200,11 @@ struct TileArgs {
 /// A tile of WM x WN waves of MT x NT products of 16 x 16 each, over steps of 64
 /// bytes of k through a ring of kStages in LDS.
 ///
-/// Rows of a and b, whole 16-byte pieces at 16 bytes, go straight to LDS, all but
-/// one of the ring's steps ahead. The smaller tiles have longer rings, as they have
-/// to ask for as many bytes to keep memory busy: 64 x 16384 of k = 4096 by 64 x 64
-/// in 17.4 us with a ring of four, 14.4 with eight. Rows past the last repeat it, pieces past k are zeros.
+/// Rows of a and b, whole 16-byte pieces at 16 bytes, go straight to LDS, a ring of
+/// steps ahead. The smaller tiles, with less to do a step, have longer rings and ask
+/// for two steps at once, which fetches whole lines: 64 x 8000 of k = 4096 by 64 x 64,
+/// b from memory, takes 24.3 us with a ring of four, 17.4 with one of eight, 15.7 by
+/// two steps. Rows past the last repeat it, pieces past k are zeros.
 ///
 /// LDS holds 64-byte rows, piece c of row r at c ^ (r / 4 % 4): a fragment's
 /// read takes one piece of 16 rows at a time, which then lie in all banks. In
@@ -215,6 +216,8 @@ template <typename T, int WM, int WN, int MT, int NT, int kStages>
 __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) {
     constexpr int NW = WM * WN, BM = WM * MT * 16, BN = WN * NT * 16;
     constexpr int kStage = (BM + BN) * kStep, LOADS = (BM + BN) / 16 / NW, HM = MT / 2;
+    constexpr bool PAIRS = kStages > 4;
+    constexpr int kAhead = kStages - (PAIRS ? 2 : 1);   // the first steps asked for
     static_assert(LOADS * NW * 16 == BM + BN && HM * 2 == MT, "whole loads and halves");
     extern __shared__ __align__(16) char lds[];
     const mlkd_matmul_i8& p = args.p;
@@ -274,17 +277,17 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
         asm volatile("s_barrier" ::: "memory");
     };
 #pragma unroll
-    for (int t = 0; t < kStages - 1; ++t) {
+    for (int t = 0; t < kAhead; ++t) {
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) issue(t, t, j, yes);
     }
-    landed([] { return kStages - 2; });
+    landed([] { return kAhead - 1; });
     i32x4 aLo[HM], aHi[HM], bX[NT], bY[NT];
 #pragma unroll
     for (int i = 0; i < HM; ++i) aLo[i] = readA(0, i);
 #pragma unroll
     for (int i = 0; i < NT; ++i) bX[i] = readB(0, i);
-    // Step s in slot q.
+    // Step s in slot q. In pairs: an even step asks for two, an odd one for none.
     auto step = [&](int s, const int q, i32x4 (&bCur)[NT], i32x4 (&bNext)[NT], auto ends) __attribute__((always_inline)) {
         constexpr int N = HM * NT;
         const int next = (q + 1) % kStages;
@@ -299,7 +302,7 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
             __builtin_amdgcn_sched_barrier(0);
         }
         // Step s + 1 is in LDS; every wave is past step s - 1, whose slot is free.
-        landed([] { return kStages - 3; });
+        landed([] { return kAhead - 2; });   // of two asked for at once, both
         __builtin_amdgcn_sched_barrier(0);
         constexpr int READS = NT + HM;   // B 0, A 0, the other Bs, the other As
 #pragma unroll
@@ -315,8 +318,11 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
                 else aLo[r - NT] = readA(next, r - NT);
             }
 #pragma unroll
-            for (int l = 0; l < LOADS; ++l) {
-                if ((2 * l + 1) * N / (2 * LOADS) == x) issue(s + kStages - 1, (q + kStages - 1) % kStages, l, ends);
+            for (int l = 0; l < (PAIRS ? 2 * LOADS : LOADS); ++l) {
+                constexpr int ALL = PAIRS ? 2 * LOADS : LOADS;
+                const int ahead = PAIRS ? kAhead + l % 2 : kAhead;
+                if ((2 * l + 1) * N / (2 * ALL) != x || (PAIRS && (q & 1) != 0)) continue;
+                issue(s + ahead, (q + ahead) % kStages, PAIRS ? l / 2 : l, ends);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -433,19 +439,19 @@ __global__ __launch_bounds__(256) void matmulI8Join(TileArgs args) {
 // --------------------------------------------------------------- launch ----
 enum Form { kFew, kTile64, kTile128x64, kTile128, kTile256 };
 
-/// A tile's rows and columns, and the time of a round of 256 of them, one a unit,
-/// in halves of a microsecond at k = 4096 (measured 10, 13 to 16, 17 to 25, 45 to 60 us).
+/// A tile's rows and columns, and what a round of 256 of them, one a unit, adds to
+/// the time of k = 4096, in halves of a microsecond.
 struct TileSize {
     int rows, cols, round;
 };
-constexpr TileSize kTiles[] = {{}, {64, 64, 20}, {128, 64, 30}, {128, 128, 46}, {256, 256, 100}};
+constexpr TileSize kTiles[] = {{}, {64, 64, 16}, {128, 64, 25}, {128, 128, 40}, {256, 256, 104}};
 
 struct Plan {
     Form form{kFew};
     bool aligned{false}, wide{false}, pack{false};
     int mb{1}, nb{1};      // kFew: 16 rows of a, of b, a workgroup
     int64_t tilesM{0}, tilesN{0};
-    int splits{1};
+    int splits{1}, stages{4};
 };
 
 int outBytes(const mlkd_matmul_i8* p) { return p->dtype == MLKD_F32 ? 4 : 2; }
@@ -471,25 +477,26 @@ Plan planOf(const mlkd_matmul_i8* p, bool room) {
     n.wide = p->ldo * size % 16 == 0 && reinterpret_cast<uintptr_t>(p->out) % 16 == 0;
     // A tile's rows lie 2^32 bytes apart at most.
     n.aligned = p->k % 16 == 0 && rowsAt(p, 16) && std::max(p->lda, p->ldb) < (int64_t{1} << 23);
-    // Few rows go without LDS while reading b is what takes the time: 32 x 8000 of
-    // k = 4096 in 10.1 us there and 11.4 by tiles, 64 x 8000 in 13.9 and 11.5; of
-    // k = 2048 in 8.5 and 7.0, of 1024 in 5.8 and 7.1, but 64 x 12800 of 1024, two
-    // rounds of workgroups, in 10.1 and 5.9; 32 x 2048 of 16384 in 23.3 and 14.0.
-    const bool few = p->m <= 16 || (p->m <= 32 && p->k <= 8192) || (p->m <= 64 && p->k < 2048 && p->n <= 8192) || (p->m <= 64 && !n.aligned);
+    // (Here and below: us, b from memory rather than a cache, bf16 out.) Few rows go
+    // without LDS while that is faster, in one round of workgroups of 32 columns.
+    // Without and with, 32 x 8000 of k = 4096: 11.1 and 13.5, 32 x 2048 of 8192 13.6
+    // and 11.7, 32 x 16384 of 4096 20.0 and 17.6; 64 x 8000 of 4096 14.9 and 13.6, of
+    // 2048 9.4 and 9.6, 64 x 2048 of 2048 7.6 and 9.2, 64 x 12800 of 1024 11.4 and 7.2.
+    const bool few = p->m <= 16 || (p->m <= 64 && (!n.aligned || (p->n <= 8192 && (p->m <= 32 ? p->k < 8192 : p->k <= 2048))));
     // The tiles take rows at 16 bytes: others are copied to such first.
     n.pack = !n.aligned && !few && room;
     if (few || !(n.aligned || n.pack)) {
         n.mb = p->m <= 16 ? 1 : p->m <= 32 ? 2 : 4;
         n.aligned = rowsAt(p, 4);
         // 32 of b's rows a workgroup where that still makes 200: 16 x 8000 of k = 4096
-        // in 7.9 us, by 16 in 9.7; 32 x 2048 in 9.6, by 16 in 7.7.
+        // in 9.3, by 16 in 10.5; 16 x 4096 in 8.4, by 16 in 6.7.
         n.nb = p->n >= 32 * 200 ? 2 : 1;
         return n;
     }
-    // The size whose rounds over 256 units take least: 256 x 4096 of k = 4096 by
-    // 64 x 64 in 10.8 us and 128 x 64 in 12.9; 384 x 4096 in 19.5, 13.1 and, by
-    // 128 x 128, 17.2; 512 x 8192 in 34.9, 30.7 and 25.1; 2560 x 4096 by 128 x 128
-    // in 59.4 and 256 x 256 in 47.3.
+    // The size whose rounds over 256 units take least. Of k = 4096, 256 x 4096 by
+    // 64 x 64 takes 14.7 and by 128 x 64 20.3; 512 x 4096 22.8, 20.5 and by 128 x 128
+    // 27.6; 512 x 8192 42.2, 34.9 and 28.9; 2048 x 4096 by 128 x 64 60.6, by 128 x 128
+    // 50.5 and by 256 x 256 54.7; 2560 x 4096 63.5 and 56.6, 4096^2 98.8 and 65.2.
     int64_t best = INT64_MAX;
     for (Form f : {kTile64, kTile128x64, kTile128, kTile256}) {
         const int64_t rows = (p->m + kTiles[f].rows - 1) / kTiles[f].rows, cols = (p->n + kTiles[f].cols - 1) / kTiles[f].cols;
@@ -499,10 +506,14 @@ Plan planOf(const mlkd_matmul_i8* p, bool room) {
         n.form = f;
         n.tilesM = rows;
         n.tilesN = cols;
+        // A ring of 128 x 128 fits LDS once with six steps, twice with four: 512 x 8192
+        // 28.9 and 32.8, 2048 x 4096, two rounds, 54.1 and 50.5.
+        n.stages = f == kTile64 ? 8 : f == kTile128x64 || (f == kTile128 && rows * cols <= 256) ? 6 : 4;
     }
-    // Ranges of k of 2048 bytes and more where the tiles leave units idle: 64 x 2048
-    // of k = 16384 in 32.0 us whole, 14.0 in eight; of k = 4096 9.7 either way.
-    if (room) n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / (n.tilesM * n.tilesN), p->k / 2048, 32})));
+    // Ranges of k of 1024 bytes and more where the tiles leave units idle, from
+    // k = 4096 on: 64 x 4096 of 2048 takes 9.2 whole and 10.7 in two, of 4096 14.5 and,
+    // in four, 11.3, 64 x 2048 of 8192 24.1 and, in eight, 12.3.
+    if (room && p->k >= 4096) n.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({256 / (n.tilesM * n.tilesN), p->k / 1024, 32})));
     return n;
 }
 
@@ -560,7 +571,7 @@ int launch(const mlkd_matmul_i8* p, hipStream_t st) {
         a.p.lda = a.p.ldb = a.p.k = pitch;
     }
     const int rc = n.form == kTile256      ? launchTiles<T, 4, 2, 4, 8, 4>(a, st)
-                   : n.form == kTile128    ? launchTiles<T, 2, 2, 4, 4, 4>(a, st)
+                   : n.form == kTile128    ? n.stages == 6 ? launchTiles<T, 2, 2, 4, 4, 6>(a, st) : launchTiles<T, 2, 2, 4, 4, 4>(a, st)
                    : n.form == kTile128x64 ? launchTiles<T, 2, 2, 4, 2, 6>(a, st)
                                            : launchTiles<T, 2, 2, 2, 2, 8>(a, st);
     if (rc != 0 || n.splits == 1) return rc;
@@ -589,7 +600,8 @@ const char* mlkd_matmul_i8_kernel_names(const mlkd_matmul_i8* p) {
         return name.c_str();
     }
     name = std::string(n.pack ? "matmulI8Pack+" : "") + "matmulI8Tiles<" + type +
-           (n.form == kTile256 ? ", 4, 2, 4, 8, 4>" : n.form == kTile128 ? ", 2, 2, 4, 4, 4>" : n.form == kTile128x64 ? ", 2, 2, 4, 2, 6>" : ", 2, 2, 2, 2, 8>");
+           (n.form == kTile256 ? ", 4, 2, 4, 8, " : n.form == kTile128 ? ", 2, 2, 4, 4, " : n.form == kTile128x64 ? ", 2, 2, 4, 2, " : ", 2, 2, 2, 2, ") +
+           std::to_string(n.stages) + ">";
     if (n.splits > 1) name += "+matmulI8Join<" + type + ">";
     return name.c_str();
 }

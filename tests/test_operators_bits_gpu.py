@@ -149,7 +149,7 @@ def test_matmul_many_tiles(hip, dtype, m, n, k):
 
 
 @pytest.mark.parametrize("m,n,k", [(33, 64, 2048), (64, 130, 2064), (32, 70, 8208), (17, 70, 16384), (40, 8200, 64), (32, 6500, 48), (16, 6400, 80),
-                                   (256, 5120, 80), (250, 5100, 96), (640, 5120, 72), (600, 5100, 144), (2560, 4096, 64), (2500, 4000, 80)])
+                                   (256, 5120, 80), (250, 5100, 96), (640, 5120, 72), (600, 5100, 144), (2040, 4090, 400), (2560, 4096, 64), (2500, 4000, 80)])
 def test_matmul_each_tile(hip, m, n, k):
     matmul_case(hip, m, n, k, "bf16", bias=True)
 
