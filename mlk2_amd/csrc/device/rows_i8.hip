@@ -67,14 +67,14 @@ __global__ __launch_bounds__(LANES < 256 ? 256 : LANES) void quantizeRows(mlkd_q
             __syncthreads();
         }
         const Scale s = mlk::scaleOf(top, 127.0f);
-        const float inv = 1.0f / s.s;
         int8_t* codes = p.codes + r * p.codes_stride;
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             const int c = (i * LANES + lane) * E;
+            uint32_t words[E / 4];
+            mlk::codesI8(v[i], s, words);
             int8_t q[E];
-#pragma unroll
-            for (int e = 0; e < E; ++e) q[e] = static_cast<int8_t>(mlk::codeI8(v[i][e], s, inv));
+            __builtin_memcpy(q, words, E);
             if (c + E <= cols) {
                 __builtin_memcpy(codes + c, q, E);
             } else {
