@@ -74,64 +74,52 @@ __global__ __launch_bounds__(256) void kv4RowsAny(mlkd_kv4_rows p) {
 
 /// Eight elements a lane, LANES lanes a head of up to 8 LANES elements, of any
 /// alignment: the heads of a token's k, then those of its v, side by side. A
-/// head is read once and written once. Bound by memory: a thread has TURNS heads
-/// in flight, and asks for them before it knows their slots or how many tokens
-/// there are (what comes is dropped where those say so).
-template <typename T, int LANES, int TURNS, bool STORE>
+/// head is read once and written once. Bound by memory: a store of 8191 tokens of
+/// 8 heads of 128 in f16, 42 MB, takes 16 to 17 us and their load into f32, 76 MB,
+/// 16; 64 tokens 3.6 and 2.9. x is asked for before its slot or the count of tokens
+/// is known (what comes is dropped where those say so), which had it wait three
+/// times. Two heads a thread in flight were as fast for many tokens and took 5.3 us
+/// for 64.
+template <typename T, int LANES, bool STORE>
 __global__ __launch_bounds__(256) void kv4Rows(mlkd_kv4_rows p) {
     const int lane = threadIdx.x % LANES, c = lane * 8, bytes = p.dim / 2;
     const uint32_t heads = p.kv_heads, most = static_cast<uint32_t>(p.tokens) * 2 * heads, step = 256 / LANES;
-    // A wave's lanes take as many turns, as their exchange asks.
-    for (uint32_t n0 = blockIdx.x * TURNS * step + threadIdx.x / LANES; n0 / step * step < most; n0 += gridDim.x * TURNS * step) {
-        float v[TURNS][8], s[TURNS];
-        uint32_t word[TURNS];
-        int64_t row[TURNS];
-        bool held[TURNS];
-        T* x[TURNS];
-        uint8_t* codes[TURNS];
-        float* scale[TURNS];
+    // A workgroup's lanes take as many turns, as their exchange asks.
+    for (uint32_t n0 = blockIdx.x * step; n0 < most; n0 += gridDim.x * step) {
+        const uint32_t own = n0 + threadIdx.x / LANES, n = min(own, most - 1), part = n / heads, h = n - part * heads, t = part >> 1;
+        const bool value = (part & 1) != 0;
+        T* x = static_cast<T*>(value ? p.v : p.k) + t * (value ? p.v_stride : p.k_stride) + static_cast<int64_t>(h) * p.dim + c;
+        T raw[8] = {};
+        if (STORE && c < p.dim) __builtin_memcpy(raw, x, sizeof(raw));
+        const int64_t row = p.slots != nullptr ? p.slots[t] : static_cast<int64_t>(t);
+        const bool held = own < static_cast<uint32_t>(tokensOf(p)) * 2 * heads && row >= 0 && row < p.cache_rows && c < p.dim;
+        uint8_t* codes = (value ? p.v_codes : p.k_codes) + row * (value ? p.v_codes_stride : p.k_codes_stride) + static_cast<int64_t>(h) * bytes + c / 2;
+        float* scale = (value ? p.v_scale : p.k_scale) + row * p.kv_heads + h;
+        if constexpr (STORE) {
+            float v[8];
+            uint32_t top = 0;
 #pragma unroll
-        for (int u = 0; u < TURNS; ++u) {
-            const uint32_t n = min(n0 + u * step, most - 1), part = n / heads, h = n - part * heads, t = part >> 1;
-            const bool value = (part & 1) != 0;
-            row[u] = p.slots != nullptr ? p.slots[t] : static_cast<int64_t>(t);
-            held[u] = row[u] >= 0 && row[u] < p.cache_rows && c < p.dim && n0 + u * step < most;
-            x[u] = static_cast<T*>(value ? p.v : p.k) + t * (value ? p.v_stride : p.k_stride) + static_cast<int64_t>(h) * p.dim + c;
-            codes[u] = (value ? p.v_codes : p.k_codes) + row[u] * (value ? p.v_codes_stride : p.k_codes_stride) + static_cast<int64_t>(h) * bytes + c / 2;
-            scale[u] = (value ? p.v_scale : p.k_scale) + row[u] * p.kv_heads + h;
-            if constexpr (STORE) {
-                T raw[8] = {};
-                if (c < p.dim) __builtin_memcpy(raw, x[u], sizeof(raw));
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[u][e] = static_cast<float>(raw[e]);
-            } else if (held[u]) {
-                s[u] = *scale[u];
-                __builtin_memcpy(&word[u], codes[u], 4);
+            for (int e = 0; e < 8; ++e) {
+                v[e] = static_cast<float>(raw[e]);
+                top = max(top, mlk::magnitude(v[e]));
             }
-        }
-        const uint32_t all = static_cast<uint32_t>(tokensOf(p)) * 2 * heads;
 #pragma unroll
-        for (int u = 0; u < TURNS; ++u) {
-            held[u] = held[u] && n0 + u * step < all;
-            if constexpr (STORE) {
-                uint32_t top = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = max(top, mlk::magnitude(v[u][e]));
-#pragma unroll
-                for (int d = LANES / 2; d > 0; d >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d, 64)));
-                const Scale of = mlk::scaleOf(top, 6.0f);
-                const uint32_t out = top < 0x7f800000u ? mlk::codesFp4(v[u], of) : 0u;
-                if (held[u]) {
-                    __builtin_memcpy(codes[u], &out, 4);
-                    if (lane == 0) *scale[u] = of.stored;
-                }
-            } else if (held[u]) {
-                const mlk::F32x2 y[4] = {mlk::numbersOf<0>(word[u]), mlk::numbersOf<1>(word[u]), mlk::numbersOf<2>(word[u]), mlk::numbersOf<3>(word[u])};
-                T out[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) out[e] = static_cast<T>(y[e / 2][e % 2] * s[u]);
-                __builtin_memcpy(x[u], out, sizeof(out));
+            for (int d = LANES / 2; d > 0; d >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d, 64)));
+            const Scale s = mlk::scaleOf(top, 6.0f);
+            const uint32_t word = top < 0x7f800000u ? mlk::codesFp4(v, s) : 0u;
+            if (held) {
+                __builtin_memcpy(codes, &word, 4);
+                if (lane == 0) *scale = s.stored;
             }
+        } else if (held) {
+            const float s = *scale;
+            uint32_t word;
+            __builtin_memcpy(&word, codes, 4);
+            const mlk::F32x2 v[4] = {mlk::numbersOf<0>(word), mlk::numbersOf<1>(word), mlk::numbersOf<2>(word), mlk::numbersOf<3>(word)};
+            T out[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[e] = static_cast<T>(v[e / 2][e % 2] * s);
+            __builtin_memcpy(x, out, sizeof(out));
         }
     }
 }
@@ -141,17 +129,12 @@ bool rowsApply(const mlkd_kv4_rows* p) { return p->dim % 8 == 0 && p->tokens * p
 
 int lanesOf(const mlkd_kv4_rows* p) { return p->dim <= 32 ? 4 : p->dim <= 64 ? 8 : p->dim <= 128 ? 16 : 32; }
 
-constexpr int kTurns = 1;
-
 template <typename T, bool STORE>
 void launchRows(const mlkd_kv4_rows* p, hipStream_t st) {
     const int lanes = lanesOf(p);
-    const int64_t heads = p->tokens * p->kv_heads * 2, each = kTurns * 256 / lanes;
+    const int64_t heads = p->tokens * p->kv_heads * 2, each = 256 / lanes;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((heads + each - 1) / each, int64_t{1} << 16)));
-    auto* kernel = lanes == 4   ? kv4Rows<T, 4, kTurns, STORE>
-                   : lanes == 8 ? kv4Rows<T, 8, kTurns, STORE>
-                   : lanes == 16 ? kv4Rows<T, 16, kTurns, STORE>
-                                 : kv4Rows<T, 32, kTurns, STORE>;
+    auto* kernel = lanes == 4 ? kv4Rows<T, 4, STORE> : lanes == 8 ? kv4Rows<T, 8, STORE> : lanes == 16 ? kv4Rows<T, 16, STORE> : kv4Rows<T, 32, STORE>;
     hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, *p);
 }
 
@@ -160,7 +143,7 @@ const char* typeName(int dtype) { return dtype == MLKD_F32 ? "float" : dtype == 
 template <bool STORE>
 const char* kernelName(const mlkd_kv4_rows* p) {
     static thread_local std::string name;
-    name = rowsApply(p) ? std::string("kv4Rows<") + typeName(p->dtype) + ", " + std::to_string(lanesOf(p)) + ", " + std::to_string(kTurns)
+    name = rowsApply(p) ? std::string("kv4Rows<") + typeName(p->dtype) + ", " + std::to_string(lanesOf(p))
                         : std::string("kv4RowsAny<") + typeName(p->dtype);
     name += STORE ? ", true>" : ", false>";
     return name.c_str();
