@@ -325,7 +325,8 @@ int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* bind
  * cache, read as it is. q and out are f16, bf16 or f32. Scores are sums of q
  * times codes in f32, then times the key's scale; a weight times the value's
  * scale is rounded to bf16 for bf16 rows, carried as two bf16 parts for f16 ones
- * and three for f32 ones, its sum and lse are of f32 weights. 32 single tokens
+ * and three for f32 ones, its sum and lse are of f32 weights. The sums that have
+ * to stay in f32's range are attention's, with codes times scales for values. 32 single tokens
  * over 1000 to 8192 keys (32 heads on 8 of 128, bf16) take 51 us, 4 prompts of
  * 125 to 1000 tokens behind up to 4000 200 us. As attention's, its form and its
  * workspace follow the buffers' sizes; the matrix-core kernels take dims of

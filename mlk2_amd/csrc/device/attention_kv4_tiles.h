@@ -1,5 +1,5 @@
-// Attention over a cache in 4 bits on matrix cores: a wave 32 query rows, over
-// tiles of 32 keys.
+// Attention over a cache in 4 bits on matrix cores: a wave 16 or 32 query rows,
+// over tiles of 32 keys.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -130,8 +130,8 @@ struct Kv4Unit {
 /// Unit `unit` of `units`, which are dealt out by the keys there are: a sequence's
 /// row blocks are split into as many ranges, `parts` at most, as make all of them
 /// about equally long, so that all units of a launch run at once and end together
-/// (32 single tokens over 1000 to 8192 keys 50.4 us, whole 59.6). For 64 sequences at most, a
-/// lane each, and more units than there are row blocks.
+/// (32 single tokens over 1000 to 8192 keys 50.4 us, whole 59.6). For 64 sequences at
+/// most, a lane each, and more units than there are row blocks.
 template <int ROWS>
 __device__ __forceinline__ bool dealtUnit(const mlkd_attention& p, int group, int unit, int units, int parts, Kv4Unit& u) {
     const int ln = threadIdx.x & 63;
@@ -180,9 +180,10 @@ constexpr int kv4Waves(int dt, int rows) {
 /// overlap little (1700 cycles for 32 rows and keys of 128; 4 prompts of 125 to 1000
 /// tokens behind up to 4000, 32 heads on 8: 200 us, 0.70 PFLOP/s), single tokens by
 /// memory and the start (32 over 1000 to 8192 keys, 165 MB: 46 us, 3.5 TB/s; all of
-/// 8192: 4.8 TB/s whole). The products run on the codes as numbers, which either 16-bit type holds
-/// exactly: a key's scale goes to its scores, a value's to its weights. Codes come
-/// straight to LDS, three tiles ahead; a word of a key's row is eight elements of
+/// 8192: 4.8 TB/s whole). The products run on the codes as numbers, which either
+/// 16-bit type holds exactly: a key's scale goes to its scores, a value's to its
+/// weights. Codes come
+/// straight to LDS, two tiles ahead; a word of a key's row is eight elements of
 /// the product's operand as it lies. Values are read transposed, 4 bits at a time:
 /// a lane gets a column's numbers of the keys whose weights it holds, in their
 /// order.
