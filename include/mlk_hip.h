@@ -323,10 +323,12 @@ int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* bind
  * attention_kv4 (attention's operands with k_codes, k_scale, v_codes, v_scale
  * for k and v, and its attrs, without prefixes): attention over rows of such a
  * cache, read as it is. q and out are f16, bf16 or f32. Scores are sums of q
- * times codes in f32, then times the key's scale; a weight times the value's
- * scale is rounded to bf16 for bf16 rows, carried as two bf16 parts for f16 ones
- * and three for f32 ones, its sum and lse are of f32 weights. The sums that have
- * to stay in f32's range are attention's, with codes times scales for values. 32 single tokens
+ * times codes in f32, a row of q taken times a power of two where it is far from
+ * one, then times the key's scale; a weight times the value's scale is rounded to
+ * bf16 for bf16 rows, carried as two bf16 parts for f16 ones and three for f32
+ * ones (half a step of itself, or 2^-134 where that is more), its sum and lse are
+ * of f32 weights. The sums that have to stay in f32's range are attention's, with
+ * codes times scales for keys and values. 32 single tokens
  * over 1000 to 8192 keys (32 heads on 8 of 128, bf16) take 51 us, 4 prompts of
  * 125 to 1000 tokens behind up to 4000 200 us. As attention's, its form and its
  * workspace follow the buffers' sizes; the matrix-core kernels take dims of

@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "attention_kv4_tiles.h"
@@ -20,11 +21,10 @@ using mlk::spanOf;
 /// key for the scores, then a lane per output column. 32 single tokens over 1000 to
 /// 8192 keys of dim 120 take 5.2 ms, 2048 tokens 8.7.
 template <typename T>
-__global__ __launch_bounds__(256) void attentionKv4Rows(mlkd_attention_kv4 args) {
-    const mlkd_attention& p = args.a;
+__global__ __launch_bounds__(256) void attentionKv4Rows(mlk::Kv4Args args) {
+    const mlkd_attention& p = args.t.p;
     const int ln = threadIdx.x & 63, d = p.dim, group = p.heads / p.kv_heads;
     const int64_t waves = static_cast<int64_t>(gridDim.x) * 4, rows = p.q_rows * p.heads;
-    const float scale = static_cast<float>(p.scale * 1.4426950408889634);
     for (int64_t r = blockIdx.x * int64_t{4} + (threadIdx.x >> 6); r < rows; r += waves) {
         const int64_t t = r / p.heads;
         const int h = static_cast<int>(r % p.heads), g = h / group;
@@ -39,6 +39,12 @@ __global__ __launch_bounds__(256) void attentionKv4Rows(mlkd_attention_kv4 args)
             q[i] = ln + 64 * i < d ? static_cast<float>(qr[ln + 64 * i]) : 0.0f;
             acc[i] = 0.0f;
         }
+        // A row's elements are taken at a size below 1, so that sums of them times codes
+        // stay in range, and 2^lacks comes with the key's scale.
+        const float size = waveMax(fmaxf(fmaxf(fabsf(q[0]), fabsf(q[1])), fmaxf(fabsf(q[2]), fabsf(q[3]))));
+        const int by = size < INFINITY ? __builtin_amdgcn_frexp_expf(size) : 0, lacks = by + args.up;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = __builtin_amdgcn_ldexpf(q[i], -by);
         auto query = [&](int c) { return lane(c < 64 ? q[0] : c < 128 ? q[1] : c < 192 ? q[2] : q[3], c & 63); };
         float m = -INFINITY, l = 0.0f;
         const uint8_t* k = static_cast<const uint8_t*>(p.k) + s.k0 * p.k_stride + g * (d / 2);
@@ -53,7 +59,8 @@ __global__ __launch_bounds__(256) void attentionKv4Rows(mlkd_attention_kv4 args)
                 x += query(2 * c) * n[0];
                 x += query(2 * c + 1) * n[1];
             }
-            x *= args.k_scale[at] * scale;
+            const float ks = args.k_scale[at];
+            x = __builtin_amdgcn_ldexpf(x * (__builtin_amdgcn_frexp_mantf(ks) * args.c), __builtin_amdgcn_frexp_expf(ks) + lacks);
             const float vs = args.v_scale[at];
             if (ln >= seen) x = -INFINITY;
             const float top = fmaxf(m, waveMax(x));
@@ -173,12 +180,20 @@ int launchForm(const mlk::Kv4Args& a, const Plan& n, hipStream_t st) {
     return launchTiles<T, DT, 32, 1>(a, st);
 }
 
-template <typename T>
-int launchPlan(const mlkd_attention_kv4* p, const Plan& n, hipStream_t st) {
+mlk::Kv4Args argsOf(const mlkd_attention_kv4* p) {
     mlk::Kv4Args a{};
     a.t.p = p->a;
     a.k_scale = p->k_scale;
     a.v_scale = p->v_scale;
+    a.c = static_cast<float>(p->a.scale * 1.4426950408889634);
+    a.up = std::fabs(a.c) >= 2.0f ? std::ilogb(a.c) : 0;
+    a.c = std::ldexp(a.c, -a.up);
+    return a;
+}
+
+template <typename T>
+int launchPlan(const mlkd_attention_kv4* p, const Plan& n, hipStream_t st) {
+    mlk::Kv4Args a = argsOf(p);
     a.t.parts = n.parts;
     if (n.units >= (int64_t{1} << 30)) return -1;
     a.units = static_cast<int>(n.units);
@@ -239,7 +254,7 @@ int mlkd_launch_attention_kv4(const mlkd_attention_kv4* p, void* stream) {
     }
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>((rows + 3) / 4, int64_t{1} << 20)));
     auto* kernel = p->a.dtype == MLKD_F32 ? attentionKv4Rows<float> : p->a.dtype == MLKD_F16 ? attentionKv4Rows<_Float16> : attentionKv4Rows<__bf16>;
-    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, *p);
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, argsOf(p));
     return hipGetLastError() == hipSuccess ? 0 : MLKD_RT_LAUNCH;
 }
 

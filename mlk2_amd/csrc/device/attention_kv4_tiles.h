@@ -21,6 +21,8 @@ struct Kv4Args {
     TileArgs t;                      // p's k and v: the codes, strides in bytes
     const float *k_scale, *v_scale;  // [kv_rows, kv_heads]
     int units;                       // row blocks, or with parts their key ranges, of one head at most
+    float c;                         // scale log2 e = c 2^up, c below 2 in size: a key's scale times c is in range,
+    int up;                          // and the queries take 2^up
 };
 
 /// The numbers of a word's eight codes, exact in either type.
@@ -73,6 +75,37 @@ __device__ __forceinline__ float sumOf(float v) {
     return v + otherHalf(v);
 }
 
+/// Whether some of the queries that a lane takes, eight at a time, may be too far from
+/// one for sums of them times codes, or for their parts.
+template <typename T>
+struct Sizes;
+template <>
+struct Sizes<__bf16> {
+    float squares[2] = {};
+    __device__ __forceinline__ void take(Piece<__bf16> v) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bf16x2 two = {v[2 * i], v[2 * i + 1]};
+            squares[i & 1] = __builtin_amdgcn_fdot2_f32_bf16(two, two, squares[i & 1], false);
+        }
+    }
+    __device__ __forceinline__ bool far() const { return squares[0] + squares[1] > 0x1p120f; }
+};
+template <>
+struct Sizes<_Float16> {
+    __device__ __forceinline__ void take(Piece<_Float16>) {}
+    __device__ __forceinline__ bool far() const { return false; }
+};
+template <>
+struct Sizes<float> {
+    float top = 0.0f;
+    __device__ __forceinline__ void take(float __attribute__((ext_vector_type(8))) v) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));
+    }
+    __device__ __forceinline__ bool far() const { return top > 0.0f && !(top >= 0x1p-60f && top <= 0x1p100f); }
+};
+
 /// NW waves with the same ROWS query rows, tiles of 32 keys in turn; their sums are
 /// joined at the end.
 template <typename T, int DT, int ROWS, int NW>
@@ -96,6 +129,10 @@ struct Kv4Tiles {
     static constexpr int kJoin = 16 * (kRow + 8);                           // sixteen rows at a time
     static constexpr int kLds = NW * (kRing > kJoin ? kRing : kJoin);
     static_assert(kPerTile * (kStages - 1) <= 63, "the loads waited on by number fit the counter");
+    // Exponents between which a row's largest query is left as it is: sums of 256 of
+    // them times 6 stay in f32's range, and the last of three bf16 parts in bf16's. f16
+    // itself holds less.
+    static constexpr int kLeast = std::is_same_v<T, _Float16> ? -24 : -60, kMost = std::is_same_v<T, _Float16> ? 16 : 100;
 
     /// Turn of row j's pieces, so that the rows that are read at a time lie in
     /// different banks: 16 from one on, or fours of them eight or sixteen apart.
@@ -168,10 +205,12 @@ __device__ __forceinline__ bool dealtUnit(const mlkd_attention& p, int group, in
     return true;
 }
 
-/// Waves of a SIMD that the registers have to hold.
+/// Waves of a SIMD that the registers have to hold. f32 rows by 32 of dims up to 96
+/// keep to 256 registers with it (3 x 129 of dim 64 over 777 12.9 us, 14.0 without; 2
+/// x 500 of 96 over 1000 44.6, and 68.3 with one wave); of 256 they spill 35.
 template <typename T>
 constexpr int kv4Waves(int dt, int rows) {
-    return rows == 16 ? (std::is_same_v<T, float> || dt > 128 ? 2 : 3) : std::is_same_v<T, float> || dt > 128 ? 1 : 2;
+    return rows == 16 ? (std::is_same_v<T, float> || dt > 128 ? 2 : 3) : dt > (std::is_same_v<T, float> ? 96 : 128) ? 1 : 2;
 }
 
 /// One row block of one key/value head. With S^T = K Q^T a lane holds some keys'
@@ -189,8 +228,9 @@ constexpr int kv4Waves(int dt, int rows) {
 /// order.
 ///
 /// What is rounded: a weight times its value's scale to bf16 (f16 rows: to two
-/// bf16 parts, 16 bits, f32 rows three), half a step of itself; f32 queries are
-/// three bf16 parts, exactly. Scores, weights, their sum and out's sums are f32.
+/// bf16 parts, 16 bits, f32 rows three), half a step of itself or, below 2^-126,
+/// 2^-134; f32 queries are three bf16 parts, exactly down to 2^-50 of the row's largest.
+/// Scores, weights, their sum and out's sums are f32.
 /// The maximum that the weights are relative to follows the running one only when
 /// that has grown by 2^8.
 template <typename T, int DT, int ROWS, int NW>
@@ -272,30 +312,59 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT, ROWS)) void attentionKv4Ti
 
     // Queries: step i takes the eight elements whose codes a lane's i-th word holds.
     Piece<Q> q[S::kPartsQ][QB][KS];
-#pragma unroll
-    for (int b = 0; b < QB; ++b) {
+    using V8 = T __attribute__((ext_vector_type(8)));
+    auto queries = [&](int b, auto take) __attribute__((always_inline)) {
         const int r = min(r0 + b * EDGE + col, rows - 1), t = tokenOf(r);
         const T* row = static_cast<const T*>(p.q) + (s.q0 + token0 + t) * p.q_stride + static_cast<int64_t>(headOf(r, t)) * p.dim;
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
             const int place = part * KS + i, d = elementsAt(place / 2);
-            using V8 = T __attribute__((ext_vector_type(8)));
             V8 v = {};
             if (d >= 0) v = *reinterpret_cast<const V8*>(row + d + place % 2 * 8);
-            if constexpr (S::kPartsQ == 1) {
-                q[0][b][i] = v;
-            } else {
+            take(i, v);
+        }
+    };
+    auto hold = [&](int b, int i, V8 v) __attribute__((always_inline)) {
+        if constexpr (S::kPartsQ == 1) {
+            q[0][b][i] = v;
+        } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    float left = v[e];
+            for (int e = 0; e < 8; ++e) {
+                float left = v[e];
 #pragma unroll
-                    for (int n = 0; n < S::kPartsQ; ++n) {
-                        q[n][b][i][e] = static_cast<Q>(left);
-                        left -= static_cast<float>(q[n][b][i][e]);
-                    }
+                for (int n = 0; n < S::kPartsQ; ++n) {
+                    q[n][b][i][e] = static_cast<Q>(left);
+                    left -= static_cast<float>(q[n][b][i][e]);
                 }
             }
         }
+    };
+    static_assert(QB == 1, "c is of a lane's one query");
+    float c = args.c;
+    Sizes<T> sizes;
+    queries(0, [&](int i, V8 v) {
+        sizes.take(v);
+        hold(0, i, v);
+    });
+    // Queries far from one are taken times a power of two, a row's all alike, and their
+    // scores' c times its reciprocal: c is a lane's own, so that tiles are as they were
+    // (a token over 100 keys 4.96 us for 4.84, prompts 1 % more).
+    if (__builtin_expect(args.up != 0 || __any(sizes.far()), 0)) {
+        float top = 0.0f;
+        queries(0, [&](int, V8 v) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(static_cast<float>(v[e])));
+        });
+        top = largestOf<EDGE>(top);
+        const int size = __builtin_amdgcn_frexp_expf(top);
+        const bool some = top > 0.0f && top < INFINITY;
+        const int by = some ? min(max(args.up, S::kLeast - size), S::kMost - size) : args.up;
+        queries(0, [&](int i, V8 v) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = static_cast<T>(__builtin_amdgcn_ldexpf(static_cast<float>(v[e]), by));
+            hold(0, i, v);
+        });
+        c = __builtin_amdgcn_ldexpf(c, args.up - by);
     }
     // They are taken here: the compiler knows nothing of the loads to LDS and would
     // wait for these, and so for all, in every tile.
@@ -311,7 +380,6 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT, ROWS)) void attentionKv4Ti
             }
         }
     }
-    const float c = static_cast<float>(p.scale * 1.4426950408889634);
 
     // A lane's words of key block kb: those of row kb EDGE + col from `part` on.
     constexpr int WB = KS * 4;   // bytes of them

@@ -1,0 +1,178 @@
+"""Calls of the operators in 8 and 4 bits at the ends of their ranges:
+magnitudes of queries, keys, values and scales, scores far from zero, long tails."""
+import numpy as np
+import pytest
+
+from mlk2_amd import operators as op
+from operators_bits_ref import load_kv4, store_kv4
+from operators_ref import TINY, U, U32, attention, rounded
+from test_operators_gpu import TYPES, close, run
+
+pytestmark = pytest.mark.gpu
+
+# Row blocks of 16 and 32 rows, one key range and several, a wave to a row:
+# (heads, key/value heads, queries, keys).
+SHAPES = {"token": (4, 2, [1, 1], [70, 33]), "ranges": (4, 1, [1, 1], [9000, 40]), "prompt": (4, 2, [40, 3], [90, 3])}
+
+
+def heads_of(values):
+    """A cache of these heads: codes and scales, and the numbers they stand for."""
+    codes, scale = store_kv4(values)
+    return codes, scale, load_kv4(codes, scale)
+
+
+# ------------------------------------------------------------ attention_kv4 --
+# Queries and keys whose products are about 1 while one of them is far from it.
+FAR = {"large": (1e37, 1e-37), "largest": (2e38, 1e-38), "small": (1e-37, 1e37), "smallest": (1e-40, 1e38), "f16 large": (4e4, 1e-4),
+       "f16 small": (1e-6, 1e6), "f16 smallest": (1e-7, 1e30)}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256, 34])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("name", FAR)
+def test_queries_far_from_one(hip, dtype, d, shape, name):
+    # Every other row of a block has queries of the magnitude that makes scores of
+    # about 1 with these keys, the others of about 1 (f16: of a tenth).
+    if dtype == "f16" and not name.startswith("f16"):
+        return
+    size_q, size_k = FAR[name]
+    h, g, q_lens, k_lens = SHAPES[shape]
+    rng = np.random.default_rng(d)
+    t, rows = sum(q_lens), sum(k_lens)
+    size = np.where(np.arange(t * h).reshape(t, h, 1) % 2 == 0, size_q, min(1.0, 0.1 * size_q))
+    q = rounded(rng.standard_normal((t, h, d)).clip(-1.5, 1.5) * size, dtype)
+    k_codes, k_scale, k = heads_of((rng.standard_normal((rows, g, d)).clip(-3, 3) * size_k).astype(np.float32).astype(np.float64))
+    v_codes, v_scale, v = heads_of(rounded(rng.standard_normal((rows, g, d)), "bf16"))
+    offsets, start = np.concatenate([[0], np.cumsum(q_lens)]), np.concatenate([[0], np.cumsum(k_lens)[:-1]])
+    km = op.attention_kv4_module(t, kv_rows=rows, sequences=len(q_lens), heads=h, kv_heads=g, dim=d, dtype=dtype, lse=True)
+    got = run(hip, km, {"q": q, "k_codes": k_codes, "k_scale": k_scale, "v_codes": v_codes, "v_scale": v_scale, "q_offsets": offsets,
+                        "kv_start": start, "kv_len": k_lens})
+    out, bound, lse, lse_bound, _ = attention(q, k, v, offsets, start, k_lens, scale=d ** -0.5, causal=True, dtype=dtype)
+    close(got["out"], out, bound, "out")
+    close(got["lse"], lse, lse_bound, "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 34])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("scale,size_q,size_k", [(1e20, 1e-18, 1e-2), (1e20, 1e-36, 1e16), (-1e3, 1e-5, 1e1), (5e2, 1e4, 1e-7), (1e2, 1.0, 1e-2),
+                                                 (1e3, 1e-4, 1e37), (1e-20, 1e3, 1e17), (1e-20, 1e36, 1e-16)])
+def test_scales_far_from_one(hip, dtype, d, shape, scale, size_q, size_k):
+    # A scale of any size, where scale q k^T is about 1, or one key's is far the largest.
+    if dtype == "f16" and not 6e-6 <= size_q <= 1e4:
+        return
+    h, g, q_lens, k_lens = SHAPES[shape]
+    rng = np.random.default_rng(d)
+    t, rows = sum(q_lens), sum(k_lens)
+    q = rounded(rng.standard_normal((t, h, d)) * size_q, dtype)
+    q[0] = 0.0
+    k_codes, k_scale, k = heads_of((rng.standard_normal((rows, g, d)).clip(-3, 3) * size_k).astype(np.float32).astype(np.float64))
+    v_codes, v_scale, v = heads_of(rounded(rng.standard_normal((rows, g, d)), "bf16"))
+    offsets, start = np.concatenate([[0], np.cumsum(q_lens)]), np.concatenate([[0], np.cumsum(k_lens)[:-1]])
+    km = op.attention_kv4_module(t, kv_rows=rows, sequences=len(q_lens), heads=h, kv_heads=g, dim=d, dtype=dtype, scale=scale, lse=True)
+    got = run(hip, km, {"q": q, "k_codes": k_codes, "k_scale": k_scale, "v_codes": v_codes, "v_scale": v_scale, "q_offsets": offsets,
+                        "kv_start": start, "kv_len": k_lens})
+    out, bound, lse, lse_bound, _ = attention(q, k, v, offsets, start, k_lens, scale=scale, causal=True, dtype=dtype)
+    close(got["lse"], lse, lse_bound, "lse")
+    # Scores so large that a rounding of one decides who has the weight are left to the lse.
+    sure = np.abs(scale) * size_q * size_k * d < 1e5
+    assert np.isfinite(got["out"]).all()
+    if sure:
+        close(got["out"], out, bound, "out")
+    else:
+        close(got["out"][0], out[0], bound[0], "out")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256, 34])
+@pytest.mark.parametrize("shape", ["token", "ranges", "prompt"])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("size", [23, 26, 31, 40, 60])
+def test_scores_far_from_zero(hip, dtype, d, shape, sign, size):
+    """Scores of about 2^size: the keys with the largest share the weight.
+
+    Scores are one product, the same for the same operands, and a sixteenth and
+    more apart, which is 2^19 and more; so the result is a mean of n values, each
+    product and sum within 2^-24 n, the weights and out rounded once."""
+    h, g, q_lens, k_lens = SHAPES[shape]
+    rng = np.random.default_rng(d)
+    t, rows = sum(q_lens), sum(k_lens)
+    q = np.zeros((t, h, d))
+    q[..., 1] = 1.375 * 2.0 ** 8
+    k_scale = rng.choice([1.25, 1.3828125, 1.5] if sign > 0 else [1.8671875, 1.99], (rows, g)).astype(np.float32).astype(np.float64)
+    best, start = [], np.concatenate([[0], np.cumsum(k_lens)[:-1]])
+    for s, n, m in zip(start, k_lens, q_lens):
+        best.append(s + np.sort(rng.choice(n - m + 1, min(7, n - m + 1), replace=False)))
+        k_scale[best[-1]] = 1.7109375
+    k_codes = np.zeros((rows, g, d // 2))
+    k_codes[..., 0] = (7 if sign > 0 else 15) << 4   # element 1: 6, the others 0
+    v_codes, v_scale, v = heads_of(rounded(rng.standard_normal((rows, g, d)), "bf16"))
+    scale = 2.0 ** (size - 12)
+    offsets = np.concatenate([[0], np.cumsum(q_lens)])
+    km = op.attention_kv4_module(t, kv_rows=rows, sequences=len(q_lens), heads=h, kv_heads=g, dim=d, dtype=dtype, scale=scale, lse=True)
+    got = run(hip, km, {"q": q, "k_codes": k_codes, "k_scale": k_scale, "v_codes": v_codes, "v_scale": v_scale, "q_offsets": offsets,
+                        "kv_start": start, "kv_len": k_lens})
+    for i, at in enumerate(best):
+        rows_of = slice(offsets[i], offsets[i + 1])
+        want, size_of = (np.repeat(x.mean(0), h // g, 0) for x in (v[at], np.abs(v[at])))
+        close(got["out"][rows_of], np.broadcast_to(want, got["out"][rows_of].shape),
+              (U[dtype] + 64 * U32) * size_of + U[dtype] * np.abs(want) + TINY[dtype], "out")
+        lse = sign * 1.375 * 2.0 ** 8 * 6 * 1.7109375 * scale + np.log(len(at))
+        close(got["lse"][rows_of], np.full(got["lse"][rows_of].shape, lse), 8 * U32 * abs(lse), "lse")
+
+
+TAILS = {"token": (4, 2, 1, 300), "ranges": (4, 1, 1, 20000), "prompt": (4, 2, 40, 900)}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("name", TAILS)
+def test_tail_behind_one_key(hip, dtype, d, name):
+    """One key with the largest score and no value, all others 2^-26 of it, with
+    values about 1: what is left of a tail in rounded weights.
+
+    Bound, scores being exact products: a weight times its value's scale is within
+    half a step of the type's of itself, its exponential and the running sums
+    within (n + 64) 2^-24, and out is rounded once."""
+    h, g, nq, nk = TAILS[name]
+    rng = np.random.default_rng(nk)
+    q = np.zeros((nq, h, d))
+    q[..., 0] = 1.0
+    k_codes, k_scale = np.zeros((nk, g, d // 2)), np.full((nk, g), 3.0)
+    k_codes[..., 0] = 15   # -6 * 3
+    k_codes[nk // 3] = 0
+    v = 0.5 + rng.random((nk, g, d))
+    v[nk // 3] = 0.0
+    v_codes, v_scale, v = heads_of(rounded(v, "bf16"))
+    km = op.attention_kv4_module(nq, kv_rows=nk, sequences=1, heads=h, kv_heads=g, dim=d, dtype=dtype, causal=False, scale=1.0, lse=True)
+    got = run(hip, km, {"q": q, "k_codes": k_codes, "k_scale": k_scale, "v_codes": v_codes, "v_scale": v_scale, "q_offsets": [0, nq],
+                        "kv_start": [0], "kv_len": [nk]})
+    w = np.full(nk, np.exp(-18.0))
+    w[nk // 3] = 1.0
+    want = np.repeat((w[:, None, None] * v).sum(0) / w.sum(), h // g, 0)
+    sum_error = (nk + 64) * U32
+    close(got["out"], np.broadcast_to(want, got["out"].shape), want * (2 * U[dtype] + 2 * sum_error) + TINY[dtype], "out")
+    close(got["lse"], np.full((nq, h), np.log(w.sum())), sum_error + 2.0 ** -22, "lse")
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256, 34])
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("size", [1e-20, 1e-26, 1e-32, 1e-36, 1e20, 1e32, 1e35])
+def test_values_far_from_one(hip, dtype, d, shape, size):
+    # Values all of one magnitude. A weight times its value's scale is off by half a
+    # step of bf16's least, 2^-134, where it is that small: 6 times that for a key's
+    # largest code, over a sum of weights of 1 at least.
+    h, g, q_lens, k_lens = SHAPES[shape]
+    rng = np.random.default_rng(d)
+    t, rows = sum(q_lens), sum(k_lens)
+    q = rounded(rng.standard_normal((t, h, d)), dtype)
+    k_codes, k_scale, k = heads_of(rounded(rng.standard_normal((rows, g, d)), "bf16"))
+    v_codes, v_scale, v = heads_of((rng.standard_normal((rows, g, d)).clip(-3, 3) * size).astype(np.float32).astype(np.float64))
+    offsets, start = np.concatenate([[0], np.cumsum(q_lens)]), np.concatenate([[0], np.cumsum(k_lens)[:-1]])
+    km = op.attention_kv4_module(t, kv_rows=rows, sequences=len(q_lens), heads=h, kv_heads=g, dim=d, dtype=dtype, lse=True)
+    got = run(hip, km, {"q": q, "k_codes": k_codes, "k_scale": k_scale, "v_codes": v_codes, "v_scale": v_scale, "q_offsets": offsets,
+                        "kv_start": start, "kv_len": k_lens})
+    out, bound, *_ = attention(q, k, v, offsets, start, k_lens, scale=d ** -0.5, causal=True, dtype=dtype)
+    close(got["out"], out, bound + max(k_lens) * 6 * 2.0 ** -134, "out")
