@@ -300,7 +300,8 @@ int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* bind
  * out[t, n] = (sum over k < inner of a[t, k] b[n, k]) * a_scale[t] * b_scale[n]
  * + bias[n] for n < cols. a [rows, inner] and b [cols, inner] are i8 and may
  * hold -128; scales and bias are f32; out is f16, bf16 or f32. Sums are exact
- * (inner <= 131071), times the scales in f32, rounded once to out. Rows and
+ * (inner <= 131071), times the scales in f32, of any sizes whose product with
+ * them is in its range, rounded once to out. Rows and
  * cols <= 2^30. 8192^3 takes 0.45 ms, 4096^3 65 us; one row by 4096 x 4096 5.6, 64
  * by 8000 x 4096 13.7 (b from memory). Rows whose addresses or `inner` are no
  * multiples of 16 bytes are copied to aligned ones in the workspace first where

@@ -72,9 +72,19 @@ __device__ __forceinline__ i32x4 take(const Window& w, const int8_t* from, const
     return v;
 }
 
+/// A row's scale as 2^-91 to 2^90 times a power of two, which comes last: a sum times
+/// the one and the other operand's scale is in f32's range then where the result is.
+struct RowScale {
+    float s, rest;
+};
+__device__ __forceinline__ RowScale rowScale(float s) {
+    const int e = __builtin_amdgcn_frexp_expf(s), by = e - max(-90, min(e, 90));
+    return {__builtin_amdgcn_ldexpf(s, -by), __builtin_amdgcn_ldexpf(1.0f, by)};
+}
+
 template <typename T>
-__device__ __forceinline__ T scaled(int sum, float sa, float sb, float bias, bool has) {
-    float v = static_cast<float>(sum) * sa * sb;
+__device__ __forceinline__ T scaled(int sum, const RowScale& sa, float sb, float bias, bool has) {
+    float v = static_cast<float>(sum) * sa.s * sb * sa.rest;
     if (has) v += bias;
     return static_cast<T>(v);
 }
@@ -82,7 +92,7 @@ __device__ __forceinline__ T scaled(int sum, float sa, float sb, float bias, boo
 /// Columns n .. n + 3 of row m from their sums, n a multiple of 4. `wide`: rows
 /// of whole 16-byte pieces at 16 bytes.
 template <typename T>
-__device__ __forceinline__ void store4(const mlkd_matmul_i8& p, int64_t m, int64_t n, i32x4 sum, float sa, bool wide) {
+__device__ __forceinline__ void store4(const mlkd_matmul_i8& p, int64_t m, int64_t n, i32x4 sum, const RowScale& sa, bool wide) {
     using V = T __attribute__((ext_vector_type(4)));
     T* out = static_cast<T*>(p.out) + m * p.ldo + n;
     const bool has = p.bias != nullptr;
@@ -183,7 +193,7 @@ __global__ __launch_bounds__(512) void matmulI8Few(mlkd_matmul_i8 p, int wide) {
 #pragma unroll
             for (int w = 1; w < 8; ++w) sum += sums[w][t][ln];
             const int64_t m = rows + t / NB * 16 + l16, n = n0 + t % NB * 16 + 4 * g;
-            if (m < p.m && n < p.n) store4<T>(p, m, n, sum, p.a_scale[m], wide != 0);
+            if (m < p.m && n < p.n) store4<T>(p, m, n, sum, rowScale(p.a_scale[m]), wide != 0);
         }
         __syncthreads();
     }
@@ -396,9 +406,9 @@ __global__ __launch_bounds__(WM * WN * 64, 2) void matmulI8Tiles(TileArgs args) 
         store(0, true, [&](int, int, i32x4 sum) { return sum; }, [&](int64_t m) { return args.work + (split * p.m + m) * args.ldw; });
         return;
     }
-    float sa[MT];
+    RowScale sa[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) sa[i] = p.a_scale[min(m0 + i * 16 + l16, p.m - 1)];
+    for (int i = 0; i < MT; ++i) sa[i] = rowScale(p.a_scale[min(m0 + i * 16 + l16, p.m - 1)]);
     store(static_cast<T>(0.0f), args.wide != 0, [&](int i, int j, i32x4 sum) {
         T __attribute__((ext_vector_type(4))) v;
 #pragma unroll
@@ -432,7 +442,7 @@ __global__ __launch_bounds__(256) void matmulI8Join(TileArgs args) {
         i32x4 sum = {};
         for (int s = 0; s < args.splits; ++s) sum += reinterpret_cast<const i32x4*>(args.work)[s * total + i];
         const int64_t m = i / quads;
-        store4<T>(p, m, (i - m * quads) * 4, sum, p.a_scale[m], args.wide != 0);
+        store4<T>(p, m, (i - m * quads) * 4, sum, rowScale(p.a_scale[m]), args.wide != 0);
     }
 }
 

@@ -176,3 +176,27 @@ def test_values_far_from_one(hip, dtype, d, shape, size):
                         "kv_start": start, "kv_len": k_lens})
     out, bound, *_ = attention(q, k, v, offsets, start, k_lens, scale=d ** -0.5, causal=True, dtype=dtype)
     close(got["out"], out, bound + max(k_lens) * 6 * 2.0 ** -134, "out")
+
+
+# ---------------------------------------------------------------- matmul_i8 --
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 256), (40, 90, 512), (70, 130, 4096), (70, 130, 8192), (300, 260, 320)])
+@pytest.mark.parametrize("size_a,size_b", [(1e36, 1e-30), (1e-30, 1e36), (1e-40, 1e37), (1e37, 1e-40), (1e-20, 1e-10), (1e10, 1e15)])
+def test_matmul_scales_far_from_one(hip, dtype, m, n, k, size_a, size_b):
+    # Rows of about 1e38, or 1e-38, whose products with the other operand's are in
+    # range. Three roundings of f32, then one to the type.
+    rng = np.random.default_rng(m + k)
+    a, b = rng.integers(-127, 128, (m, k)), rng.integers(-127, 128, (n, k))
+    a[0] = 0
+    sa, sb = ((size * (0.5 + rng.random(x))).astype(np.float32).astype(np.float64) for size, x in ((size_a, m), (size_b, n)))
+    got = run(hip, op.matmul_i8_module(m, n, k, dtype=dtype), {"a": a, "b": b, "a_scale": sa, "b_scale": sb})["out"]
+    want = (a.astype(np.float64) @ b.T.astype(np.float64)) * sa[:, None] * sb
+    close(got, want, (3 * U32 * (1 + U[dtype]) + U[dtype]) * (1 + 4 * U32) * np.abs(want) + TINY["f32"] + TINY[dtype], "out")
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 40, 256), (70, 130, 4096), (300, 260, 320)])
+def test_matmul_sums_of_zero_under_any_scale(hip, m, n, k):
+    a, b = np.zeros((m, k)), np.ones((n, k))
+    for size in (3e38, 1e-45):
+        got = run(hip, op.matmul_i8_module(m, n, k, dtype="f32"), {"a": a, "b": b, "a_scale": np.full(m, size), "b_scale": np.full(n, 3e38)})["out"]
+        assert (got == 0).all()
