@@ -333,8 +333,8 @@ int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* bind
  * over 1000 to 8192 keys (32 heads on 8 of 128, bf16) take 51 us, 4 prompts of
  * 125 to 1000 tokens behind up to 4000 200 us. As attention's, its form and its
  * workspace follow the buffers' sizes; the matrix-core kernels take dims of
- * whole sixteens from 32 on, rows of whole 16-byte pieces and up to 4096
- * sequences, other Calls run a wave to a row (32 over up to 8192 keys at dim
+ * whole sixteens from 32 on, rows of q and out of whole 16-byte pieces, codes whose
+ * rows start at 8 bytes and up to 4096 sequences, other Calls run a wave to a row (32 over up to 8192 keys at dim
  * 120: 5.2 ms; 2048 tokens: 8.7). */
 
 /* ---- launch-form search (fastkernel on the gfx950 kernels) ------------ */

@@ -100,15 +100,16 @@ struct Plan {
     int64_t units{0};
 };
 
-/// The matrix-core kernels take rows of whole 16-byte pieces, and heads of
-/// 32 and more elements in whole sixteens.
+/// The matrix-core kernels take rows of q and out of whole 16-byte pieces, codes at 8
+/// bytes, where their heads lie in any case, and heads of 32 and more elements in whole
+/// sixteens. (Of 16 for codes as well, one kv head of dim 80 ran row by row.)
 bool tilesApply(const mlkd_attention* p) {
     const int size = p->dtype == MLKD_F32 ? 4 : 2;
     // As attention's: a block reads the lengths 64 at a time, rows and keys are
     // counted in 32 bits.
     return p->dim % 16 == 0 && p->dim >= 32 && p->sequences <= 4096 && p->q_rows * (p->heads / p->kv_heads) < (int64_t{1} << 30) &&
            p->kv_rows <= (int64_t{1} << 30) && aligned(p->q, p->q_stride, 16, size) && aligned(p->out, p->out_stride, 16, size) &&
-           aligned(p->k, p->k_stride, 16, 1) && aligned(p->v, p->v_stride, 16, 1);
+           aligned(p->k, p->k_stride, 8, 1) && aligned(p->v, p->v_stride, 8, 1);
 }
 
 int dimOf(int dim) { return dim <= 64 ? 64 : dim <= 96 ? 96 : dim <= 128 ? 128 : 256; }

@@ -46,7 +46,7 @@ they meet it, so that f16 and bf16 run on the matrix cores; their sum is of the
 f32 values. Codes are i8 (``quantize_rows``, ``matmul_i8``) and u8 (the cache's), scales
 f32; a row or head with a value that is not finite has scale NaN and codes 0.
 Buffers' sizes decide how an attention runs, not the lengths in them,
-and rows off 16 bytes or more than 4096 sequences run a wave to a row (see
+and rows off 16 bytes (codes: 8) or more than 4096 sequences run a wave to a row (see
 include/mlk_hip.h).
 """
 from __future__ import annotations
