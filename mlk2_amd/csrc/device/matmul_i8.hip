@@ -452,9 +452,9 @@ enum Form { kFew, kTile64, kTile128x64, kTile128, kTile256 };
 /// A tile's rows and columns, and what a round of 256 of them, one a unit, adds to
 /// the time of k = 4096, in halves of a microsecond.
 struct TileSize {
-    int rows, cols, round;
+    int rows, cols, round, threads;
 };
-constexpr TileSize kTiles[] = {{}, {64, 64, 16}, {128, 64, 25}, {128, 128, 40}, {256, 256, 104}};
+constexpr TileSize kTiles[] = {{}, {64, 64, 16, 256}, {128, 64, 25, 256}, {128, 128, 40, 256}, {256, 256, 104, 512}};
 
 struct Plan {
     Form form{kFew};
@@ -493,9 +493,14 @@ Plan planOf(const mlkd_matmul_i8* p, bool room) {
     // and 11.7, 32 x 16384 of 4096 20.0 and 17.6; 64 x 8000 of 4096 14.9 and 13.6, of
     // 2048 9.4 and 9.6, 64 x 2048 of 2048 7.6 and 9.2, 64 x 12800 of 1024 11.4 and 7.2.
     const bool few = p->m <= 16 || (p->m <= 64 && (!n.aligned || (p->n <= 8192 && (p->m <= 32 ? p->k < 8192 : p->k <= 2048))));
+    // A launch holds fewer than 2^32 threads.
+    auto fits = [&](Form f) {
+        return ((p->m + kTiles[f].rows - 1) / kTiles[f].rows) * ((p->n + kTiles[f].cols - 1) / kTiles[f].cols) < (int64_t{1} << 32) / kTiles[f].threads;
+    };
+    const bool tiles = !few && fits(kTile256);
     // The tiles take rows at 16 bytes: others are copied to such first.
-    n.pack = !n.aligned && !few && room;
-    if (few || !(n.aligned || n.pack)) {
+    n.pack = !n.aligned && tiles && room;
+    if (!tiles || !(n.aligned || n.pack)) {
         n.mb = p->m <= 16 ? 1 : p->m <= 32 ? 2 : 4;
         n.aligned = rowsAt(p, 4);
         // 32 of b's rows a workgroup where that still makes 200: 16 x 8000 of k = 4096
@@ -511,7 +516,7 @@ Plan planOf(const mlkd_matmul_i8* p, bool room) {
     for (Form f : {kTile64, kTile128x64, kTile128, kTile256}) {
         const int64_t rows = (p->m + kTiles[f].rows - 1) / kTiles[f].rows, cols = (p->n + kTiles[f].cols - 1) / kTiles[f].cols;
         const int64_t time = (rows * cols + 255) / 256 * kTiles[f].round;
-        if (time >= best) continue;
+        if (time >= best || !fits(f)) continue;
         best = time;
         n.form = f;
         n.tilesM = rows;
