@@ -23,7 +23,7 @@ constexpr const char* kSlotNames[kOperandSlots] = {
 
 constexpr int64_t kMaxRows = INT32_MAX;   // rows are named by i32 buffers
 constexpr int kMaxDim = 256, kMaxHeads = 4096;
-constexpr int64_t kMaxProduct = int64_t{1} << 30;   // rows and columns of a product in 8 bits: their tiles' threads are counted in 32
+constexpr int64_t kMaxProduct = int64_t{1} << 30;   // rows and columns of a product in 8 bits: its tiles are counted in 32
 constexpr int64_t kMaxInner = (1 << 17) - 1;   // of a product in 8 bits: 2^14 a term, sums below 2^31
 
 int operandCode(Dtype d) {
@@ -424,28 +424,34 @@ void* place(const Step& st, int slot, const std::vector<void*>& ptr, int bytes) 
 
 }  // namespace
 
-bool isOperator(const Step& st) { return st.kind >= StepKind::NormRope; }
+namespace {
 
-Dtype operatorDtype(const KernelModule& km, const Step& st) {
-    const Operand* op = st.oper.op;
-    const int slot = st.kind == StepKind::QuantizeRows ? kOpX
-                     : st.kind == StepKind::MatmulI8   ? kOpOut
-                     : st.kind == StepKind::StoreKv4   ? kOpK
-                     : st.kind == StepKind::LoadKv4    ? kOpKOut
-                                                       : kOpQ;
-    return km.buffers[op[slot].buffer].dtype;
-}
-
-int64_t operatorRows(const Step& st) {
-    const Operand* op = st.oper.op;
-    switch (st.kind) {
-        case StepKind::QuantizeRows: return op[kOpX].rows;
-        case StepKind::StoreKv4: return op[kOpK].rows;
-        case StepKind::LoadKv4: return op[kOpKOut].rows;
-        case StepKind::MatmulI8: return op[kOpOut].rows;
-        default: return op[kOpQ].rows;
+/// The operand whose rows and dtype an operator's results have; -1 for other steps.
+int resultSlot(StepKind kind) {
+    switch (kind) {
+        case StepKind::NormRope:
+        case StepKind::Attention:
+        case StepKind::AttentionKv4: return kOpQ;
+        case StepKind::QuantizeRows: return kOpX;
+        case StepKind::MatmulI8: return kOpOut;
+        case StepKind::StoreKv4: return kOpK;
+        case StepKind::LoadKv4: return kOpKOut;
+        case StepKind::Elementwise:
+        case StepKind::Softmax:
+        case StepKind::Gemm:
+        case StepKind::RowSum:
+        case StepKind::ScoreSoftmax:
+        case StepKind::Nest:
+        case StepKind::Fail: return -1;
     }
+    return -1;
 }
+
+}  // namespace
+
+bool isOperator(const Step& st) { return resultSlot(st.kind) >= 0; }
+Dtype operatorDtype(const KernelModule& km, const Step& st) { return km.buffers[st.oper.op[resultSlot(st.kind)].buffer].dtype; }
+int64_t operatorRows(const Step& st) { return st.oper.op[resultSlot(st.kind)].rows; }
 
 Result<Step> operatorStep(const KernelModule& km, const KernelNode& call) {
     Step st;

@@ -1080,7 +1080,14 @@ void markTemps(const KernelModule& km, const Step& st, std::vector<bool>& need) 
         case StepKind::Nest:
             for (const uint32_t b : st.nestBufs) mark(b);
             break;
-        default:   // Fail, and operators: no temps among their operands
+        case StepKind::NormRope:
+        case StepKind::Attention:
+        case StepKind::QuantizeRows:
+        case StepKind::MatmulI8:
+        case StepKind::StoreKv4:
+        case StepKind::LoadKv4:
+        case StepKind::AttentionKv4:   // no temps among their operands
+        case StepKind::Fail:
             break;
     }
 }
@@ -1116,12 +1123,18 @@ void stepIO(const Step& st, std::vector<uint32_t>& reads, std::vector<uint32_t>&
             reads.push_back(st.bias);
             writes.push_back(st.s);
             break;
-        case StepKind::Fail: break;
-        default:
+        case StepKind::NormRope:
+        case StepKind::Attention:
+        case StepKind::QuantizeRows:
+        case StepKind::MatmulI8:
+        case StepKind::StoreKv4:
+        case StepKind::LoadKv4:
+        case StepKind::AttentionKv4:
             for (int i = 0; i < kOperandSlots; ++i) {
                 if (st.oper.op[i].buffer != kInvalidId) (i < kFirstOpOutput ? reads : writes).push_back(st.oper.op[i].buffer);
             }
             break;
+        case StepKind::Fail: break;
     }
 }
 
@@ -1217,8 +1230,16 @@ std::string policyFor(const KernelModule& km, const std::vector<Step>& steps) {
                 else gemm32 = true;
                 break;
             case StepKind::ScoreSoftmax: score = true; break;
+            case StepKind::NormRope:
+            case StepKind::Attention:
+            case StepKind::QuantizeRows:
+            case StepKind::MatmulI8:
+            case StepKind::StoreKv4:
+            case StepKind::LoadKv4:
+            case StepKind::AttentionKv4:
+                (operatorDtype(km, st) == Dtype::F32 ? oper32 : oper16) = true;
+                break;
             case StepKind::Fail: break;
-            default: (operatorDtype(km, st) == Dtype::F32 ? oper32 : oper16) = true; break;
         }
     }
     bool crossF16 = false;
