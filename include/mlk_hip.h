@@ -417,11 +417,13 @@ int mlkhip_autotune(mlkhip_artifact* a, const mlkhip_binding* binds, int n_binds
  * bound is max(min_bytes / bytes_per_sec, min_ops / ops_per_sec), 0 when a
  * count is unknown (a dynamic extent without dims). bytes_per_sec <= 0
  * takes MI355X HBM (8e12 B/s); ops_per_sec <= 0 takes the datasheet rate
- * of the plan (2.5e15 with an f16 GEMM or score step, 78.6e12 for f64-only
+ * of the plan (5e15 with a product in 8 bits, 2.5e15 with an f16 GEMM or score
+ * step or an attention of 16-bit rows or a 4-bit cache, 78.6e12 for f64-only
  * modules, else 157.3e12). No device needed. mlkhip_autotune reports the
  * same quantities with its winner's gap over the bound, and a launch
  * coverage certificate per step (certifyLaunchCoverage, fast_kernel.cpp:
- * 386-497, restated for the GPU decomposition). */
+ * 386-497, restated for the GPU decomposition; the operators in 8 and 4 bits,
+ * whose grids go by addresses too, name no workgroups). */
 int mlkhip_essential_work(const char* module_json, size_t len, double bytes_per_sec, double ops_per_sec,
                           int64_t* min_bytes, int64_t* min_ops, int* bytes_known, int* ops_known,
                           double* roofline_lower_sec);

@@ -227,9 +227,9 @@ def summary(title: str, art: "be.LoadedKernel", rep: dict) -> List[str]:
     if not rep.get("steps"):
         out.append("no step declares more than one launch form: defaults kept, nothing timed")
     for st in rep.get("steps", []):
-        out.append(f"step {st.get('step', 0)} ({st.get('class', '')}): launch "
-                   f"{'covered' if st.get('launch', {}).get('covered') else 'NOT covered'}, "
-                   f"{st.get('launch', {}).get('workgroups', 0)} workgroups")
+        launch = st.get("launch", {})
+        out.append(f"step {st.get('step', 0)} ({st.get('class', '')}): launch {'covered' if launch.get('covered') else 'NOT covered'}" +
+                   (f", {launch['workgroups']} workgroups" if "workgroups" in launch else ""))
         out.append(f"  {'form':<6} {'identity':<11} {'U_run(ms)':<11} {'min(ms)':<10} status")
         for c in st.get("candidates", []):
             if c.get("admissible"):

@@ -268,21 +268,24 @@ EssentialWork essentialWork(const KernelModule& km) {
 }
 
 double peakOpsPerSec(const KernelModule& km, const Plan& plan) {
-    // MI355X datasheet (dense): f16 MFMA 2.5 PFLOP/s, f32 157.3 TFLOP/s,
-    // f64 78.6 TFLOP/s. A plan with an f16 GEMM is priced at the f16 rate,
-    // one touching only f64 buffers at the f64 rate, anything else at f32.
+    // MI355X datasheet (dense): i8 MFMA 5 POP/s, f16 2.5 PFLOP/s, f32 157.3
+    // TFLOP/s, f64 78.6 TFLOP/s. A plan with a product in 8 bits is priced at
+    // the i8 rate, one with an f16 GEMM or attention at the f16 rate, one
+    // touching only f64 buffers at the f64 rate, anything else at f32.
     bool allF64 = true;
     for (const KernelBuffer& b : km.buffers) {
         if (!b.isTemp && b.dtype != Dtype::F64) allF64 = false;
     }
+    bool half = false;
     for (const Step& st : plan.steps) {
+        if (st.kind == StepKind::MatmulI8) return 5.0e15;
         if ((st.kind == StepKind::Gemm && st.a != kInvalidId && km.buffers[st.a].dtype == Dtype::F16) ||
             st.kind == StepKind::ScoreSoftmax ||
             st.kind == StepKind::AttentionKv4 || (st.kind == StepKind::Attention && operatorDtype(km, st) != Dtype::F32)) {
-            return 2.5e15;
+            half = true;
         }
     }
-    return allF64 ? 78.6e12 : 157.3e12;
+    return half ? 2.5e15 : allF64 ? 78.6e12 : 157.3e12;
 }
 
 const MeasuredEnvironment& measuredEnvironment() {
@@ -311,7 +314,7 @@ std::string launchCoverage(const KernelModule& km, const Step& st, int64_t eleme
     // cover when the tile divides the extent (the launcher checks the same
     // divisibility and falls back to the bounds-checked general kernel).
     int64_t instances = 0, workgroups = 0, perGroup = 0;
-    bool covered = true;
+    bool covered = true, grid = true;
     const char* form = "";
     switch (st.kind) {
         case StepKind::Elementwise: {
@@ -448,9 +451,10 @@ std::string launchCoverage(const KernelModule& km, const Step& st, int64_t eleme
         case StepKind::StoreKv4:
         case StepKind::LoadKv4:
         case StepKind::AttentionKv4:
+            // Their grids go by addresses and, for the attention, run past what the
+            // lengths in the buffers need: none is given here.
             instances = operatorRows(st);
-            workgroups = instances;
-            perGroup = 1;
+            grid = false;
             form = "rows, by the sizes of the buffers";
             break;
         case StepKind::Fail:
@@ -458,7 +462,7 @@ std::string launchCoverage(const KernelModule& km, const Step& st, int64_t eleme
             break;
     }
     return "{\"form\":\"" + std::string(form) + "\",\"instances\":" + std::to_string(instances) +
-           ",\"workgroups\":" + std::to_string(workgroups) + ",\"per_workgroup\":" + std::to_string(perGroup) +
+           (grid ? ",\"workgroups\":" + std::to_string(workgroups) + ",\"per_workgroup\":" + std::to_string(perGroup) : std::string()) +
            ",\"covered\":" + (covered ? "true" : "false") + "}";
 }
 

@@ -71,3 +71,16 @@ class _Past8:
         b.ptr += 8
         b.elements -= 8
         return b
+
+
+# ------------------------------------------------------------------- search --
+def test_the_search_prices_them_and_claims_no_grid(hip):
+    # The declared rate is that of the fastest matrix instructions a plan runs on.
+    for km, rate in ((op.linear_i8_module(20, 30, 48, dtype="f32"), 5e15), (op.matmul_i8_module(20, 30, 48), 5e15),
+                     (op.attention_kv4_module(4, sequences=1, heads=2, kv_heads=1, dim=64, dtype="f32"), 2.5e15),
+                     (op.quantize_rows_module(20, 48), 157.3e12), (op.store_load_kv4_module(4, cache_rows=9, kv_heads=1, dim=64), 157.3e12)):
+        art = hip.build(km)
+        report = art.autotune({i: DeviceBuffer.from_array(np.zeros(km.buffers[i].dims), km.buffers[i].dtype) for i in km.bindable_ids()}, reps=2)
+        assert report["environment"]["declared_ops_per_sec"] == rate
+        for step in report["steps"]:
+            assert step["launch"]["covered"] and step["launch"]["instances"] > 0 and "workgroups" not in step["launch"], step["launch"]
