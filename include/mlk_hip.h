@@ -287,9 +287,9 @@ int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* bind
  * The following hold numbers in 8 and 4 bits: codes with an f32 scale each for
  * a row, or a row's head. A scale is the largest magnitude over the largest
  * code, rounded to f32, and the code is the one nearest to the exact x / scale,
- * half way to the even one. Rows of zeros have scale 0 and codes 0 (4-bit ones
- * keep the sign); a row or head with a value that is not finite has scale NaN
- * and codes 0.
+ * half way to the even one. Rows of zeros, or of numbers so small that their scale
+ * rounds to 0, have scale 0 and codes 0 (4-bit ones keep the sign); a row or head
+ * with a value that is not finite has scale NaN and codes 0.
  *
  * quantize_rows (operands x, codes_out, scale_out; attrs cols): rows of `cols`
  * elements of x, f16, bf16 or f32, as i8 codes from -127 to 127 and f32 scales
@@ -301,9 +301,9 @@ int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* bind
  * + bias[n] for n < cols. a [rows, inner] and b [cols, inner] are i8 and may
  * hold -128; scales and bias are f32; out is f16, bf16 or f32. Sums are exact
  * (inner <= 131071), times the scales in f32, of any sizes whose product with
- * them is in its range, rounded once to out. Rows and
- * cols <= 2^30. 8192^3 takes 0.45 ms, 4096^3 65 us; one row by 4096 x 4096 5.6, 64
- * by 8000 x 4096 13.7 (b from memory). Rows whose addresses or `inner` are no
+ * them is in its range, rounded once to out. Rows and cols <= 2^30. 8192^3 takes
+ * 0.46 ms, 4096^3 63 us; one row by 4096 x 4096 5.7, 64 by 8000 x 4096 12.8 (b
+ * from memory). Rows whose addresses or `inner` are no
  * multiples of 16 bytes are copied to aligned ones in the workspace first where
  * there are more than 64 (8191 x 4096 and the like: a read and a write of a and
  * b), and without a workspace run by 64 rows at a time without LDS, slower.
@@ -315,7 +315,8 @@ int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* bind
  * [rows, kv_heads], max |x| / 6. Byte i holds elements 2i, in its low half, and
  * 2i + 1; a code is a sign bit and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6. With
  * q_offsets the tokens from its last element on are left alone. Slots are meant
- * to differ: of tokens that name the same row, codes and scale of either remain.
+ * to differ: tokens that name the same row store there in no order, and a head may
+ * be left with the codes of one, or of both, and the scale of the other.
  * load_kv4 (k_codes, k_scale, v_codes, v_scale, k_out, v_out; slots; q_offsets;
  * the same attrs) reads such rows back, code times scale, rounded to the type;
  * a token whose slot lies outside the rows is left as it was. 8191 tokens of 8
@@ -329,13 +330,16 @@ int mlkhip_time_device_span(const mlkhip_artifact* a, const mlkhip_binding* bind
  * bf16 for bf16 rows, carried as two bf16 parts for f16 ones and three for f32
  * ones (half a step of itself, or 2^-134 where that is more), its sum and lse are
  * of f32 weights. The sums that have to stay in f32's range are attention's, with
- * codes times scales for keys and values. 32 single tokens
- * over 1000 to 8192 keys (32 heads on 8 of 128, bf16) take 51 us, 4 prompts of
- * 125 to 1000 tokens behind up to 4000 200 us. As attention's, its form and its
- * workspace follow the buffers' sizes; the matrix-core kernels take dims of
+ * codes times scales for keys and values. 32 single tokens over 1000 to 8192 keys
+ * (32 heads on 8 of 128, bf16) take 52 us, 4 prompts of 125 to 1000 tokens behind
+ * up to 4000 204 us. As attention's, its form and its workspace follow the
+ * buffers' sizes: a cache with room takes the form of long sequences (8 x 1000
+ * keys in a cache of 8 x 8192 rows 12.7 us, of 8 x 1000 10.2; 32 of them 17.6 and
+ * 11.4), and sequences that share rows that of short ones (8 over the same 8192
+ * keys 48 us, 24 with rows of their own). The matrix-core kernels take dims of
  * whole sixteens from 32 on, rows of q and out of whole 16-byte pieces, codes whose
- * rows start at 8 bytes and up to 4096 sequences, other Calls run a wave to a row (32 over up to 8192 keys at dim
- * 120: 5.2 ms; 2048 tokens: 8.7). */
+ * rows start at 8 bytes, and up to 4096 sequences; other Calls run a wave to a row
+ * (32 over up to 8192 keys at dim 120: 5.3 ms; 2048 tokens: 8.8). */
 
 /* ---- launch-form search (fastkernel on the gfx950 kernels) ------------ */
 /* The reference's fastkernel search (fastkernel/include/mlk/fastkernel/

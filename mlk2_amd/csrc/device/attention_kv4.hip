@@ -19,7 +19,7 @@ using mlk::spanOf;
 
 /// A query row in one wave, with any even dim, strides and alignment: a lane per
 /// key for the scores, then a lane per output column. 32 single tokens over 1000 to
-/// 8192 keys of dim 120 take 5.2 ms, 2048 tokens 8.7.
+/// 8192 keys of dim 120 take 5.3 ms, 2048 tokens 8.8.
 template <typename T>
 __global__ __launch_bounds__(256) void attentionKv4Rows(mlk::Kv4Args args) {
     const mlkd_attention& p = args.t.p;
@@ -130,18 +130,31 @@ Plan planOf(const mlkd_attention* p) {
     n.rows = each <= 16 ? 16 : 32;
     const int64_t blocks = p->sequences * ((each + n.rows - 1) / n.rows), most = rowBlocks(p, n.rows);
     // One wave a block needs no join of sums where there are blocks for all of them: 8 x
-    // 2048 tokens 395 us, by four waves 489; 8 x 512 over 4096 keys 329 and 346; 4 x 125
-    // to 1000 over up to 5000 242 and 200.
+    // 2048 tokens 412 us, by four waves 489; 8 x 512 over 4096 keys 329 and 346; 4 x 125
+    // to 1000 over up to 5000 242 and 204.
     n.waves = n.rows == 32 && blocks * p->kv_heads >= 4096 ? 1 : 4;
     n.units = most;
     // Dealt out by the keys, with a join, over the chip's room: three of four waves
-    // of 16 rows a unit or two of 32. That costs 6 to 10 us (more row blocks, more
-    // parts to join), and a block's keys take 5.5 to 6.5 us a thousand, so it pays
-    // where few blocks have many keys. Heads 32 on 8, dim 128, bf16, all of one
-    // length, whole and dealt: a token over 1024 keys 9.7 and 12.6 us, 2048 15.3 and
-    // 12.7, 8192 46.9 and 14.4; 8 over 2048 15.7 and 14.9; 32 over 4096 35.8 and 41.9;
-    // 32 over 1000 to 8192 59.6 and 50.4; 128 tokens over 1024 14.5 and 25.9, 4096 33.0
-    // and 34.0, 8192 57.1 and 43.2; twice 128 over 8192 59.6 and 67.0.
+    // of 16 rows a unit or two of 32. That costs 3 us for a sequence, 6 for 32 (more
+    // row blocks, more parts to join), and a block's keys take 5.5 us a thousand, so it
+    // pays where few blocks have many keys, or sequences unlike ones. Heads 32 on 8, dim
+    // 128, bf16, from memory, us whole and dealt; sequences by their keys, all of one
+    // length:
+    //   1 by 1024 9.8 12.8, 1500 13.2 13.1, 2048 15.9 13.1, 8192 48.0 14.4
+    //   8 by 1024 10.1 13.3, 2048 16.4 15.8, 4096 27.0 19.6, 8192 48.2 24.4
+    //   16 by 2048 16.5 18.3, 4096 27.1 23.3, 8192 61.5 43.3
+    //   32 by 2048 17.0 23.0, 4096 38.1 43.2, 8192 69.0 75.1, 16384 130 137
+    //   48 by 8192 122 105; 64 by 4096 68.4 75.2
+    // and of an eighth of that up to it:
+    //   16 by 8192 48.6 27.0; 32 by 4096 28.0 26.4, 8192 60.9 51.7, 16384 117 92.6
+    //   48 by 8192 102 74.1; 64 by 4096 55.5 55.3
+    // The lengths are not known here, only the buffer's rows: 32 sequences are dealt from
+    // 4500 rows each on, which costs equal ones 5 to 12 % and gains unlike ones 15 to 20,
+    // 48 and 64 never. A cache with room takes the form of its rows (8 x 1000 keys in 8
+    // x 8192 rows 12.7 for 10.2, 32 x 1000 in 32 x 8192 17.6 for 11.4), and sequences
+    // that share rows have fewer each than they read (8 over the same 8192 48.2 whole,
+    // 21.9 dealt). Prompts: 128 tokens over 1024 14.5 and 25.9, 4096 33.0 and 34.0, 8192
+    // 57.1 and 43.2; twice 128 over 8192 59.6 and 67.0.
     const int64_t room = (n.rows == 16 ? 768 : 512) / p->kv_heads;
     if (p->sequences <= 64 && keys * (room - 2 * blocks) >= 1500 * room) {
         n.units = std::max(room, most + 1);

@@ -167,7 +167,7 @@ struct Kv4Unit {
 /// Unit `unit` of `units`, which are dealt out by the keys there are: a sequence's
 /// row blocks are split into as many ranges, `parts` at most, as make all of them
 /// about equally long, so that all units of a launch run at once and end together
-/// (32 single tokens over 1000 to 8192 keys 50.4 us, whole 59.6). For 64 sequences at
+/// (32 single tokens over 1000 to 8192 keys 51.7 us, whole 60.9). For 64 sequences at
 /// most, a lane each, and more units than there are row blocks.
 template <int ROWS>
 __device__ __forceinline__ bool dealtUnit(const mlkd_attention& p, int group, int unit, int units, int parts, Kv4Unit& u) {
@@ -217,9 +217,10 @@ constexpr int kv4Waves(int dt, int rows) {
 /// scores of one query, so the softmax is register work but for one exchange of
 /// maxima. Prompts are bound by the wave's vector instructions and products, which
 /// overlap little (1700 cycles for 32 rows and keys of 128; 4 prompts of 125 to 1000
-/// tokens behind up to 4000, 32 heads on 8: 200 us, 0.70 PFLOP/s), single tokens by
-/// memory and the start (32 over 1000 to 8192 keys, 165 MB: 46 us, 3.5 TB/s; all of
-/// 8192: 4.8 TB/s whole). The products run on the codes as numbers, which either
+/// tokens behind up to 4000, 32 heads on 8: 204 us, 0.69 PFLOP/s, matrix units busy in
+/// 0.31 of the units' cycles), single tokens by memory and the start, 5 us to a first
+/// tile's sums (32 over 1000 to 8192 keys, 165 MB: 47 us; all of 8192, whole, 285 MB:
+/// 69, 4.1 TB/s). The products run on the codes as numbers, which either
 /// 16-bit type holds exactly: a key's scale goes to its scores, a value's to its
 /// weights. Codes come
 /// straight to LDS, two tiles ahead; a word of a key's row is eight elements of
