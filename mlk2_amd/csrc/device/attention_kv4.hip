@@ -42,7 +42,7 @@ __global__ __launch_bounds__(256) void attentionKv4Rows(mlk::Kv4Args args) {
         // A row's elements are taken at a size below 1, so that sums of them times codes
         // stay in range, and 2^lacks comes with the key's scale.
         const float size = waveMax(fmaxf(fmaxf(fabsf(q[0]), fabsf(q[1])), fmaxf(fabsf(q[2]), fabsf(q[3]))));
-        const int by = size < INFINITY ? __builtin_amdgcn_frexp_expf(size) : 0, lacks = by + args.up;
+        const int by = size < INFINITY ? __builtin_amdgcn_frexp_expf(size) : 0, lacks = by + args.up + __builtin_amdgcn_frexp_expf(args.codes) - 1;
 #pragma unroll
         for (int i = 0; i < 4; ++i) q[i] = __builtin_amdgcn_ldexpf(q[i], -by);
         auto query = [&](int c) { return lane(c < 64 ? q[0] : c < 128 ? q[1] : c < 192 ? q[2] : q[3], c & 63); };
@@ -200,8 +200,10 @@ mlk::Kv4Args argsOf(const mlkd_attention_kv4* p) {
     a.k_scale = p->k_scale;
     a.v_scale = p->v_scale;
     a.c = static_cast<float>(p->a.scale * 1.4426950408889634);
-    a.up = std::fabs(a.c) >= 2.0f ? std::ilogb(a.c) : 0;
-    a.c = std::ldexp(a.c, -a.up);
+    const int all = std::fabs(a.c) >= 2.0f ? std::ilogb(a.c) : 0, codes = std::min(all, 13);
+    a.c = std::ldexp(a.c, -all);
+    a.codes = std::ldexp(1.0f, codes);
+    a.up = all - codes;
     return a;
 }
 

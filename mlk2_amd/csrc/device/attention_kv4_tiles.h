@@ -21,23 +21,26 @@ struct Kv4Args {
     TileArgs t;                      // p's k and v: the codes, strides in bytes
     const float *k_scale, *v_scale;  // [kv_rows, kv_heads]
     int units;                       // row blocks, or with parts their key ranges, of one head at most
-    float c;                         // scale log2 e = c 2^up, c below 2 in size: a key's scale times c is in range,
-    int up;                          // and the queries take 2^up
+    // scale log2 e = c codes 2^up, c below 2 in size, so that a key's scale times c is in
+    // range: the keys' codes are taken times `codes`, 2^13 at most, the queries times 2^up.
+    float c, codes;
+    int up;
 };
 
-/// The numbers of a word's eight codes, exact in either type.
+/// The numbers of a word's eight codes times a power of two, exact in either type (f16:
+/// up to 2^13).
 template <typename T>
-__device__ __forceinline__ Piece<T> numbers(int word);
+__device__ __forceinline__ Piece<T> numbers(int word, float by);
 template <>
-__device__ __forceinline__ Piece<__bf16> numbers<__bf16>(int word) {
-    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, 1.0f, 1),
-                 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, 1.0f, 3);
+__device__ __forceinline__ Piece<__bf16> numbers<__bf16>(int word, float by) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, by, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, by, 1),
+                 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, by, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, by, 3);
     return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 template <>
-__device__ __forceinline__ Piece<_Float16> numbers<_Float16>(int word) {
-    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 1),
-                c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, 1.0f, 3);
+__device__ __forceinline__ Piece<_Float16> numbers<_Float16>(int word, float by) {
+    const f16x2 a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, by, 0), b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, by, 1),
+                c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, by, 2), d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(word, by, 3);
     return __builtin_shufflevector(__builtin_shufflevector(a, b, 0, 1, 2, 3), __builtin_shufflevector(c, d, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
@@ -130,9 +133,9 @@ struct Kv4Tiles {
     static constexpr int kLds = NW * (kRing > kJoin ? kRing : kJoin);
     static_assert(kPerTile * (kStages - 1) <= 63, "the loads waited on by number fit the counter");
     // Exponents between which a row's largest query is left as it is: sums of 256 of
-    // them times 6 stay in f32's range, and the last of three bf16 parts in bf16's. f16
-    // itself holds less.
-    static constexpr int kLeast = std::is_same_v<T, _Float16> ? -24 : -60, kMost = std::is_same_v<T, _Float16> ? 16 : 100;
+    // them times 6 2^13 stay in f32's range, and the last of three bf16 parts in bf16's.
+    // f16 itself holds less.
+    static constexpr int kLeast = std::is_same_v<T, _Float16> ? -24 : -60, kMost = std::is_same_v<T, _Float16> ? 16 : 103;
 
     /// Turn of row j's pieces, so that the rows that are read at a time lie in
     /// different banks: 16 from one on, or fours of them eight or sixteen apart.
@@ -427,7 +430,7 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT, ROWS)) void attentionKv4Ti
             words(tile, kb, w);
 #pragma unroll
             for (int i = 0; i < KS; ++i) {
-                const Piece<Q> k = numbers<Q>(w[i]);
+                const Piece<Q> k = numbers<Q>(w[i], args.codes);
 #pragma unroll
                 for (int b = 0; b < QB; ++b) {
 #pragma unroll
@@ -502,7 +505,7 @@ __global__ __launch_bounds__(NW * 64, kv4Waves<T>(DT, ROWS)) void attentionKv4Ti
             for (int n = 0; n < 2; ++n) {
                 // Of 32 columns a read's halves are those of the first and the second
                 // eight keys, of 16 those of two blocks of columns.
-                const Piece<__bf16> vv = numbers<__bf16>(v[n]);
+                const Piece<__bf16> vv = numbers<__bf16>(v[n], 1.0f);
                 const int block = EDGE == 32 ? i : 2 * i + n, keys = EDGE == 32 ? n : 0;
 #pragma unroll
                 for (int b = 0; b < QB; ++b) {

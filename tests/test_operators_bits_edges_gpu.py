@@ -84,6 +84,46 @@ def test_scales_far_from_one(hip, dtype, d, shape, scale, size_q, size_k):
         close(got["out"][0], out[0], bound[0], "out")
 
 
+def scores_about_one(hip, dtype, d, shape, scale, size_q, size_k, seed):
+    h, g, q_lens, k_lens = SHAPES[shape]
+    rng = np.random.default_rng(seed)
+    t, rows = sum(q_lens), sum(k_lens)
+    q = rounded(rng.standard_normal((t, h, d)).clip(-1.9, 1.9) * size_q, dtype)
+    k_codes, k_scale, k = heads_of((rng.standard_normal((rows, g, d)).clip(-3, 3) * size_k).astype(np.float32).astype(np.float64))
+    v_codes, v_scale, v = heads_of(rounded(rng.standard_normal((rows, g, d)), "bf16"))
+    offsets, start = np.concatenate([[0], np.cumsum(q_lens)]), np.concatenate([[0], np.cumsum(k_lens)[:-1]])
+    km = op.attention_kv4_module(t, kv_rows=rows, sequences=len(q_lens), heads=h, kv_heads=g, dim=d, dtype=dtype, scale=scale, lse=True)
+    got = run(hip, km, {"q": q, "k_codes": k_codes, "k_scale": k_scale, "v_codes": v_codes, "v_scale": v_scale, "q_offsets": offsets,
+                        "kv_start": start, "kv_len": k_lens})
+    out, bound, lse, lse_bound, _ = attention(q, k, v, offsets, start, k_lens, scale=scale, causal=True, dtype=dtype)
+    close(got["out"], out, bound, "out")
+    close(got["lse"], lse, lse_bound, "lse")
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 96, 128, 256, 34])
+@pytest.mark.parametrize("shape", ["token", "prompt"])
+def test_every_power_of_a_scale(hip, dtype, d, shape):
+    # Past 2^13 / log2 e the codes' factor ends and the queries take the rest.
+    for n in list(range(-2, 16)) + [20, 40, 60]:
+        scale = 1.3 * 2.0 ** n * (-1) ** n
+        size_q = 2.0 ** -(n // 2) if dtype == "f16" else 1.0
+        scores_about_one(hip, dtype, d, shape, scale, size_q if n < 20 else 0.01, 1 / (abs(scale) * d ** 0.5 * (size_q if n < 20 else 0.01)), n + 9)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("shape", ["token", "prompt"])
+@pytest.mark.parametrize("scale", [None, 8000.0, 30000.0])
+def test_queries_of_every_size(hip, dtype, d, shape, scale):
+    # Sizes around those from which a row is taken times a power of two.
+    scale = scale or d ** -0.5
+    for e in (-125, -100, -65, -61, -60, -59, -30, 30, 55, 57, 59, 60, 61, 99, 100, 101, 103, 104, 105, 115, 117, 125):
+        size_k = 2.0 ** -e / (scale * d ** 0.5)
+        if 1e-43 < size_k < 1e37:
+            scores_about_one(hip, dtype, d, shape, scale, 2.0 ** e, size_k, e + 200)
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 128, 256, 34])
 @pytest.mark.parametrize("shape", ["token", "ranges", "prompt"])
