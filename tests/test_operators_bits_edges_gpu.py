@@ -4,9 +4,10 @@ import numpy as np
 import pytest
 
 from mlk2_amd import operators as op
-from operators_bits_ref import load_kv4, store_kv4
+from mlk2_amd.kernel_ir import KernelBuffer, KernelModule
+from operators_bits_ref import load_bound, load_kv4, store_kv4
 from operators_ref import TINY, U, U32, attention, rounded
-from test_operators_gpu import TYPES, close, run
+from test_operators_gpu import KEEP, TYPES, close, run
 
 pytestmark = pytest.mark.gpu
 
@@ -240,3 +241,85 @@ def test_matmul_sums_of_zero_under_any_scale(hip, m, n, k):
     for size in (3e38, 1e-45):
         got = run(hip, op.matmul_i8_module(m, n, k, dtype="f32"), {"a": a, "b": b, "a_scale": np.full(m, size), "b_scale": np.full(n, 3e38)})["out"]
         assert (got == 0).all()
+
+
+# ---------------------------------------------------------- buffers, lengths --
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128, 34])
+@pytest.mark.parametrize("rows", [300, 9000])
+def test_offsets_and_lengths_are_clipped(hip, dtype, d, rows):
+    # Offsets and lengths outside the buffers, and below 0: what lies in them counts.
+    h, g, t = 4, 2, 50
+    offsets = [-5, 20, 21, 21, 45, 2 ** 31 - 1]
+    start, lens = [rows - 100, -1, 7, rows, 0], [2 ** 31 - 1, 50, 40, 3, -9]
+    for offsets, start, lens in ((offsets, start, lens), ([0, 10, 20, 30, 40, 50], [0, rows - 1, 2 ** 31 - 1, -2 ** 31, 5], [rows + 1, 2, 1, 2 ** 31 - 1, 1])):
+        rng = np.random.default_rng(d)
+        q = rounded(rng.standard_normal((t, h, d)), dtype)
+        k_codes, k_scale, k = heads_of(rounded(rng.standard_normal((rows, g, d)), "bf16"))
+        v_codes, v_scale, v = heads_of(rounded(rng.standard_normal((rows, g, d)), "bf16"))
+        km = op.attention_kv4_module(t, kv_rows=rows, sequences=5, heads=h, kv_heads=g, dim=d, dtype=dtype, lse=True)
+        got = run(hip, km, {"q": q, "k_codes": k_codes, "k_scale": k_scale, "v_codes": v_codes, "v_scale": v_scale, "q_offsets": offsets,
+                            "kv_start": start, "kv_len": lens})
+        held = [max(0, min(rows - s, n)) if 0 <= s < rows else 0 for s, n in zip(start, lens)]
+        out, bound, lse, lse_bound, written = attention(q, k, v, np.clip(offsets, 0, t), [s if n > 0 else 0 for s, n in zip(start, held)], held,
+                                                        scale=d ** -0.5, causal=True, dtype=dtype)
+        assert written.all()
+        close(got["out"], out, bound, "out")
+        real = np.isfinite(lse)
+        close(got["lse"][real], lse[real], lse_bound[real], "lse")
+        assert (got["lse"][~real] == -np.inf).all() and not real.all()
+
+
+@pytest.mark.parametrize("build", [lambda: op.quantize_rows_module(0, 8), lambda: op.matmul_i8_module(0, 8, 16), lambda: op.linear_i8_module(0, 8, 16),
+                                   lambda: op.store_load_kv4_module(0, cache_rows=9, kv_heads=2, dim=64), lambda: op.store_kv4_module(0, kv_heads=2, dim=64),
+                                   lambda: op.attention_kv4_module(0, kv_rows=4000, sequences=1, heads=4, kv_heads=2, dim=64, lse=True)])
+def test_no_rows(hip, build):
+    km = build()
+    host = {b.name: np.zeros(b.dims) for b in km.buffers if b.is_input}
+    got = run(hip, km, {**host, **{b.name: np.full(b.dims, 9) for b in km.buffers if b.name.endswith("codes")}})
+    for name, a in got.items():
+        assert (a == (9 if name.endswith("codes") else KEEP)).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_an_empty_cache(hip, dtype):
+    # A cache of no rows: nothing is stored or loaded, and queries see no keys.
+    t, h, g, d = 5, 4, 2, 64
+    x = np.ones((t, g, d))
+    got = run(hip, op.store_load_kv4_module(t, cache_rows=0, kv_heads=g, dim=d, dtype=dtype), {"k": x, "v": x, "slots": np.arange(t)})
+    assert (got["k_read"] == KEEP).all() and (got["v_read"] == KEEP).all()
+    empty = {f"{p}_{w}": np.zeros((0, g, d // 2) if w == "codes" else (0, g)) for p in "kv" for w in ("codes", "scale")}
+    km = op.attention_kv4_module(t, kv_rows=0, sequences=2, heads=h, kv_heads=g, dim=d, dtype=dtype, lse=True)
+    got = run(hip, km, {"q": np.ones((t, h, d)), "q_offsets": [0, 2, 4], "kv_start": [0, 0], "kv_len": [3, 0], **empty})
+    assert (got["out"][:4] == 0).all() and (got["lse"][:4] == -np.inf).all() and (got["out"][4:] == KEEP).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("d,extra", [(64, 0), (64, 8), (80, 8), (128, 3)])
+def test_keys_and_values_in_one_buffer(hip, dtype, d, extra):
+    # Codes of k and v as columns of one buffer's rows, `extra` bytes behind them;
+    # attended, and read back.
+    h, g, rows, lens = 4, 2, 500, [90, 400]
+    rng = np.random.default_rng(d + extra)
+    q = rounded(rng.standard_normal((41, h, d)), dtype)
+    both = [heads_of(rounded(rng.standard_normal((rows, g, d)), "bf16")) for _ in "kv"]
+    part, width = g * d // 2, g * d + extra
+    codes = np.full((rows, width), 255)
+    codes[:, :part], codes[:, part:2 * part] = (b[0].reshape(rows, part) for b in both)
+    km = KernelModule(name="one buffer")
+
+    def buf(name, kind, dims, out=False):
+        return km.add_buffer(KernelBuffer(name, kind, is_input=not out, is_output=out, elements=int(np.prod(dims)), dims=list(dims)))
+
+    cache = buf("codes", "u8", [rows, width])
+    ids = {"k_codes": cache, "v_codes": cache, "k_scale": buf("k_scale", "f32", [rows, g]), "v_scale": buf("v_scale", "f32", [rows, g])}
+    at = {"v_codes": part}
+    sides = {"q": buf("q", dtype, [41, h, d]), "q_offsets": buf("q_offsets", "i32", [3]), "kv_start": buf("kv_start", "i32", [2]),
+             "kv_len": buf("kv_len", "i32", [2]), "out": buf("out", dtype, [41, h, d], True)}
+    op.add_attention_kv4(km, {**ids, **sides}, heads=h, kv_heads=g, dim=d, columns=at)
+    op.add_load_kv4(km, {**ids, "k_out": buf("k", dtype, [rows, g, d], True), "v_out": buf("v", dtype, [rows, g, d], True)}, kv_heads=g, dim=d, columns=at)
+    got = run(hip, km, {"codes": codes, "k_scale": both[0][1], "v_scale": both[1][1], "q": q, "q_offsets": [0, 40, 41], "kv_start": [3, 100], "kv_len": lens})
+    out, bound, *_ = attention(q, both[0][2], both[1][2], [0, 40, 41], [3, 100], lens, scale=d ** -0.5, causal=True, dtype=dtype)
+    close(got["out"], out, bound, "out")
+    for name, (_, _, want) in zip("kv", both):
+        close(got[name], want, load_bound(want, dtype), name)
