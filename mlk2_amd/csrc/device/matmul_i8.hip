@@ -449,8 +449,8 @@ __global__ __launch_bounds__(256) void matmulI8Join(TileArgs args) {
 // --------------------------------------------------------------- launch ----
 enum Form { kFew, kTile64, kTile128x64, kTile128, kTile256 };
 
-/// A tile's rows and columns, and what a round of 256 of them, one a unit, adds to
-/// the time of k = 4096, in halves of a microsecond.
+/// A tile's rows and columns, what a round of 256 of them, one a unit, adds to the time
+/// of k = 4096, in halves of a microsecond, and its threads.
 struct TileSize {
     int rows, cols, round, threads;
 };
